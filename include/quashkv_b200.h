@@ -344,6 +344,94 @@ int qkv_attention_tiled(const void* q, int q_dtype, qkv_tiled_cache_t cache,
                         const float* S, float qjl_scale, float scale, int causal,
                         float* out, void* workspace, size_t workspace_bytes, void* stream);
 
+/* ---- pages of 8-bit codes -------------------------------------------------------------------------
+ * A cache in the form that serving engines use beside the compressed one: per (block, KV head) block_size
+ * tokens of d codes for keys and for values and one fp32 scale for each; coordinate = code * scale.  No
+ * rotation, no tables.  The reference has no such storage (its page manager stops at integrations/
+ * vllm_backend.py:82-195).
+ *   codes    QKV_E4M3 (at most 448) or QKV_INT8 (-127 .. 127)
+ *   strides  bytes from one block, head, token to the next (any order of heads and tokens in memory);
+ *            the d bytes of a token are contiguous; base and strides multiples of 16
+ *   scales   strides in elements from one block, head to the next
+ *   d 32, 64, 96 or 128; block_size a multiple of 16 */
+enum { QKV_E4M3 = 0, QKV_INT8 = 1 };
+typedef struct {
+  uint8_t* k_codes;
+  uint8_t* v_codes;
+  float* k_scales;
+  float* v_scales;
+  int64_t k_stride[3];
+  int64_t v_stride[3];
+  int64_t ks_stride[2];
+  int64_t vs_stride[2];
+  int64_t num_blocks;
+  int Hkv;
+  int block_size;
+  int d;
+  int code;
+} qkv_pages8_t;
+
+/* Quantises keys and values into pages.  Token t of sequence i (of n_seq with `tokens` each) and head h is
+ * the d contiguous elements at i * strides[0] + t * strides[1] + h * strides[2]; base and strides multiples
+ * of 16 bytes.  It goes to slot block * block_size + offset: slots[t] (n_seq = 1; a negative slot drops the token), or,
+ * with slots == NULL, to position start_lens[i] + t of the pages in row i of block_table.  A position outside
+ * the table or in a block with a negative number, and a slot outside the pool, are dropped and counted
+ * (qkv_dropped_paged8_tokens).
+ *   A run (consecutive tokens with consecutive slots inside one page) takes the least power of two s (at
+ *   least 2^-120) with every |x| <= (largest code) * s.  Where it begins the page (offset 0) the page's scale becomes
+ *   s, else the larger of s and the old one, and the codes in front of the run are rounded to the new scale.  Codes
+ *   are round(x * (1 / scale)), ties to even.  All zeros give scale 0; an infinity or NaN gives the scale NaN and codes 0.
+ * The tokens of one page form one run: two runs of one call in the same page (a slot listed twice among
+ * them) leave it with either's scale; nothing outside that page and head is touched. */
+int qkv_append_paged8(const void* keys, const void* values, int dtype, const int64_t* key_strides,
+                      const int64_t* value_strides, int64_t n_seq, int64_t tokens, qkv_pages8_t pages,
+                      const int64_t* slots, const int32_t* block_table, int64_t table_stride, int max_blocks,
+                      const int32_t* start_lens, void* stream);
+/* (Token, head) pairs that appends on the current device have dropped since the library was loaded.  Waits
+ * for the device. */
+int64_t qkv_dropped_paged8_tokens(void);
+
+/* Attention over pages of 8-bit codes: softmax(scale * q k^T) v in fp32, one rounding to the queries' type.
+ *   q          query head h reads KV head h / (Hq / Hkv); element strides of (sequence, token, head); d
+ *              contiguous elements; base and strides multiples of 16 bytes; out likewise, of q's dtype
+ *   dense      query_starts == NULL: q_len tokens of every sequence
+ *   ragged     tokens query_starts[i] .. query_starts[i+1]-1 (of total_q) are sequence i's, q_len the most of
+ *              any (tokens beyond it are not attended); strides[0] is not used; rows of no sequence are left as
+ *              they were
+ *   seq_lens   tokens held, clamped to max_kv_len and to the table; a block number outside the pool hides
+ *              its tokens; bytes behind the last token may be anything; codes within hold no NaN
+ *   causal     query token t of n sits at position seq_lens[i] - n + t and sees positions up to its own
+ * A row that sees nothing is zeros.  Any scales, 0 and NaN among them: NaN reaches what sees its page.
+ * Workspace: qkv_attention_paged8_workspace_bytes(...) bytes, 16-byte aligned. */
+size_t qkv_attention_paged8_workspace_bytes(int n_seq, int Hq, int Hkv, int q_len, int64_t max_kv_len, int d, int q_dtype);
+int qkv_attention_paged8(const void* q, int q_dtype, const int64_t* q_strides, qkv_pages8_t pages,
+                         const int32_t* block_table, int64_t table_stride, int max_blocks, const int32_t* seq_lens,
+                         const int32_t* query_starts, int64_t total_q, int n_seq, int Hq, int q_len, int64_t max_kv_len,
+                         float scale, int causal, void* out, const int64_t* out_strides, void* workspace,
+                         size_t workspace_bytes, void* stream);
+
+/* ---- block tables and slots on the device ----------------------------------------------------------------
+ * A pool's bookkeeping as device memory: a block table of max_blocks entries a sequence (table_stride apart),
+ * tokens held (seq_lens), a stack of free blocks (n_free_pages entries, the first pool[0] of them free) and
+ * pool[1], the tokens that found no place so far (it stops at 2^31 - 1).
+ * qkv_extend_pages takes new_lens[i] more tokens for every sequence: blocks come off the top of the stack in
+ * the order of the sequences and are entered in the table behind the ceil(seq_lens[i] / block_size) that a
+ * sequence has; slots[t] (of max_tokens) is block * block_size + offset of new token t, the sequences' tokens one
+ * after the other, -1 behind them and for tokens that found no place (stack empty, row of the table full);
+ * query_starts (n_seq + 1) are the exclusive sums of new_lens, none above max_tokens; seq_lens_out and pool_out
+ * may be seq_lens and pool; start_lens_out (may be NULL) gets the lengths before.
+ * qkv_shrink_pages keeps the first min(keep_lens[i], seq_lens[i]) tokens and puts the blocks behind them back; after an
+ * extend it restores the stack.  In place.
+ * n_seq up to QKV_PAGES_MAX_SEQS; negative lengths count as 0. */
+#define QKV_PAGES_MAX_SEQS 16384
+int qkv_extend_pages(int32_t* block_table, int64_t table_stride, int max_blocks, const int32_t* seq_lens,
+                     const int32_t* new_lens, const int32_t* free_pages, int64_t n_free_pages, const int32_t* pool,
+                     int n_seq, int block_size, int64_t max_tokens, int64_t* slots, int32_t* query_starts,
+                     int32_t* seq_lens_out, int32_t* start_lens_out, int32_t* pool_out, void* stream);
+int qkv_shrink_pages(const int32_t* block_table, int64_t table_stride, int max_blocks, int32_t* seq_lens,
+                     const int32_t* keep_lens, int32_t* free_pages, int64_t n_free_pages, int32_t* pool, int n_seq,
+                     int block_size, void* stream);
+
 /* ---- index scan ------------------------------------------------------------------------------
  * Replaces QuashIndex.search (reference nn_search/index.py:121-163):
  * score[m,n] = norm_n * (q_rot_m . c[code_n] + qjl_scale * sum(|q_rot_m| * S * (2*sign_n-1))),

@@ -49,7 +49,15 @@ class KvDest(C.Structure):
                 ("max_blocks", _i), ("block_size", _i)]
 
 
+class Pages8(C.Structure):
+    """qkv_pages8_t: pages of 8-bit codes, their strides (bytes; block, head, token) and their scales' (elements)."""
+    _fields_ = [("k_codes", _vp), ("v_codes", _vp), ("k_scales", _vp), ("v_scales", _vp), ("k_stride", _i64 * 3),
+                ("v_stride", _i64 * 3), ("ks_stride", _i64 * 2), ("vs_stride", _i64 * 2), ("num_blocks", _i64),
+                ("Hkv", _i), ("block_size", _i), ("d", _i), ("code", _i)]
+
+
 TILE_TOKENS, TILE_BYTES = 16, 1664
+PAGES_MAX_SEQS = 16384
 
 # symbol -> (restype, argtypes); every symbol include/quashkv_b200.h declares is listed here
 SIGNATURES = {
@@ -80,6 +88,13 @@ SIGNATURES = {
     "qkv_append_kv": (_i, [_vp, _i, _vp, _i, _i, _i, _i64, _i, _vp, _vp, _vp, _vp, _i, _vp, _i, KvDest, _vp, _sz, _vp]),
     "qkv_dropped_append_rows": (_i64, []),
     "qkv_scatter_rows": (_i, [_vp, _vp, _vp, _i64, _i, _vp]),
+    "qkv_append_paged8": (_i, [_vp, _vp, _i, C.POINTER(_i64), C.POINTER(_i64), _i64, _i64, Pages8, _vp, _vp, _i64, _i, _vp, _vp]),
+    "qkv_dropped_paged8_tokens": (_i64, []),
+    "qkv_attention_paged8_workspace_bytes": (_sz, [_i, _i, _i, _i, _i64, _i, _i]),
+    "qkv_attention_paged8": (_i, [_vp, _i, C.POINTER(_i64), Pages8, _vp, _i64, _i, _vp, _vp, _i64, _i, _i, _i, _i64, _f, _i,
+                                  _vp, C.POINTER(_i64), _vp, _sz, _vp]),
+    "qkv_extend_pages": (_i, [_vp, _i64, _i, _vp, _vp, _vp, _i64, _vp, _i, _i, _i64, _vp, _vp, _vp, _vp, _vp, _vp]),
+    "qkv_shrink_pages": (_i, [_vp, _i64, _i, _vp, _vp, _vp, _i64, _vp, _i, _i, _vp]),
     "qkv_index_workspace_bytes": (_sz, [_i64, _i, _i, _i]),
     "qkv_index_scan_topk": (_i, [_vp, _i, _i, _vp, _vp, _vp, _i64, _i, _vp, _vp, _vp, _f, _i, _i64, _vp, _vp,
                                  _vp, _sz, _vp]),

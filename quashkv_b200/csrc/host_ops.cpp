@@ -28,7 +28,8 @@ using OptTensor = std::optional<Tensor>;
 #define QKV_FOR_EACH_ENTRY(X)                                                                                     \
   X(qkv_strerror) X(qkv_compress_mse) X(qkv_compress_ip) X(qkv_compress_mixed) X(qkv_mixed_row_bytes)             \
   X(qkv_decompress) X(qkv_decompress_mixed) X(qkv_attention_workspace_bytes) X(qkv_attention)                     \
-  X(qkv_attention_paged) X(qkv_attention_tiled) X(qkv_append_workspace_bytes) X(qkv_append_kv) X(qkv_index_workspace_bytes) X(qkv_index_scan_topk)
+  X(qkv_attention_paged) X(qkv_attention_tiled) X(qkv_append_workspace_bytes) X(qkv_append_kv) X(qkv_index_workspace_bytes) X(qkv_index_scan_topk) \
+  X(qkv_append_paged8) X(qkv_attention_paged8_workspace_bytes) X(qkv_attention_paged8) X(qkv_extend_pages) X(qkv_shrink_pages)
 
 struct Api {
 #define QKV_MEMBER(name) decltype(&::name) name = nullptr;
@@ -394,6 +395,199 @@ Tensor attention_tiled(const Tensor& q, const Tensor& records, int64_t capacity,
   return out;
 }
 
+// ---- pages of 8-bit codes ------------------------------------------------------------------------------------------
+
+// (blocks, Hkv, block_size, d) codes, a view of any order in memory whose tokens are contiguous, and (blocks, Hkv) scales.
+qkv_pages8_t pages8(const Tensor& k_codes, const Tensor& v_codes, const Tensor& k_scales, const Tensor& v_scales) {
+  TORCH_CHECK_VALUE(k_codes.dim() == 4 && k_codes.sizes() == v_codes.sizes() && k_codes.scalar_type() == v_codes.scalar_type(),
+                    "quashkv_b200: key and value codes of shape (num_blocks, kv_heads, block_size, head_size) and one type, got ",
+                    k_codes.sizes(), " and ", v_codes.sizes());
+  TORCH_CHECK_VALUE(k_codes.scalar_type() == at::kFloat8_e4m3fn || k_codes.scalar_type() == at::kChar,
+                    "quashkv_b200: codes are float8_e4m3fn or int8, got ", k_codes.scalar_type());
+  TORCH_CHECK_VALUE(k_codes.stride(3) == 1 && v_codes.stride(3) == 1, "quashkv_b200: the codes of a token must be contiguous");
+  const at::IntArrayRef head = k_codes.sizes().slice(0, 2);
+  TORCH_CHECK_VALUE(k_scales.scalar_type() == at::kFloat && v_scales.scalar_type() == at::kFloat && k_scales.sizes() == head && v_scales.sizes() == head,
+                    "quashkv_b200: fp32 scales of shape ", head, " (num_blocks, kv_heads)");
+  qkv_pages8_t p{};
+  p.k_codes = static_cast<uint8_t*>(k_codes.data_ptr());
+  p.v_codes = static_cast<uint8_t*>(v_codes.data_ptr());
+  p.k_scales = fpm(k_scales);
+  p.v_scales = fpm(v_scales);
+  for (int i = 0; i < 3; ++i) {
+    p.k_stride[i] = k_codes.stride(i);
+    p.v_stride[i] = v_codes.stride(i);
+  }
+  for (int i = 0; i < 2; ++i) {
+    p.ks_stride[i] = k_scales.stride(i);
+    p.vs_stride[i] = v_scales.stride(i);
+  }
+  p.num_blocks = k_codes.size(0);
+  p.Hkv = static_cast<int>(k_codes.size(1));
+  p.block_size = static_cast<int>(k_codes.size(2));
+  p.d = static_cast<int>(k_codes.size(3));
+  p.code = k_codes.scalar_type() == at::kChar ? QKV_INT8 : QKV_E4M3;
+  return p;
+}
+
+// Rows of the last dimension contiguous, everything on 16-byte boundaries: as the caller has it, else a copy.
+Tensor rows16(const Tensor& t) {
+  const int64_t unit = 16 / t.element_size();
+  bool ok = t.stride(-1) == 1 && reinterpret_cast<uintptr_t>(t.const_data_ptr()) % 16 == 0;
+  for (int64_t i = 0; i + 1 < t.dim(); ++i) ok = ok && (t.size(i) <= 1 || (t.stride(i) >= 0 && t.stride(i) % unit == 0));
+  if (ok) return t;
+  return t.contiguous().data_ptr() == t.data_ptr() ? t.clone() : t.contiguous();
+}
+int64_t stride16(const Tensor& t, int64_t dim) { return t.size(dim) <= 1 ? 0 : t.stride(dim); }
+
+// A block table (n, max_blocks) whose rows may be part of wider ones, and lengths (n): int32.
+void check_table(const Tensor& table, const Tensor& lens) {
+  TORCH_CHECK_VALUE(table.dim() == 2 && table.scalar_type() == at::kInt && lens.scalar_type() == at::kInt && lens.dim() == 1 && lens.size(0) == table.size(0),
+                    "quashkv_b200: an int32 block table (n_seq, max_blocks) and int32 lengths (n_seq), got ", table.sizes(), " and ", lens.sizes());
+}
+Tensor table_rows(const Tensor& t) { return t.stride(1) == 1 && t.stride(0) >= t.size(1) ? t : t.contiguous(); }
+const int32_t* ip(const Tensor& t) { return static_cast<const int32_t*>(t.const_data_ptr()); }
+
+// keys, values (tokens, Hkv, d) with slots (tokens), or (n_seq, Hkv, tokens, d) with a block table and start lengths.
+void append_paged8(const Tensor& keys_in, const Tensor& values_in, Tensor k_codes, Tensor v_codes, Tensor k_scales, Tensor v_scales,
+                   const OptTensor& slots_in, const OptTensor& table_in, const OptTensor& starts_in) {
+  const at::Device dev = keys_in.device();
+  Call call(dev);
+  same_device(dev, {&values_in, &k_codes, &v_codes, &k_scales, &v_scales, slots_in ? &*slots_in : nullptr,
+                    table_in ? &*table_in : nullptr, starts_in ? &*starts_in : nullptr});
+  const qkv_pages8_t pages = pages8(k_codes, v_codes, k_scales, v_scales);
+  const bool flat = slots_in.has_value();
+  TORCH_CHECK_VALUE(keys_in.sizes() == values_in.sizes() && keys_in.scalar_type() == values_in.scalar_type() && keys_in.dim() == (flat ? 3 : 4) &&
+                    keys_in.size(1) == pages.Hkv && keys_in.size(-1) == pages.d,
+                    "quashkv_b200: keys and values of one type and shape ", flat ? "(tokens, " : "(n_seq, ", pages.Hkv, flat ? ", " : ", tokens, ", pages.d,
+                    "), got ", keys_in.sizes(), " and ", values_in.sizes());
+  if (slots_in) {
+    TORCH_CHECK_VALUE(slots_in->scalar_type() == at::kLong && slots_in->dim() == 1 && slots_in->size(0) == keys_in.size(0),
+                      "quashkv_b200: int64 slots for ", keys_in.size(0), " tokens, got ", slots_in->sizes());
+  } else {
+    TORCH_CHECK_VALUE(table_in.has_value() && starts_in.has_value(), "quashkv_b200: slots, or a block table and start lengths");
+    check_table(*table_in, *starts_in);
+    TORCH_CHECK_VALUE(table_in->size(0) == keys_in.size(0), "quashkv_b200: a block table for ", keys_in.size(0), " sequences, got ", table_in->sizes());
+  }
+  if (keys_in.numel() == 0) return;
+  const Tensor keys = rows16(dtype_code(keys_in) < 0 ? keys_in.to(at::kFloat) : keys_in);
+  const Tensor values = rows16(dtype_code(values_in) < 0 ? values_in.to(at::kFloat) : values_in);
+  int64_t ks[3], vs[3];
+  const int64_t dims[2][3] = {{-1, 0, 1}, {0, 2, 1}};      // sequence, token, head
+  for (int i = 0; i < 3; ++i) {
+    const int64_t dim = dims[flat ? 0 : 1][i];
+    ks[i] = dim < 0 ? 0 : stride16(keys, dim);
+    vs[i] = dim < 0 ? 0 : stride16(values, dim);
+  }
+  if (flat) {
+    const Tensor slots = slots_in->contiguous();
+    check(api.qkv_append_paged8(keys.const_data_ptr(), values.const_data_ptr(), dtype_code(keys), ks, vs, 1, keys.size(0), pages,
+                                static_cast<const int64_t*>(slots.const_data_ptr()), nullptr, 0, 0, nullptr, call.stream), "append_paged8");
+    return;
+  }
+  const Tensor table = table_rows(*table_in), starts = starts_in->contiguous();
+  check(api.qkv_append_paged8(keys.const_data_ptr(), values.const_data_ptr(), dtype_code(keys), ks, vs, keys.size(0), keys.size(2), pages,
+                              nullptr, ip(table), table.stride(0), static_cast<int>(table.size(1)), ip(starts), call.stream), "append_paged8");
+}
+
+// queries (n_seq, Hq, q_len, d), or (tokens, Hq, d) with query_starts (n_seq + 1); the result has their shape and type.
+Tensor attention_paged8(const Tensor& q_in, const Tensor& k_codes, const Tensor& v_codes, const Tensor& k_scales, const Tensor& v_scales,
+                        const Tensor& table_in, const Tensor& lens_in, int64_t max_kv_len, const OptTensor& starts_in, int64_t max_q_len,
+                        double scale, bool causal) {
+  const at::Device dev = q_in.device();
+  Call call(dev);
+  same_device(dev, {&k_codes, &v_codes, &k_scales, &v_scales, &table_in, &lens_in, starts_in ? &*starts_in : nullptr});
+  const qkv_pages8_t pages = pages8(k_codes, v_codes, k_scales, v_scales);
+  check_table(table_in, lens_in);
+  const bool ragged = starts_in.has_value();
+  const int64_t n = table_in.size(0);
+  TORCH_CHECK_VALUE(q_in.dim() == (ragged ? 3 : 4) && q_in.size(-1) == pages.d && q_in.size(1) > 0 && q_in.size(1) % pages.Hkv == 0 && (ragged || q_in.size(0) == n),
+                    "quashkv_b200: queries ", q_in.sizes(), " do not match ", n, " sequences and ", pages.Hkv, " KV heads of size ", pages.d);
+  TORCH_CHECK_VALUE(max_kv_len >= 0 && max_q_len >= 0, "quashkv_b200: negative lengths");
+  const Tensor table = table_rows(table_in), lens = lens_in.contiguous(), starts = ragged ? starts_in->contiguous() : Tensor();
+  if (ragged)
+    TORCH_CHECK_VALUE(starts.scalar_type() == at::kInt && starts.dim() == 1 && starts.size(0) == n + 1,
+                      "quashkv_b200: int32 query_starts of ", n + 1, " entries, got ", starts.sizes());
+  const Tensor q = rows16(dtype_code(q_in) < 0 ? q_in.to(at::kFloat) : q_in);
+  Tensor out = empty(q.sizes(), q.scalar_type(), dev);
+  if (ragged) out.zero_();                                 // rows of no sequence
+  if (q.numel() == 0 || n == 0) return out;
+  const int64_t dims[2][3] = {{0, 2, 1}, {-1, 0, 1}};      // sequence, token, head
+  int64_t qs[3], os[3];
+  for (int i = 0; i < 3; ++i) {
+    const int64_t dim = dims[ragged][i];
+    qs[i] = dim < 0 ? 0 : stride16(q, dim);
+    os[i] = dim < 0 ? 0 : stride16(out, dim);
+  }
+  const int64_t hq = q.size(1), q_len = ragged ? std::min(max_q_len, q.size(0)) : q.size(2);
+  TORCH_CHECK_VALUE(hq * std::max<int64_t>(q_len, 1) <= INT32_MAX && n <= INT32_MAX && max_kv_len < INT32_MAX - 64, "quashkv_b200: sizes beyond 32 bits");
+  const int64_t need = api.qkv_attention_paged8_workspace_bytes(n, hq, pages.Hkv, q_len, max_kv_len, pages.d, dtype_code(q));
+  const Tensor ws = need > 0 ? empty({need}, at::kByte, dev) : Tensor();
+  check(api.qkv_attention_paged8(q.const_data_ptr(), dtype_code(q), qs, pages, ip(table), table.stride(0), static_cast<int>(table.size(1)),
+                                 ip(lens), ragged ? ip(starts) : nullptr, ragged ? q.size(0) : 0, static_cast<int>(n), static_cast<int>(hq),
+                                 static_cast<int>(q_len), max_kv_len, static_cast<float>(scale), causal, out.data_ptr(), os,
+                                 need > 0 ? ws.data_ptr() : nullptr, need, call.stream), "attention_paged8");
+  return out;
+}
+
+// ---- block tables and slots ------------------------------------------------------------------------------------------
+
+void check_pool(const Tensor& table, const Tensor& lens, const Tensor& other, const Tensor& free_pages, const Tensor& pool) {
+  same_device(table.device(), {&lens, &other, &free_pages, &pool});
+  check_table(table, lens);
+  TORCH_CHECK_VALUE(table.stride(1) == 1 && lens.is_contiguous() && free_pages.is_contiguous() && pool.is_contiguous(),
+                    "quashkv_b200: tables and counts are used in place: rows, lengths, free pages and pool must be contiguous");
+  TORCH_CHECK_VALUE(other.scalar_type() == at::kInt && other.dim() == 1 && other.size(0) == lens.size(0) && free_pages.scalar_type() == at::kInt &&
+                    free_pages.dim() == 1 && pool.scalar_type() == at::kInt && pool.dim() == 1 && pool.size(0) == 2,
+                    "quashkv_b200: int32 lengths for ", lens.size(0), " sequences, int32 free pages, and pool (2) int32");
+}
+
+// lens_out / pool_out: the tensors that get the new lengths and counts (those of the call: in place).
+void run_extend(const Tensor& table, const Tensor& lens, const Tensor& new_in, const Tensor& free_pages, const Tensor& pool, int64_t block_size,
+                const Tensor& slots, const Tensor& starts, const Tensor& lens_out, const Tensor* start_out, const Tensor& pool_out, void* stream) {
+  const Tensor news = new_in.contiguous();
+  const auto w = [](const Tensor& t) { return static_cast<int32_t*>(t.data_ptr()); };
+  TORCH_CHECK_VALUE(block_size >= 1 && block_size <= INT32_MAX, "quashkv_b200: block_size must be positive");
+  check(api.qkv_extend_pages(w(table), table.stride(0), static_cast<int>(table.size(1)), ip(lens), ip(news), ip(free_pages), free_pages.size(0),
+                             ip(pool), static_cast<int>(lens.size(0)), static_cast<int>(block_size), slots.size(0),
+                             static_cast<int64_t*>(slots.data_ptr()), w(starts), w(lens_out), start_out ? w(*start_out) : nullptr, w(pool_out), stream),
+        "extend_pages");
+}
+
+std::tuple<Tensor, Tensor, Tensor, Tensor> extend_pages(Tensor table, const Tensor& lens, const Tensor& new_lens, const Tensor& free_pages,
+                                                        const Tensor& pool, int64_t block_size, int64_t max_tokens) {
+  const at::Device dev = table.device();
+  Call call(dev);
+  check_pool(table, lens, new_lens, free_pages, pool);
+  TORCH_CHECK_VALUE(max_tokens >= 0, "quashkv_b200: negative max_tokens");
+  const int64_t n = lens.size(0);
+  Tensor slots = empty({max_tokens}, at::kLong, dev), starts = empty({n + 1}, at::kInt, dev), after = empty({n}, at::kInt, dev), count = empty({2}, at::kInt, dev);
+  run_extend(table, lens, new_lens, free_pages, pool, block_size, slots, starts, after, nullptr, count, call.stream);
+  return {slots, starts, after, count};
+}
+
+std::tuple<Tensor, Tensor, Tensor> extend_pages_(Tensor table, Tensor lens, const Tensor& new_lens, const Tensor& free_pages, Tensor pool,
+                                                 int64_t block_size, int64_t max_tokens) {
+  const at::Device dev = table.device();
+  Call call(dev);
+  check_pool(table, lens, new_lens, free_pages, pool);
+  TORCH_CHECK_VALUE(max_tokens >= 0, "quashkv_b200: negative max_tokens");
+  const int64_t n = lens.size(0);
+  Tensor slots = empty({max_tokens}, at::kLong, dev), starts = empty({n + 1}, at::kInt, dev), before = empty({n}, at::kInt, dev);
+  run_extend(table, lens, new_lens, free_pages, pool, block_size, slots, starts, lens, &before, pool, call.stream);
+  return {slots, starts, before};
+}
+
+void shrink_pages_(const Tensor& table, Tensor lens, const Tensor& keep_in, Tensor free_pages, Tensor pool, int64_t block_size) {
+  const at::Device dev = table.device();
+  Call call(dev);
+  check_pool(table, lens, keep_in, free_pages, pool);
+  const Tensor keep = keep_in.contiguous();
+  TORCH_CHECK_VALUE(block_size >= 1 && block_size <= INT32_MAX, "quashkv_b200: block_size must be positive");
+  const auto w = [](const Tensor& t) { return static_cast<int32_t*>(t.data_ptr()); };
+  check(api.qkv_shrink_pages(ip(table), table.stride(0), static_cast<int>(table.size(1)), w(lens), ip(keep), w(free_pages), free_pages.size(0), w(pool),
+                             static_cast<int>(lens.size(0)), static_cast<int>(block_size), call.stream), "shrink_pages");
+}
+
 // ---- index --------------------------------------------------------------------------------------------------------
 
 std::tuple<Tensor, Tensor> index_scan_topk(const Tensor& q_in, const Tensor& codes, const Tensor& signs,
@@ -436,7 +630,8 @@ extern "C" __attribute__((used, visibility("default"))) const char quashkv_host_
 
 #define QKV_FOR_EACH_OP(X)                                                                                          \
   X(compress_mse) X(compress_ip) X(compress_ip_into) X(compress_mixed) X(append_kv) X(append_records) X(append_paged) X(decompress) X(decompress_dense) \
-  X(decompress_mixed) X(attention) X(attention_paged) X(attention_tiled) X(attention_tiled_out) X(index_scan_topk)
+  X(decompress_mixed) X(attention) X(attention_paged) X(attention_tiled) X(attention_tiled_out) X(index_scan_topk) \
+  X(append_paged8) X(attention_paged8) X(extend_pages) X(extend_pages_) X(shrink_pages_)
 
 TORCH_LIBRARY_IMPL(quashkv_b200, CUDA, m) {
 #define QKV_IMPL(name) m.impl(#name, &name);
@@ -490,6 +685,7 @@ TORCH_LIBRARY_IMPL(quashkv_b200, Autograd, m) {
 }
 
 TORCH_LIBRARY_IMPL(quashkv_b200, ADInplaceOrView, m) {
-  for (const char* name : {"compress_ip_into", "append_kv", "append_records", "append_paged", "attention_tiled_out"})
+  for (const char* name : {"compress_ip_into", "append_kv", "append_records", "append_paged", "attention_tiled_out",
+                           "append_paged8", "extend_pages", "extend_pages_", "shrink_pages_"})
     m.impl(name, torch::CppFunction::makeFromBoxedFunction<&count_writes>());
 }

@@ -1,0 +1,572 @@
+// Attention over a cache of 8-bit pages with a scale for each page and KV head: split over the tokens, for single query
+// tokens and short blocks of them.
+//
+//   out_i = sum_j softmax_j(scale q_i . (ks_p kc_j)) vs_p vc_j        p the page of token j, kc and vc its codes
+//
+// A warp goes over granules of 16 tokens, which one page holds (a page is a multiple of 16 tokens).  Codes come by
+// cp.async into a ring of the warp's own; there is no CTA barrier in the loop.  Both products run on the tensor core with
+// the tokens in the place of the rows: scores = K (16 tokens x D) times up to eight query rows, outputs = V^T (D x 16
+// tokens) times their weights, so a query row costs a column of eight and not a row of sixteen.  A code is exact in fp16;
+// which coordinate stands at which place of the inner dimension is free as long as both operands agree, so each lane reads
+// contiguous bytes of a token's key and needs no transposition.  Values are transposed by pairing the bytes of two tokens.
+//
+// Precision.  Query rows are scaled by a power of two to below 2^14 and held as fp16, which is exact for 16-bit types, and as hi + lo for
+// fp32.  Weights go in as hi + lo (22 bits, or 2^-34 of the largest).  Softmax in base 2 with two whole-number reference
+// exponents a row, so that rescaling is exact: m for the scores t, M for t + log2 of the page's value scale.  The weights
+// of the second product, 2^(t - M) vs, are then at most 2^15 and the largest at least 2^9 whatever the scales are: a page of large
+// values that a row hardly weighs takes no bits from the others.  References rise when a score is 4 above them, which is
+// rare after the first granules.
+//
+// Bound by the bytes of the pages: (2 D + 8 / block_size) a token and KV head.
+#include <math.h>
+
+#include "mma_decode.cuh"
+#include "paged8.cuh"
+#include "paged8_attention.cuh"
+
+namespace qkv {
+
+namespace {
+
+constexpr int kWarps = 4;
+constexpr int kStages = 4;
+constexpr float kNone = -1e30f;          // reference exponent before anything has been seen
+constexpr float kSlack = 4.f;
+constexpr float kLift = 10.f;            // the largest weight is near 2^kLift: fp16 then has 2^-35 of it as its least step
+
+// Bytes from one token's row to the next in the ring: without bank conflicts for both operands' reads.
+template <int D> struct Pitch { static constexpr int kKey = D == 128 || D == 96 ? D + 16 : D, kVal = D + 16; };
+
+template <int D, int QT, int NG> struct Split {
+  static constexpr int kSlot = 16 * (Pitch<D>::kKey + Pitch<D>::kVal);
+  static constexpr int kRows = 8 * NG;
+  static constexpr int kAccPitch = D + 4;
+  static constexpr size_t kRing = static_cast<size_t>(kWarps) * kStages * kSlot;
+  static constexpr size_t kMerge = static_cast<size_t>(kWarps) * kRows * (kAccPitch + 4) * 4;
+  static constexpr size_t kSmem = kRing > kMerge ? kRing : kMerge;
+};
+
+// N words from shared memory, as wide as their address allows.
+template <int N> __device__ __forceinline__ void lds(uint32_t (&w)[N], const unsigned char* p) {
+  if constexpr (N % 4 == 0) {
+#pragma unroll
+    for (int i = 0; i < N / 4; ++i) {
+      const uint4 x = reinterpret_cast<const uint4*>(p)[i];
+      w[4 * i] = x.x; w[4 * i + 1] = x.y; w[4 * i + 2] = x.z; w[4 * i + 3] = x.w;
+    }
+  } else if constexpr (N % 2 == 0) {
+#pragma unroll
+    for (int i = 0; i < N / 2; ++i) {
+      const uint2 x = reinterpret_cast<const uint2*>(p)[i];
+      w[2 * i] = x.x; w[2 * i + 1] = x.y;
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; ++i) w[i] = reinterpret_cast<const uint32_t*>(p)[i];
+  }
+}
+
+template <int D, int CODE, int QT, int NG>
+__global__ void __launch_bounds__(kWarps * 32) paged8_split_kernel(Attn8Args a) {
+  using P = Split<D, QT, NG>;
+  constexpr int kR = P::kRows, kKeyPitch = Pitch<D>::kKey, kValPitch = Pitch<D>::kVal;
+  constexpr int kChunks = D;                               // 16-byte chunks of 16 rows of D bytes
+  constexpr int kCopies = (kChunks + 31) / 32;
+  constexpr int kKW = D / 16, kVW = D / 32;                // words of a lane: of a key row, of a value row
+  extern __shared__ __align__(16) unsigned char smem[];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
+  asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");
+
+  int item = blockIdx.x;
+  const int rt = item % a.row_tiles;
+  item /= a.row_tiles;
+  const int h = item % a.Hkv, seq = item / a.Hkv;
+  const Span8 s = span8(a, seq);
+  const int rows = a.G * s.q_len, r0 = rt * kR;
+  if (r0 >= rows || rows > a.most_rows) return;
+  const int r_end = min(r0 + kR, rows);
+  const int64_t end = visible8(a, s, (r_end - 1) / a.G);
+  const int64_t begin = static_cast<int64_t>(blockIdx.y) * a.chunk, stop = min(end, begin + a.chunk);
+  if (begin > 0 && begin >= end) return;
+
+  // ---- queries: operand B of the scores, row r0 + 8 ng + g in column g ----
+  uint32_t qf[NG][QT][kKW][2];
+  float unit[NG][2];                                       // score (base 2) per unit of the product, rows 2t and 2t + 1
+  int lim[NG][2];                                          // last token that they see, relative to `begin`
+#pragma unroll
+  for (int n = 0; n < NG; ++n) {
+    const int r = r0 + 8 * n + g;
+    const bool live = r < r_end;
+    float v[D / 4], mx = 0.f;
+    if (live) {
+      const int64_t at = s.q_row0 + static_cast<int64_t>(r / a.G) * a.q_stride[1] + static_cast<int64_t>(h * a.G + r % a.G) * a.q_stride[2] + t * (D / 4);
+      load_row8<D / 4>(a.q, a.dtype, at, v);
+    } else {
+#pragma unroll
+      for (int i = 0; i < D / 4; ++i) v[i] = 0.f;
+    }
+#pragma unroll
+    for (int i = 0; i < D / 4; ++i) mx = fmaxf(mx, fabsf(v[i]));
+    mx = fmaxf(mx, __shfl_xor_sync(QKV_FULL_MASK, mx, 1));
+    mx = fmaxf(mx, __shfl_xor_sync(QKV_FULL_MASK, mx, 2));
+    const float up = scale_to8<13>(mx);
+#pragma unroll
+    for (int k = 0; k < kKW; ++k)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const float x = v[4 * k + 2 * e] * up, y = v[4 * k + 2 * e + 1] * up;
+        const __half2 hi = __floats2half2_rn(x, y);
+        qf[n][0][k][e] = *reinterpret_cast<const uint32_t*>(&hi);
+        if (QT == 2) {
+          const float2 f = __half22float2(hi);
+          qf[n][QT - 1][k][e] = pack_half2(x - f.x, y - f.y);
+        }
+      }
+    const float u = a.scale * 1.4426950408889634f * inverse8(up);
+    const int64_t see = live ? visible8(a, s, r / a.G) : 0;
+    const int last = static_cast<int>(max(min(see - begin, a.chunk), static_cast<int64_t>(0))) - 1;
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      unit[n][e] = __shfl_sync(QKV_FULL_MASK, u, 4 * (2 * t + e));
+      lim[n][e] = __shfl_sync(QKV_FULL_MASK, last, 4 * (2 * t + e));
+    }
+  }
+  // tokens up to this one are seen by every row (rows behind the last one do not count: their results are not kept)
+  const int all_see = static_cast<int>(max(min(visible8(a, s, r0 / a.G) - begin, a.chunk), static_cast<int64_t>(0))) - 1;
+
+  float acc[NG][2 * kVW][4];                               // [m tile]: coordinates 2j, 2j + 1 of the lane's, rows 2t, 2t + 1
+  float m[NG][2], M[NG][2], l[NG][2];
+#pragma unroll
+  for (int n = 0; n < NG; ++n) {
+#pragma unroll
+    for (int j = 0; j < 2 * kVW; ++j)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) acc[n][j][e] = 0.f;
+#pragma unroll
+    for (int e = 0; e < 2; ++e) { m[n][e] = kNone; M[n][e] = 0.5f * kNone; l[n][e] = 0.f; }
+  }
+
+  // ---- granules: this warp has warp, warp + 4, ... of the chunk ----
+  const int granules = stop > begin ? static_cast<int>((stop - begin + 15) >> 4) : 0;
+  const int count = granules > warp ? (granules - warp + kWarps - 1) / kWarps : 0;
+  const int stored = static_cast<int>(min(s.len - begin, a.chunk));        // tokens that the cache holds from `begin` on
+  const int32_t* row = a.table + seq * a.table_stride;
+  unsigned char* ring = smem + warp * kStages * P::kSlot;
+  // page and scales of granule 32 b + lane of the warp, for the batch b in work and the next one
+  auto page_of = [&](int i) -> int {
+    if (i >= count) return -1;
+    const int64_t tok = begin + 16 * (warp + kWarps * i);
+    const int id = row[a.bs_shift >= 0 ? tok >> a.bs_shift : tok / a.p.block_size];
+    return id >= 0 && id < a.p.num_blocks ? id : -1;
+  };
+  auto scale_k = [&](int id) { return id < 0 ? 0.f : a.p.k_scales[id * a.p.ks_stride[0] + h * a.p.ks_stride[1]]; };
+  auto scale_v = [&](int id) { return id < 0 ? 0.f : a.p.v_scales[id * a.p.vs_stride[0] + h * a.p.vs_stride[1]]; };
+  int pg = page_of(lane), pg_next = -1;
+  const uint8_t* k_head = a.p.k_codes + h * a.p.k_stride[1];
+  const uint8_t* v_head = a.p.v_codes + h * a.p.v_stride[1];
+  auto issue = [&](int i, int id) {                        // codes of granule i, page id (all lanes)
+    if (i < count && id >= 0) {
+      const int64_t tok = begin + 16 * (warp + kWarps * i);
+      const int off = static_cast<int>(a.bs_shift >= 0 ? tok & ((1 << a.bs_shift) - 1) : tok % a.p.block_size);
+      const uint8_t* ks = k_head + id * a.p.k_stride[0] + off * a.p.k_stride[2];
+      const uint8_t* vs = v_head + id * a.p.v_stride[0] + off * a.p.v_stride[2];
+      unsigned char* dst = ring + (i % kStages) * P::kSlot;
+#pragma unroll
+      for (int c = 0; c < kCopies; ++c) {
+        const int x = lane + 32 * c, rw = x / (D / 16), col = 16 * (x % (D / 16));
+        if (kChunks % 32 == 0 || x < kChunks) {
+          cp_async16(dst + rw * kKeyPitch + col, ks + rw * a.p.k_stride[2] + col, 16);
+          cp_async16(dst + 16 * kKeyPitch + rw * kValPitch + col, vs + rw * a.p.v_stride[2] + col, 16);
+        }
+      }
+    }
+    cp_async_commit();                                     // one group a granule, empty ones too
+  };
+#pragma unroll
+  for (int i = 0; i < kStages - 1; ++i) issue(i, __shfl_sync(QKV_FULL_MASK, pg, i));
+  float ksc = scale_k(pg), vsc = scale_v(pg), ksc_next = 0.f, vsc_next = 0.f;
+
+  for (int i = 0; i < count; ++i) {
+    const int b = i & 31;
+    if (b == 0) {
+      if (i > 0) { pg = pg_next; ksc = ksc_next; vsc = vsc_next; }
+      pg_next = page_of(i + 32 + lane);
+    }
+    if (b == 16) { ksc_next = scale_k(pg_next); vsc_next = scale_v(pg_next); }
+    const int ahead = b + kStages - 1;
+    issue(i + kStages - 1, __shfl_sync(QKV_FULL_MASK, ahead < 32 ? pg : pg_next, ahead & 31));
+    cp_async_wait<kStages - 1>();
+    __syncwarp();
+
+    const unsigned char* slot = ring + (i % kStages) * P::kSlot;
+    const int tok = 16 * (warp + kWarps * i);              // relative to begin
+    const int id = __shfl_sync(QKV_FULL_MASK, pg, b);
+    const float ks = __shfl_sync(QKV_FULL_MASK, ksc, b), vs = __shfl_sync(QKV_FULL_MASK, vsc, b);
+    const int valid = id < 0 ? 0 : min(16, stored - tok);
+    const bool whole = valid == 16 && tok + 15 <= all_see; // every row sees every token
+
+    // ---- scores ----
+    float sc[NG][4];
+    {
+      uint32_t w0[kKW], w1[kKW];
+      lds<kKW>(w0, slot + g * kKeyPitch + t * (D / 4));
+      lds<kKW>(w1, slot + (g + 8) * kKeyPitch + t * (D / 4));
+      float part[NG][2][4];
+#pragma unroll
+      for (int n = 0; n < NG; ++n)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) part[n][0][e] = part[n][1][e] = 0.f;
+#pragma unroll
+      for (int k = 0; k < kKW; ++k) {
+        const uint32_t x = p8::biased<CODE>(w0[k]), y = p8::biased<CODE>(w1[k]);
+        const uint32_t av[4] = {p8::halves_low<CODE>(x), p8::halves_low<CODE>(y), p8::halves_high<CODE>(x), p8::halves_high<CODE>(y)};
+#pragma unroll
+        for (int n = 0; n < NG; ++n) {
+          if (QT == 2) mma16816(part[n][k & 1], av, qf[n][QT - 1][k][0], qf[n][QT - 1][k][1]);
+          mma16816(part[n][k & 1], av, qf[n][0][k][0], qf[n][0][k][1]);
+        }
+      }
+#pragma unroll
+      for (int n = 0; n < NG; ++n)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) sc[n][e] = (part[n][0][e] + part[n][1][e]) * (ks * unit[n][e & 1]);
+    }
+    if (!whole) {
+#pragma unroll
+      for (int n = 0; n < NG; ++n)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int k = g + 8 * (e >> 1);
+          if (k >= valid || tok + k > lim[n][e & 1]) sc[n][e] = -INFINITY;
+        }
+    }
+
+    // ---- weights ----
+    // vs = mant * 2^ex; a scale of 0 weighs nothing
+    const uint32_t vbits = __float_as_uint(vs);
+    const int vexp = static_cast<int>((vbits >> 23) & 255u);
+    const float ex = vexp ? static_cast<float>(vexp - 127) : kNone;
+    const float mant = vexp ? (vexp == 255 ? vs : __uint_as_float((vbits & 0x807fffffu) | 0x3f800000u)) : 0.f;
+    bool rise = false;
+#pragma unroll
+    for (int n = 0; n < NG; ++n)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        rise |= sc[n][e] > m[n][e & 1] + kSlack;
+        rise |= sc[n][e] + ex > M[n][e & 1] + (kLift + kSlack);
+      }
+    if (__any_sync(QKV_FULL_MASK, rise)) {
+#pragma unroll
+      for (int n = 0; n < NG; ++n)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          float top = fmaxf(sc[n][e], sc[n][e + 2]);
+          top = fmaxf(top, __shfl_xor_sync(QKV_FULL_MASK, top, 4));
+          top = fmaxf(top, __shfl_xor_sync(QKV_FULL_MASK, top, 8));
+          top = fmaxf(top, __shfl_xor_sync(QKV_FULL_MASK, top, 16));
+          top = ceilf(top);
+          const float m1 = fmaxf(m[n][e], top), M1 = fmaxf(M[n][e], top + ex - kLift);
+          l[n][e] *= ex2(m[n][e] - m1);
+          const float f = ex2(M[n][e] - M1);
+          m[n][e] = m1;
+          M[n][e] = M1;
+#pragma unroll
+          for (int j = 0; j < 2 * kVW; ++j) {
+            acc[n][j][e] *= f;
+            acc[n][j][e + 2] *= f;
+          }
+        }
+    }
+    uint32_t wh[NG][2], wl[NG][2];                         // operand B of the second product: tokens x rows
+#pragma unroll
+    for (int n = 0; n < NG; ++n) {
+      float w[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        l[n][e & 1] += ex2(sc[n][e] - m[n][e & 1]);
+        w[e] = ex2(sc[n][e] - (M[n][e & 1] - ex)) * mant;
+      }
+      if (!whole && vexp == 255) {                         // a page of NaN: nothing from tokens that are not seen
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (sc[n][e] == -INFINITY) w[e] = 0.f;
+      }
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const __half2 hi = __floats2half2_rn(w[2 * e], w[2 * e + 1]);
+        const float2 f = __half22float2(hi);
+        wh[n][e] = movmatrix_trans(*reinterpret_cast<const uint32_t*>(&hi));
+        wl[n][e] = movmatrix_trans(pack_half2(w[2 * e] - f.x, w[2 * e + 1] - f.y));
+      }
+    }
+
+    // ---- values: row = coordinate, inner dimension = tokens 2t, 2t + 1, 2t + 8, 2t + 9 ----
+    {
+      const unsigned char* vp = slot + 16 * kKeyPitch + 2 * t * kValPitch + g * (D / 8);
+      uint32_t v0[kVW], v1[kVW], v8[kVW], v9[kVW];
+      lds<kVW>(v0, vp);
+      lds<kVW>(v1, vp + kValPitch);
+      lds<kVW>(v8, vp + 8 * kValPitch);
+      lds<kVW>(v9, vp + 9 * kValPitch);
+      if (valid < 16) {                                    // bytes behind the last token may be anything
+        const uint32_t z = 0;
+#pragma unroll
+        for (int k = 0; k < kVW; ++k) {
+          v0[k] = 2 * t < valid ? v0[k] : z;
+          v1[k] = 2 * t + 1 < valid ? v1[k] : z;
+          v8[k] = 2 * t + 8 < valid ? v8[k] : z;
+          v9[k] = 2 * t + 9 < valid ? v9[k] : z;
+        }
+      }
+#pragma unroll
+      for (int k = 0; k < kVW; ++k) {
+        const uint32_t a01 = p8::biased<CODE>(prmt(v0[k], v1[k], 0x5140)), a23 = p8::biased<CODE>(prmt(v0[k], v1[k], 0x7362));
+        const uint32_t b01 = p8::biased<CODE>(prmt(v8[k], v9[k], 0x5140)), b23 = p8::biased<CODE>(prmt(v8[k], v9[k], 0x7362));
+        const uint32_t x[4] = {p8::halves_low<CODE>(a01), p8::halves_high<CODE>(a01), p8::halves_low<CODE>(b01), p8::halves_high<CODE>(b01)};
+        const uint32_t y[4] = {p8::halves_low<CODE>(a23), p8::halves_high<CODE>(a23), p8::halves_low<CODE>(b23), p8::halves_high<CODE>(b23)};
+#pragma unroll
+        for (int n = 0; n < NG; ++n) {
+          if (QT == 2) {
+            // The tensor core truncates what it adds to an accumulator: over many granules that would show in fp32, so
+            // each granule's sum is added in fp32.
+            float c[4] = {0.f, 0.f, 0.f, 0.f}, d[4] = {0.f, 0.f, 0.f, 0.f};
+            mma16816(c, x, wl[n][0], wl[n][1]);
+            mma16816(d, y, wl[n][0], wl[n][1]);
+            mma16816(c, x, wh[n][0], wh[n][1]);
+            mma16816(d, y, wh[n][0], wh[n][1]);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) { acc[n][2 * k][e] += c[e]; acc[n][2 * k + 1][e] += d[e]; }
+          } else {
+            mma16816(acc[n][2 * k], x, wl[n][0], wl[n][1]);
+            mma16816(acc[n][2 * k + 1], y, wl[n][0], wl[n][1]);
+            mma16816(acc[n][2 * k], x, wh[n][0], wh[n][1]);
+            mma16816(acc[n][2 * k + 1], y, wh[n][0], wh[n][1]);
+          }
+        }
+      }
+    }
+    __syncwarp();                                          // the slot may be filled again
+  }
+  cp_async_wait<0>();
+
+  // ---- the four warps' sums ----
+  __syncthreads();                                         // the ring has been read
+  float* sums = reinterpret_cast<float*>(smem);            // [warp][row][kAccPitch], then [warp][row][4]: m, M, l
+  float* ref = sums + kWarps * kR * P::kAccPitch;
+#pragma unroll
+  for (int n = 0; n < NG; ++n)
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      float x = l[n][e];
+      x += __shfl_xor_sync(QKV_FULL_MASK, x, 4);
+      x += __shfl_xor_sync(QKV_FULL_MASK, x, 8);
+      x += __shfl_xor_sync(QKV_FULL_MASK, x, 16);
+      const int r = 8 * n + 2 * t + e;
+      if (g == 0) *reinterpret_cast<float4*>(ref + (warp * kR + r) * 4) = make_float4(m[n][e], M[n][e], x, 0.f);
+#pragma unroll
+      for (int j = 0; j < 2 * kVW; ++j)
+        *reinterpret_cast<float2*>(sums + (warp * kR + r) * P::kAccPitch + g * (D / 8) + 2 * j) = make_float2(acc[n][j][e], acc[n][j][e + 2]);
+    }
+  __syncthreads();
+  const int n_rows = r_end - r0;
+  for (int x = threadIdx.x; x < n_rows * (D / 4); x += kWarps * 32) {
+    const int r = x / (D / 4), c = 4 * (x % (D / 4));
+    float mt = kNone, Mt = 0.5f * kNone;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) {
+      mt = max_or_nan(mt, ref[(w * kR + r) * 4]);
+      Mt = max_or_nan(Mt, ref[(w * kR + r) * 4 + 1]);
+    }
+    float lt = 0.f;
+    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) {
+      const float4 q = *reinterpret_cast<const float4*>(ref + (w * kR + r) * 4);
+      const float4 y = *reinterpret_cast<const float4*>(sums + (w * kR + r) * P::kAccPitch + c);
+      lt = fmaf(q.z, ex2(q.x - mt), lt);
+      const float f = ex2(q.y - Mt);
+      o.x = fmaf(y.x, f, o.x); o.y = fmaf(y.y, f, o.y); o.z = fmaf(y.z, f, o.z); o.w = fmaf(y.w, f, o.w);
+    }
+    const int rr = r0 + r;
+    if (a.n_splits == 1) {
+      store_out8(a, s, h, rr, c, o, mt, Mt, lt);
+    } else {
+      const int64_t slot = ((static_cast<int64_t>(seq) * a.Hkv + h) * a.most_rows + rr) * a.n_splits + blockIdx.y;
+      *reinterpret_cast<float4*>(a.part + slot * D + c) = o;
+      if (c == 0) *reinterpret_cast<float4*>(a.ref + slot * 4) = make_float4(mt, Mt, lt, 0.f);
+    }
+  }
+}
+
+// Splits of a row: a warp each; lane = four coordinates (D / 4 lanes).
+template <int D>
+__global__ void __launch_bounds__(128) paged8_merge_kernel(Attn8Args a) {
+  const int lane = threadIdx.x & 31, c = 4 * lane;
+  const int64_t job = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 5);
+  const int rr = static_cast<int>(job % a.most_rows);
+  const int64_t head = job / a.most_rows;
+  const int h = static_cast<int>(head % a.Hkv);
+  asm volatile("griddepcontrol.wait;\n" ::: "memory");
+  if (head >= static_cast<int64_t>(a.n_seq) * a.Hkv) return;
+  const int seq = static_cast<int>(head / a.Hkv);
+  const Span8 s = span8(a, seq);
+  const int rows = a.G * s.q_len;
+  if (rr >= rows || rows > a.most_rows) return;
+  const int tile_end = min((rr / a.tile_rows + 1) * a.tile_rows, rows);
+  const int64_t end = visible8(a, s, (tile_end - 1) / a.G);
+  const int parts = end > a.chunk ? static_cast<int>((end + a.chunk - 1) / a.chunk) : 1;
+  const int64_t slot = job * a.n_splits;
+  float mt = kNone, Mt = 0.5f * kNone;
+  for (int p = lane; p < parts; p += 32) {
+    mt = max_or_nan(mt, a.ref[(slot + p) * 4]);
+    Mt = max_or_nan(Mt, a.ref[(slot + p) * 4 + 1]);
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    mt = max_or_nan(mt, __shfl_xor_sync(QKV_FULL_MASK, mt, o));
+    Mt = max_or_nan(Mt, __shfl_xor_sync(QKV_FULL_MASK, Mt, o));
+  }
+  float lt = 0.f;
+  float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+  for (int p = 0; p < parts; ++p) {
+    const float4 q = *reinterpret_cast<const float4*>(a.ref + (slot + p) * 4);
+    lt = fmaf(q.z, ex2(q.x - mt), lt);
+    const float f = ex2(q.y - Mt);
+    if (c < D) {
+      const float4 y = *reinterpret_cast<const float4*>(a.part + (slot + p) * D + c);
+      o.x = fmaf(y.x, f, o.x); o.y = fmaf(y.y, f, o.y); o.z = fmaf(y.z, f, o.z); o.w = fmaf(y.w, f, o.w);
+    }
+  }
+  if (c < D) store_out8(a, s, h, rr, c, o, mt, Mt, lt);
+}
+
+// How the tokens are split: see plan8.
+struct Plan8 { int ng, row_tiles, most_rows, n_splits; int64_t chunk; size_t ws; };
+
+Plan8 plan8(int n_seq, int Hkv, int G, int q_len, int64_t max_kv_len, int d, int dtype) {
+  Plan8 p;
+  p.most_rows = G * q_len;
+  p.ng = dtype != QKV_F32 && p.most_rows > 8 ? 2 : 1;
+  p.row_tiles = (p.most_rows + 8 * p.ng - 1) / (8 * p.ng);
+  const int64_t items = static_cast<int64_t>(n_seq) * Hkv * p.row_tiles, wave = 3 * kNumSMs;
+  int64_t splits = (2 * wave + items - 1) / items;
+  const int64_t most = (max_kv_len + 63) / 64;
+  if (splits > most) splits = most;
+  if (splits > 64) splits = 64;
+  if (splits < 1) splits = 1;
+  p.chunk = (max_kv_len + splits - 1) / splits;
+  p.chunk = (p.chunk + 63) / 64 * 64;
+  if (p.chunk < 64) p.chunk = 64;
+  p.n_splits = static_cast<int>((max_kv_len + p.chunk - 1) / p.chunk);
+  if (p.n_splits < 1) p.n_splits = 1;
+  const size_t slots = static_cast<size_t>(n_seq) * Hkv * p.most_rows * p.n_splits;
+  p.ws = p.n_splits > 1 ? slots * (d + 4) * sizeof(float) : 0;
+  return p;
+}
+
+template <int D, int CODE, int QT, int NG>
+int launch_split(const Attn8Args& a, int64_t items, cudaStream_t st) {
+  using P = Split<D, QT, NG>;
+  auto kernel = paged8_split_kernel<D, CODE, QT, NG>;
+  if (P::kSmem > 48 * 1024 && cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(P::kSmem)) != cudaSuccess)
+    return QKV_ELAUNCH;
+  kernel<<<dim3(static_cast<unsigned>(items), a.n_splits), kWarps * 32, P::kSmem, st>>>(a);
+  if (const int rc = check_launch()) return rc;
+  if (a.n_splits == 1) return QKV_OK;
+  const int64_t rows = static_cast<int64_t>(a.n_seq) * a.Hkv * a.most_rows;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>((rows + 3) / 4));
+  cfg.blockDim = dim3(128);
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  if (cudaLaunchKernelEx(&cfg, paged8_merge_kernel<D>, a) != cudaSuccess) return QKV_ELAUNCH;
+  return check_launch();
+}
+
+template <int D, int CODE>
+int launch_types(const Attn8Args& a, int ng, int64_t items, cudaStream_t st) {
+  if (a.dtype == QKV_F32) return launch_split<D, CODE, 2, 1>(a, items, st);
+  return ng == 2 ? launch_split<D, CODE, 1, 2>(a, items, st) : launch_split<D, CODE, 1, 1>(a, items, st);
+}
+template <int D>
+int launch_codes(const Attn8Args& a, int ng, int64_t items, cudaStream_t st) {
+  return a.p.code == QKV_E4M3 ? launch_types<D, p8::kE4M3>(a, ng, items, st) : launch_types<D, p8::kInt8>(a, ng, items, st);
+}
+
+bool sizes_ok(int n_seq, int Hq, int Hkv, int q_len, int64_t max_kv_len) {
+  return n_seq >= 0 && Hkv >= 1 && Hq >= Hkv && Hq % Hkv == 0 && q_len >= 0 && max_kv_len >= 0 && max_kv_len <= 0x7fffffffLL - 64 &&
+         static_cast<int64_t>(Hq) * (q_len > 0 ? q_len : 1) <= 0x7fffffffLL;
+}
+
+}  // namespace
+}  // namespace qkv
+
+using namespace qkv;
+
+extern "C" size_t qkv_attention_paged8_workspace_bytes(int n_seq, int Hq, int Hkv, int q_len, int64_t max_kv_len, int d, int q_dtype) {
+  if (!sizes_ok(n_seq, Hq, Hkv, q_len, max_kv_len) || n_seq == 0 || q_len == 0) return 0;
+  return plan8(n_seq, Hkv, Hq / Hkv, q_len, max_kv_len, d, q_dtype).ws;
+}
+
+extern "C" int qkv_attention_paged8(const void* q, int q_dtype, const int64_t* q_strides, qkv_pages8_t pages,
+                                    const int32_t* block_table, int64_t table_stride, int max_blocks, const int32_t* seq_lens,
+                                    const int32_t* query_starts, int64_t total_q, int n_seq, int Hq, int q_len, int64_t max_kv_len,
+                                    float scale, int causal, void* out, const int64_t* out_strides, void* workspace,
+                                    size_t workspace_bytes, void* stream) {
+  if (!q || !q_strides || !block_table || !seq_lens || !out || !out_strides) return QKV_ENULL;
+  if (q_dtype != QKV_F32 && q_dtype != QKV_BF16 && q_dtype != QKV_F16) return QKV_EDTYPE;
+  if (const int rc = check_pages8(pages)) return rc;
+  if (!sizes_ok(n_seq, Hq, pages.Hkv, q_len, max_kv_len) || max_blocks < 1 || table_stride < max_blocks || total_q < 0) return QKV_EDIM;
+  const int item = q_dtype == QKV_F32 ? 4 : 2;
+  if ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(out)) & 15u) return QKV_EALIGN;
+  for (int i = 0; i < 3; ++i)
+    if ((q_strides[i] * item & 15) || (out_strides[i] * item & 15)) return QKV_EALIGN;
+  if (n_seq == 0 || q_len == 0) return QKV_OK;
+  Attn8Args a{};
+  a.q = q;
+  a.dtype = q_dtype;
+  for (int i = 0; i < 3; ++i) {
+    a.q_stride[i] = q_strides[i];
+    a.o_stride[i] = out_strides[i];
+  }
+  a.p = pages;
+  a.table = block_table;
+  a.table_stride = table_stride;
+  a.seq_lens = seq_lens;
+  a.starts = query_starts;
+  a.total_q = total_q;
+  a.n_seq = n_seq;
+  a.Hkv = pages.Hkv;
+  a.G = Hq / pages.Hkv;
+  a.q_len = q_len;
+  const int64_t room = static_cast<int64_t>(max_blocks) * pages.block_size;
+  a.max_kv_len = max_kv_len < room ? max_kv_len : room;
+  a.causal = causal != 0;
+  a.scale = scale;
+  a.out = out;
+  a.bs_shift = (pages.block_size & (pages.block_size - 1)) == 0 ? __builtin_ctz(pages.block_size) : -1;
+  const Plan8 p = plan8(n_seq, a.Hkv, a.G, q_len, max_kv_len, pages.d, q_dtype);
+  if (p.ws > workspace_bytes || (p.ws > 0 && !workspace)) return QKV_EWORKSPACE;
+  if (reinterpret_cast<uintptr_t>(workspace) & 15u) return QKV_EALIGN;
+  const int64_t items = static_cast<int64_t>(n_seq) * a.Hkv * p.row_tiles;
+  if (items > 0x7fffffffLL || static_cast<int64_t>(n_seq) * a.Hkv * p.most_rows > 0x7fffffffLL) return QKV_EDIM;
+  a.row_tiles = p.row_tiles;
+  a.tile_rows = 8 * p.ng;
+  a.most_rows = p.most_rows;
+  a.n_splits = p.n_splits;
+  a.chunk = p.chunk;
+  a.part = static_cast<float*>(workspace);
+  a.ref = a.part + static_cast<size_t>(n_seq) * a.Hkv * p.most_rows * p.n_splits * pages.d;
+  const cudaStream_t st = static_cast<cudaStream_t>(stream);
+  switch (pages.d) {
+    case 32: return launch_codes<32>(a, p.ng, items, st);
+    case 64: return launch_codes<64>(a, p.ng, items, st);
+    case 96: return launch_codes<96>(a, p.ng, items, st);
+    default: return launch_codes<128>(a, p.ng, items, st);
+  }
+}

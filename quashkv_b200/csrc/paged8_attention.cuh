@@ -1,0 +1,115 @@
+// What the attention kernels over 8-bit pages share: arguments, a sequence's rows and tokens, loads of query rows and
+// the store of output rows.
+#pragma once
+
+#include "mma_decode.cuh"
+#include "paged8.cuh"
+
+namespace qkv {
+
+struct Attn8Args {
+  const void* q; int dtype;                 // queries and outputs: QKV_F32 / BF16 / F16
+  int64_t q_stride[3], o_stride[3];         // elements from one sequence, token, query head to the next
+  qkv_pages8_t p;
+  const int32_t* table; int64_t table_stride; int bs_shift;      // log2 of block_size, -1 where it has none
+  const int32_t* seq_lens;
+  const int32_t* starts; int64_t total_q;   // ragged queries: rows starts[i] .. starts[i + 1] of total_q are sequence i's
+  int n_seq, Hkv, G, q_len, causal;         // q_len: of every sequence, or the most of any
+  int64_t max_kv_len;                       // within the tables
+  float scale;
+  void* out;
+  int row_tiles, tile_rows, most_rows, n_splits; int64_t chunk;
+  float* part; float* ref;                  // [seq][kv head][most_rows][n_splits] sums, and their (m, M, l, -)
+};
+
+// Tokens and queries of a sequence, within what the host has promised.
+struct Span8 { int64_t len; int q_len, q_all; int64_t q_row0, o_row0; };
+
+__device__ __forceinline__ Span8 span8(const Attn8Args& a, int seq) {
+  Span8 s;
+  s.len = min(static_cast<int64_t>(max(a.seq_lens[seq], 0)), a.max_kv_len);
+  if (a.starts) {
+    const int64_t lo = min(static_cast<int64_t>(max(a.starts[seq], 0)), a.total_q);
+    const int64_t hi = min(max(static_cast<int64_t>(a.starts[seq + 1]), lo), a.total_q);
+    s.q_all = static_cast<int>(hi - lo);
+    s.q_len = min(s.q_all, a.q_len);
+    s.q_row0 = lo * a.q_stride[1];
+    s.o_row0 = lo * a.o_stride[1];
+  } else {
+    s.q_len = s.q_all = a.q_len;
+    s.q_row0 = seq * a.q_stride[0];
+    s.o_row0 = seq * a.o_stride[0];
+  }
+  return s;
+}
+
+// How many tokens the queries at token `tok` of the sequence's block see.
+__device__ __forceinline__ int64_t visible8(const Attn8Args& a, const Span8& s, int tok) {
+  if (!a.causal) return s.len;
+  const int64_t v = s.len - s.q_all + tok + 1;
+  return v < 0 ? 0 : (v > s.len ? s.len : v);
+}
+
+// 2^(K - e) for a magnitude 2^e <= x < 2^(e+1): x times it lies in [2^K, 2^(K+1)).  A normal number, and so is its inverse.
+template <int K>
+__device__ __forceinline__ float scale_to8(float x) {
+  int e = 254 + K - static_cast<int>((__float_as_uint(x) >> 23) & 255u);
+  e = e < 1 ? 1 : (e > 253 ? 253 : e);
+  return __uint_as_float(static_cast<uint32_t>(e) << 23);
+}
+__device__ __forceinline__ float inverse8(float s) { return __uint_as_float((254u << 23) - __float_as_uint(s)); }
+
+__device__ __forceinline__ float max_or_nan(float a, float b) { return a != a ? a : (b != b ? b : fmaxf(a, b)); }
+
+// N coordinates (a multiple of 8) from element `at` of the queries.
+template <int N>
+__device__ __forceinline__ void load_row8(const void* q, int dtype, int64_t at, float (&v)[N]) {
+  if (dtype == QKV_F32) {
+    const float4* p = reinterpret_cast<const float4*>(static_cast<const float*>(q) + at);
+#pragma unroll
+    for (int i = 0; i < N / 4; ++i) {
+      const float4 x = __ldg(p + i);
+      v[4 * i] = x.x; v[4 * i + 1] = x.y; v[4 * i + 2] = x.z; v[4 * i + 3] = x.w;
+    }
+    return;
+  }
+  const uint4* p = reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(q) + at);
+#pragma unroll
+  for (int i = 0; i < N / 8; ++i) {
+    const uint4 x = __ldg(p + i);
+    const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      if (dtype == QKV_BF16) {
+        v[8 * i + 2 * k] = __uint_as_float(w[k] << 16);
+        v[8 * i + 2 * k + 1] = __uint_as_float(w[k] & 0xffff0000u);
+      } else {
+        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[k]));
+        v[8 * i + 2 * k] = f.x;
+        v[8 * i + 2 * k + 1] = f.y;
+      }
+    }
+  }
+}
+
+// Coordinates c .. c + 3 of output row r of KV head h: sums o in units of 2^M, total weight l in units of 2^m.  A row that has seen
+// nothing is zeros.  One rounding, to the queries' type.
+__device__ __forceinline__ void store_out8(const Attn8Args& a, const Span8& s, int h, int r, int c, float4 o, float m, float M, float l) {
+  float f = 0.f;
+  if (l != 0.f) f = ex2(M - m) / l;                        // M is far below m where every value was zero
+  o.x *= f; o.y *= f; o.z *= f; o.w *= f;
+  const int64_t at = s.o_row0 + static_cast<int64_t>(r / a.G) * a.o_stride[1] + static_cast<int64_t>(h * a.G + r % a.G) * a.o_stride[2] + c;
+  if (a.dtype == QKV_F32) {
+    *reinterpret_cast<float4*>(static_cast<float*>(a.out) + at) = o;
+  } else if (a.dtype == QKV_BF16) {
+    const __nv_bfloat162 x = __floats2bfloat162_rn(o.x, o.y), y = __floats2bfloat162_rn(o.z, o.w);
+    *reinterpret_cast<uint2*>(static_cast<__nv_bfloat16*>(a.out) + at) =
+        make_uint2(*reinterpret_cast<const uint32_t*>(&x), *reinterpret_cast<const uint32_t*>(&y));
+  } else {
+    const __half2 x = __floats2half2_rn(o.x, o.y), y = __floats2half2_rn(o.z, o.w);
+    *reinterpret_cast<uint2*>(static_cast<__half*>(a.out) + at) =
+        make_uint2(*reinterpret_cast<const uint32_t*>(&x), *reinterpret_cast<const uint32_t*>(&y));
+  }
+}
+
+}  // namespace qkv

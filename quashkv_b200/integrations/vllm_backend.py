@@ -145,48 +145,21 @@ def register_quashkv_backend() -> None:
 # ---------------------------------------------------------------------------------------------------
 # Real pages: a shared pool, block tables, per-sequence lengths
 # ---------------------------------------------------------------------------------------------------
-class QuashKVPagedCache:
-    """A pool of compressed KV pages shared by many sequences of one attention layer.
+class PagePool:
+    """Which pages belong to which sequence, and which are free: the host side of a pool (lists and dicts, no GPU)."""
 
-    A sequence owns a list of pages and a token count.  For head size 128 at 3/3 bits with ``block_size`` a
-    multiple of 16 the pool is ``records [num_blocks, num_kv_heads, block_size / 16, 1664]``: 16-token tile
-    records, the layout the tensor-core attention kernel streams (a 16-token page is exactly one record per
-    head).  Otherwise the pool is the five row-major planes ``[num_blocks, num_kv_heads, block_size, row
-    bytes]`` (codes, sign bits) and ``[num_blocks, num_kv_heads, block_size]`` (norms) of the generic kernel.
-    """
-
-    def __init__(self, num_blocks: int, num_kv_heads: int, head_size: int,
-                 config: Optional[QuashKVPageConfig] = None, device="cuda", layer_idx: int = 0):
-        self.config = config or QuashKVPageConfig()
-        if num_blocks < 1 or self.config.block_size < 1:
+    def __init__(self, num_blocks: int, num_kv_heads: int, head_size: int, block_size: int, device):
+        if num_blocks < 1 or block_size < 1:
             raise ValueError("num_blocks and block_size must be positive")
         self.num_blocks = num_blocks
         self.num_kv_heads = num_kv_heads
         self.head_size = head_size
-        self.block_size = self.config.block_size
+        self.block_size = block_size
         self.device = torch.device(device)
-        self.engine = QuashKVEngine(head_dim=head_size, key_bits=self.config.key_bits,
-                                    value_bits=self.config.value_bits, seed=self.config.seed + layer_idx,
-                                    device=self.device)
-        pk, ps, pv = self.engine._row_bytes()
-        shape = (num_blocks, num_kv_heads, self.block_size)
-        u8 = dict(dtype=torch.uint8, device=self.device)
-        f32 = dict(dtype=torch.float32, device=self.device)
-        self.tiled = self.engine._tiled and self.block_size % ops.TILE_TOKENS == 0
-        if self.tiled:
-            self.planes = {"records": torch.zeros((num_blocks, num_kv_heads, self.block_size // ops.TILE_TOKENS,
-                                                   ops.TILE_BYTES), **u8)}
-        else:
-            self.planes = {
-                "k_codes": torch.zeros((*shape, pk), **u8), "k_signs": torch.zeros((*shape, ps), **u8),
-                "k_norms": torch.zeros(shape, **f32),
-                "v_codes": torch.zeros((*shape, pv), **u8), "v_norms": torch.zeros(shape, **f32),
-            }
         self._free = list(range(num_blocks - 1, -1, -1))      # pop() hands out block 0 first
         self._blocks: dict = {}                                # sequence id -> list of block ids
         self._lens: dict = {}                                  # sequence id -> tokens stored
 
-    # ---- bookkeeping (host) ---------------------------------------------------------------------
     @property
     def free_blocks(self) -> int:
         return len(self._free)
@@ -225,6 +198,39 @@ class QuashKVPagedCache:
         lens = np.asarray([self._lens.get(s, 0) for s in seq_ids], dtype=np.int32)
         return (torch.from_numpy(table).to(self.device), torch.from_numpy(lens).to(self.device),
                 int(lens.max()) if len(lens) else 0)
+
+
+class QuashKVPagedCache(PagePool):
+    """A pool of compressed KV pages shared by many sequences of one attention layer.
+
+    A sequence owns a list of pages and a token count.  For head size 128 at 3/3 bits with ``block_size`` a
+    multiple of 16 the pool is ``records [num_blocks, num_kv_heads, block_size / 16, 1664]``: 16-token tile
+    records, the layout the tensor-core attention kernel streams (a 16-token page is exactly one record per
+    head).  Otherwise the pool is the five row-major planes ``[num_blocks, num_kv_heads, block_size, row
+    bytes]`` (codes, sign bits) and ``[num_blocks, num_kv_heads, block_size]`` (norms) of the generic kernel.
+    """
+
+    def __init__(self, num_blocks: int, num_kv_heads: int, head_size: int,
+                 config: Optional[QuashKVPageConfig] = None, device="cuda", layer_idx: int = 0):
+        self.config = config or QuashKVPageConfig()
+        super().__init__(num_blocks, num_kv_heads, head_size, self.config.block_size, device)
+        self.engine = QuashKVEngine(head_dim=head_size, key_bits=self.config.key_bits,
+                                    value_bits=self.config.value_bits, seed=self.config.seed + layer_idx,
+                                    device=self.device)
+        pk, ps, pv = self.engine._row_bytes()
+        shape = (num_blocks, num_kv_heads, self.block_size)
+        u8 = dict(dtype=torch.uint8, device=self.device)
+        f32 = dict(dtype=torch.float32, device=self.device)
+        self.tiled = self.engine._tiled and self.block_size % ops.TILE_TOKENS == 0
+        if self.tiled:
+            self.planes = {"records": torch.zeros((num_blocks, num_kv_heads, self.block_size // ops.TILE_TOKENS,
+                                                   ops.TILE_BYTES), **u8)}
+        else:
+            self.planes = {
+                "k_codes": torch.zeros((*shape, pk), **u8), "k_signs": torch.zeros((*shape, ps), **u8),
+                "k_norms": torch.zeros(shape, **f32),
+                "v_codes": torch.zeros((*shape, pv), **u8), "v_norms": torch.zeros(shape, **f32),
+            }
 
     # ---- data path --------------------------------------------------------------------------------
     def append(self, seq_ids: Sequence, keys: torch.Tensor, values: torch.Tensor) -> None:

@@ -118,6 +118,16 @@ for _schema in (
         f"Tensor block_table, Tensor seq_lens, SymInt max_kv_len, SymInt key_bits, SymInt val_bits, {_CONSTS}) -> Tensor",
         f"attention_tiled({_TILED}) -> Tensor",
         f"attention_tiled_out({_TILED}, Tensor(a!) out) -> ()",
+        "append_paged8(Tensor keys, Tensor values, Tensor(a!) k_codes, Tensor(b!) v_codes, Tensor(c!) k_scales, Tensor(d!) v_scales, "
+        "Tensor? slots, Tensor? block_table, Tensor? start_lens) -> ()",
+        "attention_paged8(Tensor q, Tensor k_codes, Tensor v_codes, Tensor k_scales, Tensor v_scales, Tensor block_table, "
+        "Tensor seq_lens, SymInt max_kv_len, Tensor? query_starts, SymInt max_q_len, float scale, bool causal) -> Tensor",
+        "extend_pages(Tensor(a!) block_table, Tensor seq_lens, Tensor new_lens, Tensor free_pages, Tensor pool, SymInt block_size, "
+        "SymInt max_tokens) -> (Tensor, Tensor, Tensor, Tensor)",
+        "extend_pages_(Tensor(a!) block_table, Tensor(b!) seq_lens, Tensor new_lens, Tensor free_pages, Tensor(c!) pool, "
+        "SymInt block_size, SymInt max_tokens) -> (Tensor, Tensor, Tensor)",
+        "shrink_pages_(Tensor block_table, Tensor(a!) seq_lens, Tensor keep_lens, Tensor(b!) free_pages, Tensor(c!) pool, "
+        "SymInt block_size) -> ()",
         "index_scan_topk(Tensor queries, Tensor db_codes, Tensor db_signs, Tensor db_norms, SymInt n_vectors, SymInt bits, "
         "Tensor Pi, Tensor centroids, Tensor S, float qjl_scale, SymInt k, SymInt id_base) -> (Tensor, Tensor)"):
     _LIBRARY.define(_schema, tags=torch.Tag.pt2_compliant_tag)
@@ -406,6 +416,25 @@ def _(scores, ids, k):
     return scores.new_empty((M, k), dtype=torch.float32), ids.new_empty((M, k), dtype=torch.int64)
 
 
+@torch.library.register_fake("quashkv_b200::attention_paged8")
+def _(q, k_codes, v_codes, k_scales, v_scales, block_table, seq_lens, max_kv_len, query_starts, max_q_len, scale, causal):
+    return q.new_empty(q.shape, dtype=q.dtype if q.dtype in _DT else torch.float32)
+
+
+@torch.library.register_fake("quashkv_b200::extend_pages")
+def _(block_table, seq_lens, new_lens, free_pages, pool, block_size, max_tokens):
+    n = seq_lens.shape[0]
+    i32 = lambda *s: seq_lens.new_empty(s, dtype=torch.int32)      # noqa: E731
+    return seq_lens.new_empty((max_tokens,), dtype=torch.int64), i32(n + 1), i32(n), i32(2)
+
+
+@torch.library.register_fake("quashkv_b200::extend_pages_")
+def _(block_table, seq_lens, new_lens, free_pages, pool, block_size, max_tokens):
+    n = seq_lens.shape[0]
+    i32 = lambda *s: seq_lens.new_empty(s, dtype=torch.int32)      # noqa: E731
+    return seq_lens.new_empty((max_tokens,), dtype=torch.int64), i32(n + 1), i32(n)
+
+
 append_kv = _NATIVE.append_kv.default
 append_records = _NATIVE.append_records.default
 append_paged = _NATIVE.append_paged.default
@@ -414,6 +443,11 @@ attention = _NATIVE.attention.default
 attention_paged = _NATIVE.attention_paged.default
 attention_tiled = _attention_tiled = _NATIVE.attention_tiled.default
 attention_tiled_out = _NATIVE.attention_tiled_out.default
+append_paged8 = _NATIVE.append_paged8.default
+attention_paged8 = _NATIVE.attention_paged8.default
+extend_pages = _NATIVE.extend_pages.default
+extend_pages_ = _NATIVE.extend_pages_.default
+shrink_pages_ = _NATIVE.shrink_pages_.default
 index_scan_topk = _NATIVE.index_scan_topk.default
 _compress_mse = _NATIVE.compress_mse.default
 _compress_ip = _NATIVE.compress_ip.default
