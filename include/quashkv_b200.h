@@ -400,10 +400,12 @@ int64_t qkv_dropped_paged8_tokens(void);
  *              they were
  *   seq_lens   tokens held, clamped to max_kv_len and to the table; a block number outside the pool hides
  *              its tokens; bytes behind the last token may be anything; codes within hold no NaN
+ *   scale      any number;  scales of the pages: 0 or more, or NaN, which reaches what sees its page
  *   causal     query token t of n sits at position seq_lens[i] - n + t and sees positions up to its own
- * A row that sees nothing is zeros.  Any scales, 0 and NaN among them: NaN reaches what sees its page.
+ * A row that sees nothing is zeros.
  * Workspace: qkv_attention_paged8_workspace_bytes(...) bytes, 16-byte aligned. */
-size_t qkv_attention_paged8_workspace_bytes(int n_seq, int Hq, int Hkv, int q_len, int64_t max_kv_len, int d, int q_dtype);
+size_t qkv_attention_paged8_workspace_bytes(int n_seq, int Hq, int Hkv, int q_len, int ragged, int64_t total_q,
+                                            int64_t max_kv_len, int d, int q_dtype);
 int qkv_attention_paged8(const void* q, int q_dtype, const int64_t* q_strides, qkv_pages8_t pages,
                          const int32_t* block_table, int64_t table_stride, int max_blocks, const int32_t* seq_lens,
                          const int32_t* query_starts, int64_t total_q, int n_seq, int Hq, int q_len, int64_t max_kv_len,
@@ -463,8 +465,8 @@ int qkv_topk_merge(const float* in_scores, const int64_t* in_ids, int M, int64_t
 
 /* Diagnostics, no reference counterpart: how many bounded waits ran out on the current device since the
  * library was loaded: waits on the tcgen05 tensor core (a CTA that meets one finishes its work with the
- * fp32 CUDA-core arithmetic, so results stay correct) and waits on a record copy of
- * qkv_attention_tiled (that call's output is then not valid).  0 in a healthy run.  Synchronises the
+ * fp32 CUDA-core arithmetic, so results stay correct; qkv_attention_paged8 writes NaN to the rows of that
+ * CTA) and waits on a record copy of qkv_attention_tiled (that call's output is then not valid).  0 in a healthy run.  Synchronises the
  * device. */
 int64_t qkv_tensor_core_timeouts(void);
 

@@ -90,7 +90,7 @@ SIGNATURES = {
     "qkv_scatter_rows": (_i, [_vp, _vp, _vp, _i64, _i, _vp]),
     "qkv_append_paged8": (_i, [_vp, _vp, _i, C.POINTER(_i64), C.POINTER(_i64), _i64, _i64, Pages8, _vp, _vp, _i64, _i, _vp, _vp]),
     "qkv_dropped_paged8_tokens": (_i64, []),
-    "qkv_attention_paged8_workspace_bytes": (_sz, [_i, _i, _i, _i, _i64, _i, _i]),
+    "qkv_attention_paged8_workspace_bytes": (_sz, [_i, _i, _i, _i, _i, _i64, _i64, _i, _i]),
     "qkv_attention_paged8": (_i, [_vp, _i, C.POINTER(_i64), Pages8, _vp, _i64, _i, _vp, _vp, _i64, _i, _i, _i, _i64, _f, _i,
                                   _vp, C.POINTER(_i64), _vp, _sz, _vp]),
     "qkv_extend_pages": (_i, [_vp, _i64, _i, _vp, _vp, _vp, _i64, _vp, _i, _i, _i64, _vp, _vp, _vp, _vp, _vp, _vp]),

@@ -520,7 +520,7 @@ Tensor attention_paged8(const Tensor& q_in, const Tensor& k_codes, const Tensor&
   }
   const int64_t hq = q.size(1), q_len = ragged ? std::min(max_q_len, q.size(0)) : q.size(2);
   TORCH_CHECK_VALUE(hq * std::max<int64_t>(q_len, 1) <= INT32_MAX && n <= INT32_MAX && max_kv_len < INT32_MAX - 64, "quashkv_b200: sizes beyond 32 bits");
-  const int64_t need = api.qkv_attention_paged8_workspace_bytes(n, hq, pages.Hkv, q_len, max_kv_len, pages.d, dtype_code(q));
+  const int64_t need = api.qkv_attention_paged8_workspace_bytes(n, hq, pages.Hkv, q_len, ragged, ragged ? q.size(0) : 0, max_kv_len, pages.d, dtype_code(q));
   const Tensor ws = need > 0 ? empty({need}, at::kByte, dev) : Tensor();
   check(api.qkv_attention_paged8(q.const_data_ptr(), dtype_code(q), qs, pages, ip(table), table.stride(0), static_cast<int>(table.size(1)),
                                  ip(lens), ragged ? ip(starts) : nullptr, ragged ? q.size(0) : 0, static_cast<int>(n), static_cast<int>(hq),

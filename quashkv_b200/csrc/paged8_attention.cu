@@ -391,7 +391,7 @@ __global__ void __launch_bounds__(kWarps * 32) paged8_split_kernel(Attn8Args a) 
     if (a.n_splits == 1) {
       store_out8(a, s, h, rr, c, o, mt, Mt, lt);
     } else {
-      const int64_t slot = ((static_cast<int64_t>(seq) * a.Hkv + h) * a.most_rows + rr) * a.n_splits + blockIdx.y;
+      const int64_t slot = part_row8(a, s, seq, h, rr) * a.n_splits + blockIdx.y;
       *reinterpret_cast<float4*>(a.part + slot * D + c) = o;
       if (c == 0) *reinterpret_cast<float4*>(a.ref + slot * 4) = make_float4(mt, Mt, lt, 0.f);
     }
@@ -403,15 +403,37 @@ template <int D>
 __global__ void __launch_bounds__(128) paged8_merge_kernel(Attn8Args a) {
   const int lane = threadIdx.x & 31, c = 4 * lane;
   const int64_t job = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 5);
-  const int rr = static_cast<int>(job % a.most_rows);
-  const int64_t head = job / a.most_rows;
-  const int h = static_cast<int>(head % a.Hkv);
   asm volatile("griddepcontrol.wait;\n" ::: "memory");
-  if (head >= static_cast<int64_t>(a.n_seq) * a.Hkv) return;
-  const int seq = static_cast<int>(head / a.Hkv);
-  const Span8 s = span8(a, seq);
+  int seq, h, rr;
+  Span8 s;
+  if (a.by_token) {
+    const int hq = a.Hkv * a.G, head = static_cast<int>(job % hq);
+    const int64_t tok = job / hq;
+    if (tok >= (a.starts ? a.total_q : static_cast<int64_t>(a.n_seq) * a.q_len)) return;
+    if (a.starts) {                                        // the last sequence that starts at or in front of it
+      int lo = 0, hi = a.n_seq;
+      while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (a.starts[mid] <= tok) lo = mid; else hi = mid;
+      }
+      seq = lo;
+    } else {
+      seq = static_cast<int>(tok / a.q_len);
+    }
+    s = span8(a, seq);
+    if (tok < s.tok0 || tok - s.tok0 >= s.q_len) return;
+    h = head / a.G;
+    rr = static_cast<int>(tok - s.tok0) * a.G + head % a.G;
+  } else {
+    const int64_t head = job / a.most_rows;
+    if (head >= static_cast<int64_t>(a.n_seq) * a.Hkv) return;
+    rr = static_cast<int>(job % a.most_rows);
+    h = static_cast<int>(head % a.Hkv);
+    seq = static_cast<int>(head / a.Hkv);
+    s = span8(a, seq);
+  }
   const int rows = a.G * s.q_len;
-  if (rr >= rows || rows > a.most_rows) return;
+  if (rr >= rows || rows > a.most_rows || rows <= a.few_rows) return;
   const int tile_end = min((rr / a.tile_rows + 1) * a.tile_rows, rows);
   const int64_t end = visible8(a, s, (tile_end - 1) / a.G);
   const int parts = end > a.chunk ? static_cast<int>((end + a.chunk - 1) / a.chunk) : 1;
@@ -441,12 +463,15 @@ __global__ void __launch_bounds__(128) paged8_merge_kernel(Attn8Args a) {
   if (c < D) store_out8(a, s, h, rr, c, o, mt, Mt, lt);
 }
 
-// How the tokens are split: see plan8.
-struct Plan8 { int ng, row_tiles, most_rows, n_splits; int64_t chunk; size_t ws; };
+// How a call is carried out.  Sequences of up to `few` rows (query tokens x query heads of a KV head) go to the split kernel,
+// those of more to the prefill kernel where it exists (head size 64 and 128, 16-bit queries).
+constexpr int kFewRows = 32;
 
-Plan8 plan8(int n_seq, int Hkv, int G, int q_len, int64_t max_kv_len, int d, int dtype) {
+struct Plan8 { int ng, row_tiles, most_rows, n_splits; int64_t chunk, part_rows; size_t ws; };
+
+Plan8 plan_split(int n_seq, int Hkv, int most_rows, int64_t max_kv_len, int d, int dtype) {
   Plan8 p;
-  p.most_rows = G * q_len;
+  p.most_rows = most_rows;
   p.ng = dtype != QKV_F32 && p.most_rows > 8 ? 2 : 1;
   p.row_tiles = (p.most_rows + 8 * p.ng - 1) / (8 * p.ng);
   const int64_t items = static_cast<int64_t>(n_seq) * Hkv * p.row_tiles, wave = 3 * kNumSMs;
@@ -460,21 +485,51 @@ Plan8 plan8(int n_seq, int Hkv, int G, int q_len, int64_t max_kv_len, int d, int
   if (p.chunk < 64) p.chunk = 64;
   p.n_splits = static_cast<int>((max_kv_len + p.chunk - 1) / p.chunk);
   if (p.n_splits < 1) p.n_splits = 1;
-  const size_t slots = static_cast<size_t>(n_seq) * Hkv * p.most_rows * p.n_splits;
-  p.ws = p.n_splits > 1 ? slots * (d + 4) * sizeof(float) : 0;
+  p.part_rows = static_cast<int64_t>(n_seq) * Hkv * p.most_rows;
+  p.ws = p.n_splits > 1 ? static_cast<size_t>(p.part_rows) * p.n_splits * (d + 4) * sizeof(float) : 0;
   return p;
 }
 
-template <int D, int CODE, int QT, int NG>
-int launch_split(const Attn8Args& a, int64_t items, cudaStream_t st) {
-  using P = Split<D, QT, NG>;
-  auto kernel = paged8_split_kernel<D, CODE, QT, NG>;
-  if (P::kSmem > 48 * 1024 && cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(P::kSmem)) != cudaSuccess)
-    return QKV_ELAUNCH;
-  kernel<<<dim3(static_cast<unsigned>(items), a.n_splits), kWarps * 32, P::kSmem, st>>>(a);
-  if (const int rc = check_launch()) return rc;
+// `tokens`: query tokens of all sequences.
+Plan8 plan_prefill(int Hkv, int G, int q_len, int64_t tokens, int64_t max_kv_len, int d) {
+  Plan8 p{};
+  p.most_rows = G * q_len;
+  p.row_tiles = (p.most_rows + 255) / 256;
+  const int64_t ctas = (tokens * G + 255) / 256 * Hkv;
+  int64_t splits = ctas > 0 ? kNumSMs / ctas : 1;
+  const int64_t most = max_kv_len / 512;
+  if (splits > most) splits = most;
+  if (splits > 32) splits = 32;
+  if (splits < 1) splits = 1;
+  p.chunk = (max_kv_len + splits - 1) / splits;
+  p.chunk = (p.chunk + 127) / 128 * 128;
+  if (p.chunk < 128) p.chunk = 128;
+  p.n_splits = static_cast<int>((max_kv_len + p.chunk - 1) / p.chunk);
+  if (p.n_splits < 1) p.n_splits = 1;
+  p.part_rows = tokens * Hkv * G;
+  p.ws = p.n_splits > 1 ? static_cast<size_t>(p.part_rows) * p.n_splits * (d + 4) * sizeof(float) : 0;
+  return p;
+}
+
+struct Route8 { bool split, prefill; Plan8 s, p; size_t ws; };
+
+Route8 route8(int n_seq, int Hkv, int G, int q_len, bool ragged, int64_t tokens, int64_t max_kv_len, int d, int dtype) {
+  Route8 r{};
+  const int rows = G * q_len;
+  r.prefill = rows > kFewRows && dtype != QKV_F32 && (d == 64 || d == 128);
+  r.split = !r.prefill || (ragged && G <= kFewRows);
+  if (r.split) r.s = plan_split(n_seq, Hkv, r.prefill ? kFewRows : rows, max_kv_len, d, dtype);
+  if (r.prefill) r.p = plan_prefill(Hkv, G, q_len, tokens, max_kv_len, d);
+  r.ws = r.s.ws > r.p.ws ? r.s.ws : r.p.ws;                // one after the other in the same place
+  return r;
+}
+
+template <int D>
+int launch_merge(const Attn8Args& a, cudaStream_t st) {
   if (a.n_splits == 1) return QKV_OK;
-  const int64_t rows = static_cast<int64_t>(a.n_seq) * a.Hkv * a.most_rows;
+  const int64_t rows = a.by_token ? (a.starts ? a.total_q : static_cast<int64_t>(a.n_seq) * a.q_len) * a.Hkv * a.G
+                                  : static_cast<int64_t>(a.n_seq) * a.Hkv * a.most_rows;
+  if ((rows + 3) / 4 > 0x7fffffffLL) return QKV_EDIM;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>((rows + 3) / 4));
   cfg.blockDim = dim3(128);
@@ -486,6 +541,17 @@ int launch_split(const Attn8Args& a, int64_t items, cudaStream_t st) {
   cfg.numAttrs = 1;
   if (cudaLaunchKernelEx(&cfg, paged8_merge_kernel<D>, a) != cudaSuccess) return QKV_ELAUNCH;
   return check_launch();
+}
+
+template <int D, int CODE, int QT, int NG>
+int launch_split(const Attn8Args& a, int64_t items, cudaStream_t st) {
+  using P = Split<D, QT, NG>;
+  auto kernel = paged8_split_kernel<D, CODE, QT, NG>;
+  if (P::kSmem > 48 * 1024 && cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(P::kSmem)) != cudaSuccess)
+    return QKV_ELAUNCH;
+  kernel<<<dim3(static_cast<unsigned>(items), a.n_splits), kWarps * 32, P::kSmem, st>>>(a);
+  if (const int rc = check_launch()) return rc;
+  return launch_merge<D>(a, st);
 }
 
 template <int D, int CODE>
@@ -508,9 +574,10 @@ bool sizes_ok(int n_seq, int Hq, int Hkv, int q_len, int64_t max_kv_len) {
 
 using namespace qkv;
 
-extern "C" size_t qkv_attention_paged8_workspace_bytes(int n_seq, int Hq, int Hkv, int q_len, int64_t max_kv_len, int d, int q_dtype) {
-  if (!sizes_ok(n_seq, Hq, Hkv, q_len, max_kv_len) || n_seq == 0 || q_len == 0) return 0;
-  return plan8(n_seq, Hkv, Hq / Hkv, q_len, max_kv_len, d, q_dtype).ws;
+extern "C" size_t qkv_attention_paged8_workspace_bytes(int n_seq, int Hq, int Hkv, int q_len, int ragged, int64_t total_q,
+                                                       int64_t max_kv_len, int d, int q_dtype) {
+  if (!sizes_ok(n_seq, Hq, Hkv, q_len, max_kv_len) || n_seq == 0 || q_len == 0 || total_q < 0) return 0;
+  return route8(n_seq, Hkv, Hq / Hkv, q_len, ragged != 0, ragged ? total_q : static_cast<int64_t>(n_seq) * q_len, max_kv_len, d, q_dtype).ws;
 }
 
 extern "C" int qkv_attention_paged8(const void* q, int q_dtype, const int64_t* q_strides, qkv_pages8_t pages,
@@ -550,23 +617,39 @@ extern "C" int qkv_attention_paged8(const void* q, int q_dtype, const int64_t* q
   a.scale = scale;
   a.out = out;
   a.bs_shift = (pages.block_size & (pages.block_size - 1)) == 0 ? __builtin_ctz(pages.block_size) : -1;
-  const Plan8 p = plan8(n_seq, a.Hkv, a.G, q_len, max_kv_len, pages.d, q_dtype);
-  if (p.ws > workspace_bytes || (p.ws > 0 && !workspace)) return QKV_EWORKSPACE;
+  const Route8 r = route8(n_seq, a.Hkv, a.G, q_len, query_starts != nullptr, query_starts ? total_q : static_cast<int64_t>(n_seq) * q_len,
+                          max_kv_len, pages.d, q_dtype);
+  if (r.ws > workspace_bytes || (r.ws > 0 && !workspace)) return QKV_EWORKSPACE;
   if (reinterpret_cast<uintptr_t>(workspace) & 15u) return QKV_EALIGN;
-  const int64_t items = static_cast<int64_t>(n_seq) * a.Hkv * p.row_tiles;
-  if (items > 0x7fffffffLL || static_cast<int64_t>(n_seq) * a.Hkv * p.most_rows > 0x7fffffffLL) return QKV_EDIM;
-  a.row_tiles = p.row_tiles;
-  a.tile_rows = 8 * p.ng;
-  a.most_rows = p.most_rows;
-  a.n_splits = p.n_splits;
-  a.chunk = p.chunk;
-  a.part = static_cast<float*>(workspace);
-  a.ref = a.part + static_cast<size_t>(n_seq) * a.Hkv * p.most_rows * p.n_splits * pages.d;
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
+  auto with = [&](const Plan8& p) {
+    Attn8Args b = a;
+    b.row_tiles = p.row_tiles;
+    b.most_rows = p.most_rows;
+    b.n_splits = p.n_splits;
+    b.chunk = p.chunk;
+    b.part = static_cast<float*>(workspace);
+    b.ref = b.part + static_cast<size_t>(p.part_rows) * p.n_splits * pages.d;
+    return b;
+  };
+  if (r.prefill) {
+    Attn8Args b = with(r.p);
+    b.tile_rows = 256;
+    b.by_token = 1;
+    b.few_rows = r.split ? kFewRows : 0;
+    if (static_cast<int64_t>(n_seq) * a.Hkv > 0x7fffffffLL || b.row_tiles > 65535) return QKV_EDIM;
+    if (const int rc = launch_prefill8(b, st)) return rc;
+    if (const int rc = pages.d == 64 ? launch_merge<64>(b, st) : launch_merge<128>(b, st)) return rc;
+  }
+  if (!r.split) return QKV_OK;
+  Attn8Args b = with(r.s);
+  b.tile_rows = 8 * r.s.ng;
+  const int64_t items = static_cast<int64_t>(n_seq) * a.Hkv * r.s.row_tiles;
+  if (items > 0x7fffffffLL) return QKV_EDIM;
   switch (pages.d) {
-    case 32: return launch_codes<32>(a, p.ng, items, st);
-    case 64: return launch_codes<64>(a, p.ng, items, st);
-    case 96: return launch_codes<96>(a, p.ng, items, st);
-    default: return launch_codes<128>(a, p.ng, items, st);
+    case 32: return launch_codes<32>(b, r.s.ng, items, st);
+    case 64: return launch_codes<64>(b, r.s.ng, items, st);
+    case 96: return launch_codes<96>(b, r.s.ng, items, st);
+    default: return launch_codes<128>(b, r.s.ng, items, st);
   }
 }

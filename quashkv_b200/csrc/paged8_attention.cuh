@@ -19,11 +19,17 @@ struct Attn8Args {
   float scale;
   void* out;
   int row_tiles, tile_rows, most_rows, n_splits; int64_t chunk;
-  float* part; float* ref;                  // [seq][kv head][most_rows][n_splits] sums, and their (m, M, l, -)
+  float* part; float* ref;                  // [row][n_splits] sums, and their (m, M, l, -); rows as part_row8 numbers them
+  int few_rows;                             // sequences of no more rows (query tokens x heads of a KV head) are not this kernel's,
+  int by_token;                             // most_rows: nor are those of more.  by_token: see part_row8
+  int test_drop_mma;                        // test hook of the prefill kernel
 };
 
+int launch_prefill8(const Attn8Args& a, cudaStream_t st);
+unsigned int prefill8_timeouts();
+
 // Tokens and queries of a sequence, within what the host has promised.
-struct Span8 { int64_t len; int q_len, q_all; int64_t q_row0, o_row0; };
+struct Span8 { int64_t len, tok0; int q_len, q_all; int64_t q_row0, o_row0; };      // tok0: query tokens in front of it
 
 __device__ __forceinline__ Span8 span8(const Attn8Args& a, int seq) {
   Span8 s;
@@ -32,11 +38,13 @@ __device__ __forceinline__ Span8 span8(const Attn8Args& a, int seq) {
     const int64_t lo = min(static_cast<int64_t>(max(a.starts[seq], 0)), a.total_q);
     const int64_t hi = min(max(static_cast<int64_t>(a.starts[seq + 1]), lo), a.total_q);
     s.q_all = static_cast<int>(hi - lo);
+    s.tok0 = lo;
     s.q_len = min(s.q_all, a.q_len);
     s.q_row0 = lo * a.q_stride[1];
     s.o_row0 = lo * a.o_stride[1];
   } else {
     s.q_len = s.q_all = a.q_len;
+    s.tok0 = static_cast<int64_t>(seq) * a.q_len;
     s.q_row0 = seq * a.q_stride[0];
     s.o_row0 = seq * a.o_stride[0];
   }
@@ -48,6 +56,13 @@ __device__ __forceinline__ int64_t visible8(const Attn8Args& a, const Span8& s, 
   if (!a.causal) return s.len;
   const int64_t v = s.len - s.q_all + tok + 1;
   return v < 0 ? 0 : (v > s.len ? s.len : v);
+}
+
+// Row r of KV head h among the partial results: places for most_rows rows of every sequence and head, or, where sequences differ
+// much in their rows, for the query tokens that there are.
+__device__ __forceinline__ int64_t part_row8(const Attn8Args& a, const Span8& s, int seq, int h, int r) {
+  if (a.by_token) return (s.tok0 + r / a.G) * (static_cast<int64_t>(a.Hkv) * a.G) + h * a.G + r % a.G;
+  return (static_cast<int64_t>(seq) * a.Hkv + h) * a.most_rows + r;
 }
 
 // 2^(K - e) for a magnitude 2^e <= x < 2^(e+1): x times it lies in [2^K, 2^(K+1)).  A normal number, and so is its inverse.

@@ -97,7 +97,7 @@ def attention_paged8(queries: torch.Tensor, k_codes: torch.Tensor, v_codes: torc
     int32 with ``max_kv_len`` an upper bound of them known on the host; with ``causal`` the queries of a sequence are its
     last positions.  Rows that see nothing, and rows of no sequence, are zeros.
 
-    Scales may be any numbers; codes must not hold NaN within a sequence's length, and may be anything behind it.  A
+    Scales are 0 or more, or NaN, which reaches what sees the page; codes must not hold NaN within a sequence's length, and may be anything behind it.  A
     block number outside the pool hides its tokens."""
     ops._need_cuda(queries, "attention_paged8")
     if scale is None:

@@ -298,6 +298,43 @@ def test_attention_over_a_long_cache():
         _check_attention(torch.randn(64, H * G, 1, d, generator=g, device=DEV).to(x_dtype), pages, table, _i32(lens))
 
 
+@pytest.mark.parametrize("x_dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("d,H,G,q_len", [(128, 2, 4, 70), (64, 1, 8, 33), (128, 1, 1, 257), (64, 2, 40, 1), (128, 1, 40, 3)])
+def test_pieces_of_prompts_over_a_long_cache(d, H, G, q_len, x_dtype):
+    """Few query rows over many tokens, so that the tokens are split; many token tiles in a row; more heads than a tile of
+    rows; a scale below zero."""
+    g = torch.Generator(device=DEV).manual_seed(q_len)
+    bs, lens = 48, [5000, 130, 2100]
+    total = sum(-(-n // bs) for n in lens) + 2
+    pages = ref.random_pages(g, total, H, bs, d, E4M3, "nhd")
+    table = ref.random_tables(lens, bs, total, q_len).to(DEV)
+    q = torch.randn(3, H * G, q_len, d, generator=g, device=DEV).to(x_dtype)
+    _check_attention(q, pages, table, _i32(lens), scale=-0.1)
+    starts = [0, q_len, q_len + 1, 2 * q_len + 1]
+    flat = q.transpose(1, 2).reshape(-1, H * G, d)[:starts[-1] + 2].contiguous()
+    _check_attention(flat, pages, table, _i32(lens), starts=starts, max_q_len=q_len)
+
+
+def test_a_wait_that_runs_out_gives_nan_and_is_counted(monkeypatch):
+    """The first CTA leaves out the products of one tile (nothing is left in flight): its waits give up, its rows are NaN
+    and no others, and the context stays usable."""
+    from quashkv_b200 import _lib
+    g = torch.Generator(device=DEV).manual_seed(1)
+    pages = ref.random_pages(g, 80, 2, 16, 128, E4M3)
+    table = ref.random_tables([600, 500], 16, 80, 1).to(DEV)
+    q = torch.randn(2, 4, 300, 128, generator=g, device=DEV).bfloat16()
+    want = paged8.attention_paged8(q, *pages, table, _i32([600, 500]), 600, causal=True)
+    before = _lib.lib().qkv_tensor_core_timeouts()
+    monkeypatch.setenv("QUASHKV_B200_TEST_DROP_MMA", "1")
+    got = paged8.attention_paged8(q, *pages, table, _i32([600, 500]), 600, causal=True)
+    torch.cuda.synchronize()
+    monkeypatch.delenv("QUASHKV_B200_TEST_DROP_MMA")
+    assert _lib.lib().qkv_tensor_core_timeouts() > before
+    bad = got.isnan().all(-1)
+    assert bad.any() and not bad[1].any() and not bad[0, 2:].any() and torch.equal(got[~bad], want[~bad])
+    assert torch.equal(paged8.attention_paged8(q, *pages, table, _i32([600, 500]), 600, causal=True), want)
+
+
 @pytest.mark.parametrize("q_len", [1, 90])
 @pytest.mark.parametrize("x_dtype", [torch.bfloat16, torch.float32])
 def test_what_is_hidden_may_be_anything(q_len, x_dtype):

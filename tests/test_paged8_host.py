@@ -71,8 +71,8 @@ def test_bad_arguments_are_refused_without_launching():
     assert attend(q=at8) == -5 and attend(os_=odd3) == -5 and attend(ws=at8, kv=4096) == -5
     assert attend(kv=4096, size=16) == -6 and attend(kv=4096, ws=None) == -6
     assert attend(n=0) == 0 and attend(q_len=0) == 0                        # nothing to do
-    assert L.qkv_attention_paged8_workspace_bytes(1, 32, 8, 1, 4096, 128, 1) > 0
-    assert L.qkv_attention_paged8_workspace_bytes(1, 7, 2, 1, 4096, 128, 1) == 0
+    assert L.qkv_attention_paged8_workspace_bytes(1, 32, 8, 1, 0, 0, 4096, 128, 1) > 0
+    assert L.qkv_attention_paged8_workspace_bytes(1, 7, 2, 1, 0, 0, 4096, 128, 1) == 0
 
     def extend(table=one, stride=8, blocks=8, n=4, bs=16, tokens=10, slots=one, pool=one, free=4):
         return L.qkv_extend_pages(table, stride, blocks, one, one, one, free, pool, n, bs, tokens, slots, one, one, None, one, None)
