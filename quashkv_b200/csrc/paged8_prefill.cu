@@ -3,7 +3,7 @@
 //
 // A CTA holds 256 query rows of one (sequence, KV head), a row being a query token and one of the head's query heads, as
 // two row tiles of 128 (the M of an MMA), and goes over tokens in tiles of 128:
-//   warps 9-11   bring the codes of a tile from their pages (cp.async) and turn them into fp16 operands in the swizzled
+//   warps 9-15   bring the codes of a tile from their pages (cp.async) and turn them into fp16 operands in the swizzled
 //                order of the tensor core; both K and V as they lie in memory, a row a token: the scores read K with the
 //                inner dimension contiguous, the second product reads V with the outer one contiguous, so nothing is
 //                transposed
@@ -11,7 +11,7 @@
 //                into an accumulator that stays in tensor memory over the whole sequence
 //   warps 0-7    a thread per query row: scores of a tile from tensor memory, softmax, weights as fp16 in their place
 // The tensor core works for one row tile while the softmax of the other runs.  Rows hold two whole-number reference
-// exponents as in the split kernel, which rise only when a score passes them by 2^4; only then is the accumulator
+// exponents as in the split kernel, which rise only when a score passes them by 2^8; only then is the accumulator
 // rescaled (exactly), by the row's own thread.
 //
 // Precision: codes are exact in fp16, 16-bit queries too (scaled by a power of two per row); weights are rounded to
@@ -33,7 +33,8 @@ namespace qkv {
 namespace {
 
 constexpr int kTok = 128, kRowsT = 128, kStages = 2, kMetaSlots = 4, kGroups = kTok / 16;
-constexpr float kNone = -1e30f, kSlack = 4.f, kLift = 10.f;
+constexpr int kThreads = 512, kConverters = 7;             // warps that turn codes into operands
+constexpr float kNone = -1e30f, kSlack = 8.f, kLift = 6.f;      // weights reach 2^15 and the largest is at least 2^5
 __device__ unsigned int g_prefill8_timeouts = 0;
 
 struct TileMeta { float ks[kGroups], ex[kGroups], mant[kGroups]; uint32_t bad; uint32_t pad[7]; };   // per group of 16 tokens
@@ -69,8 +70,129 @@ __device__ __forceinline__ uint64_t smem_desc_outer(uint32_t smem_addr, uint32_t
 }
 constexpr uint32_t kOuterB = 1u << 16;                     // instruction descriptor: operand B has its outer dimension contiguous
 
+// Waits for a phase; a thread that finds it incomplete sleeps until it ends, for at most a millisecond at a time (polling took
+// more issue slots than the work).  Gives up after about 0.2 s, or once another wait of the CTA has.
+__device__ __forceinline__ bool sleep_on(uint64_t* bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\tselp.u32 %0, 1, 0, p;\n\t}\n"
+               : "=r"(ok) : "r"(umma::smem_u32(bar)), "r"(parity), "r"(1000000u) : "memory");
+  return ok != 0;
+}
+__device__ __forceinline__ bool wait_on(uint64_t* bar, uint32_t parity, volatile int* dead) {
+  const long long t0 = clock64();
+  while (!*dead) {
+    if (sleep_on(bar, parity)) return true;
+    if (clock64() - t0 > 400000000LL) {
+      *dead = 1;
+      atomicAdd(&g_prefill8_timeouts, 1u);
+    }
+  }
+  return false;
+}
+
+__device__ __forceinline__ bool elect_one() {
+  uint32_t one;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}\n" : "=r"(one));
+  return one != 0;
+}
+
+// Two fp32 numbers in one register pair.
+__device__ __forceinline__ uint64_t pair(float lo, float hi) {
+  uint64_t d;
+  asm("mov.b64 %0, {%1, %2};\n" : "=l"(d) : "f"(lo), "f"(hi));
+  return d;
+}
+__device__ __forceinline__ float2 both(uint64_t x) {
+  float2 d;
+  asm("mov.b64 {%0, %1}, %2;\n" : "=f"(d.x), "=f"(d.y) : "l"(x));
+  return d;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;\n" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+  return d;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("mul.rn.f32x2 %0, %1, %2;\n" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("add.rn.f32x2 %0, %1, %2;\n" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+__device__ __forceinline__ uint32_t ex2v(uint32_t x) {      // keeps its place in the order of the source
+  float y;
+  asm volatile("ex2.approx.ftz.f32 %0, %1;\n" : "=f"(y) : "f"(__uint_as_float(x)));
+  return __float_as_uint(y);
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float d;
+  asm("max.f32 %0, %1, %2, %3;\n" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+
+// Where row r of a CTA's (sequence, KV head) lies in the queries or the output, in elements.
+__device__ __forceinline__ int64_t row_at(const Attn8Args& a, int64_t row0, const int64_t* stride, int h, int r) {
+  const int tok = r / a.G;
+  return row0 + tok * stride[1] + (h * a.G + r - tok * a.G) * stride[2];
+}
+
+// The 32 query rows of a warp as fp16 operands, each scaled by a power of two (and turned round for a negative scale of the
+// scores): D / 8 lanes fetch a row.  Returns the score in base 2 that one unit of a product stands
+// for in the lane's own row.
+template <int D, bool BF16>
+__device__ __forceinline__ float stage_queries(const Attn8Args& a, const Span8& s, int h, int first, int r_end, unsigned char* dst, int row0) {
+  constexpr int kLanes = D / 8, kRows = 32 / kLanes;
+  const int lane = threadIdx.x & 31, sub = lane / kLanes, c = lane % kLanes;
+  auto values = [](uint32_t x) {
+    return BF16 ? make_float2(__uint_as_float(x << 16), __uint_as_float(x & 0xffff0000u)) : __half22float2(*reinterpret_cast<const __half2*>(&x));
+  };
+  // (cp.async, because the little that is left of L1 beside the operands holds up loads that pass through it)
+  const int64_t mine = row_at(a, s.q_row0, a.q_stride, h, first + lane < r_end ? first + lane : first);
+#pragma unroll 4
+  for (int i = 0; i < kLanes; ++i) {
+    const int k = kRows * i + sub;
+    const int64_t at = __shfl_sync(QKV_FULL_MASK, mine, k);
+    cp_async16(dst + umma::sw128_offset(row0 + k, 8 * c, kRowsT), static_cast<const uint16_t*>(a.q) + at + 8 * c, first + k < r_end ? 16 : 0);
+  }
+  cp_async_commit();
+  cp_async_wait<0>();
+  // Each step for all rows, so that none waits for the one before.  A thread turns the chunks that it copied.
+  float mx[kLanes];
+  auto chunk = [&](int i) { return reinterpret_cast<uint4*>(dst + umma::sw128_offset(row0 + kRows * i + sub, 8 * c, kRowsT)); };
+#pragma unroll
+  for (int i = 0; i < kLanes; ++i) {
+    const uint4 w = *chunk(i);
+    const float2 v0 = values(w.x), v1 = values(w.y), v2 = values(w.z), v3 = values(w.w);
+    mx[i] = max3(max3(fabsf(v0.x), fabsf(v0.y), fabsf(v1.x)), max3(fabsf(v1.y), fabsf(v2.x), fabsf(v2.y)), fmaxf(fabsf(v3.x), fabsf(v3.y)));
+  }
+#pragma unroll
+  for (int o = 1; o < kLanes; o <<= 1)
+#pragma unroll
+    for (int i = 0; i < kLanes; ++i) mx[i] = fmaxf(mx[i], __shfl_xor_sync(QKV_FULL_MASK, mx[i], o));
+  float unit = 0.f;
+#pragma unroll
+  for (int i = 0; i < kLanes; ++i) {
+    const float up = scale_to8<13>(mx[i]), sg = a.scale < 0.f ? -up : up;
+    const uint4 w = *chunk(i);
+    const uint32_t y[4] = {w.x, w.y, w.z, w.w};
+    uint32_t x[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const float2 v = values(y[e]);
+      x[e] = pack_half2(v.x * sg, v.y * sg);
+    }
+    *chunk(i) = make_uint4(x[0], x[1], x[2], x[3]);
+    const float u = __shfl_sync(QKV_FULL_MASK, up, lane % kRows * kLanes);
+    if (lane / kRows == i) unit = fabsf(a.scale) * 1.4426950408889634f * inverse8(u);
+  }
+  return unit;
+}
+
 template <int D, int CODE>
-__global__ void __launch_bounds__(384, 1) paged8_prefill_kernel(Attn8Args a) {
+__global__ void __launch_bounds__(kThreads, 1) paged8_prefill_kernel(Attn8Args a) {
   using P = Pf8<D>;
   extern __shared__ __align__(1024) unsigned char smem[];
   unsigned char* q_s = smem;                                               // [2]
@@ -79,7 +201,7 @@ __global__ void __launch_bounds__(384, 1) paged8_prefill_kernel(Attn8Args a) {
   unsigned char* raw_s = v_s + kStages * P::kOpBytes;                      // codes of one K and one V tile
   TileMeta* meta = reinterpret_cast<TileMeta*>(raw_s + 2 * P::kRawBytes);  // [kMetaSlots]
   uint64_t* bars = reinterpret_cast<uint64_t*>(meta + kMetaSlots);
-  uint64_t* k_full = bars;                  // [2] 96 threads have stored their part
+  uint64_t* k_full = bars;                  // [2] every converter thread has stored its part
   uint64_t* v_full = bars + 2;              // [2]
   uint64_t* k_free = bars + 4;              // [2] its MMAs have read it
   uint64_t* v_free = bars + 6;              // [2]
@@ -103,7 +225,7 @@ __global__ void __launch_bounds__(384, 1) paged8_prefill_kernel(Attn8Args a) {
   const int n = stop > begin ? static_cast<int>((stop - begin + kTok - 1) / kTok) : 0;
 
   if (tid == 0) {
-    for (int i = 0; i < 19; ++i) umma::mbar_init(bars + i, i < 4 ? 96 : (i == 10 || i == 11 ? kRowsT : 1));
+    for (int i = 0; i < 19; ++i) umma::mbar_init(bars + i, i < 4 ? 32 * kConverters : (i == 10 || i == 11 ? kRowsT : 1));
     asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
     *dead = 0;
   }
@@ -111,75 +233,74 @@ __global__ void __launch_bounds__(384, 1) paged8_prefill_kernel(Attn8Args a) {
   umma::fence_before_sync();
   __syncthreads();
   umma::fence_after_sync();
-  const uint32_t tmem = *tmem_slot;
-  auto wait = [&](uint64_t* bar, uint32_t parity) {                        // bounded; false once anything ran out
-    if (*dead) return false;
-    if (umma::mbar_wait(bar, parity)) return true;
-    *dead = 1;
-    atomicAdd(&g_prefill8_timeouts, 1u);
-    return false;
+  constexpr uint32_t tmem = 0;              // all 512 columns of it are this CTA's
+  auto wait = [&](uint64_t* bar, uint32_t parity) {                        // bounded; false when it, or another one, ran out
+    return sleep_on(bar, parity) || wait_on(bar, parity, dead);
   };
   auto wait_all = [&](uint64_t* bar, uint32_t parity) { return __all_sync(QKV_FULL_MASK, wait(bar, parity)) != 0; };
 
   if (warp >= 8) {
-    // 384 threads start with 168 registers; 256 x 200 + 128 x 104 = 384 x 168
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 104;\n");
+    // 512 threads start with 128 registers; 256 x 192 + 256 x 64 = 512 x 128
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 64;\n");
     if (warp == 8) {
-      if (lane == 0) {
-        // ---- MMAs ----
-        constexpr uint32_t id_s = umma::instr_desc(umma::kFmtF16, 128, kTok), id_o = umma::instr_desc(umma::kFmtF16, 128, D) | kOuterB;
-        auto scores = [&](int t, int j) {
-          const uint32_t qa = umma::smem_u32(q_s + t * P::kQBytes), ka = umma::smem_u32(k_s + (j % kStages) * P::kOpBytes);
+      // ---- MMAs: the warp goes through this as one, one of its threads issues ----
+      constexpr uint32_t id_s = umma::instr_desc(umma::kFmtF16, 128, kTok), id_o = umma::instr_desc(umma::kFmtF16, 128, D) | kOuterB;
+      const bool leader = elect_one();
+      const uint64_t q_desc = umma::smem_desc_sw128(umma::smem_u32(q_s)), k_desc = umma::smem_desc_sw128(umma::smem_u32(k_s));
+      const uint64_t v_desc = smem_desc_outer(umma::smem_u32(v_s), kTok * 128);
+      auto scores = [&](int t, int j) {
+        const uint64_t qd = q_desc + t * (P::kQBytes >> 4), kd = k_desc + (j % kStages) * (P::kOpBytes >> 4);
+        if (leader) {
 #pragma unroll
           for (int k = 0; k < D / 16; ++k)
-            umma::mma_f16(tmem + kTok * t, umma::smem_desc_sw128(qa + (k >> 2) * (kRowsT * 128) + (k & 3) * 32),
-                          umma::smem_desc_sw128(ka + (k >> 2) * (kTok * 128) + (k & 3) * 32), id_s, k != 0);
+            umma::mma_f16(kTok * t, qd + (((k >> 2) * (kRowsT * 128) + (k & 3) * 32) >> 4), kd + (((k >> 2) * (kTok * 128) + (k & 3) * 32) >> 4), id_s, k != 0);
           umma::commit(s_full + t);
           if (t == nt - 1) umma::commit(k_free + j % kStages);
-        };
-        auto values = [&](int t, int j) {
-          const uint32_t va = umma::smem_u32(v_s + (j % kStages) * P::kOpBytes);
+        }
+        __syncwarp();
+      };
+      auto values = [&](int t, int j) {
+        const uint64_t vd = v_desc + (j % kStages) * (P::kOpBytes >> 4);
+        if (leader) {
 #pragma unroll
           for (int k = 0; k < kTok / 16; ++k)
-            umma::mma_f16_ts(tmem + P::kO + 128 * t, tmem + kTok * t + 8 * k, smem_desc_outer(va + k * 2048, kTok * 128), id_o, j != 0 || k != 0);
+            umma::mma_f16_ts(P::kO + kTok * t, kTok * t + 8 * k, vd + (k * 2048 >> 4), id_o, j != 0 || k != 0);
           if (t == nt - 1) umma::commit(v_free + j % kStages);
-        };
-        bool ok = true;
-        for (int t = 0; t < nt && ok; ++t) ok = wait(p_ready + t, 0);
-        if (n > 0 && ok && (ok = wait(k_full, 0))) {
-          umma::fence_after_sync();
-          for (int t = 0; t < nt; ++t) scores(t, 0);
+          if (j + 1 == n) umma::commit(o_full + t);
         }
-        for (int j = 0; j < n && ok; ++j)
-          for (int t = 0; t < nt && ok; ++t) {
-            if (!(ok = wait(p_ready + t, (j + 1) & 1))) break;
-            if (t == 0 && !(ok = wait(v_full + j % kStages, (j / kStages) & 1))) break;
-            if (a.test_drop_mma && (blockIdx.x | blockIdx.y | blockIdx.z) == 0 && t == 0 && j == 1) continue;      // test hook
-            umma::fence_after_sync();
-            values(t, j);
-            if (j + 1 == n) {
-              umma::commit(o_full + t);
-            } else {
-              if (t == 0 && !(ok = wait(k_full + (j + 1) % kStages, ((j + 1) / kStages) & 1))) break;
-              umma::fence_after_sync();
-              scores(t, j + 1);
-            }
+        __syncwarp();
+      };
+      bool ok = true;
+      for (int t = 0; t < nt && ok; ++t) ok = wait_all(p_ready + t, 0);
+      if (n > 0 && ok && (ok = wait_all(k_full, 0))) {
+        umma::fence_after_sync();
+        for (int t = 0; t < nt; ++t) scores(t, 0);
+      }
+      for (int j = 0; j < n && ok; ++j)
+        for (int t = 0; t < nt && ok; ++t) {
+          if (t == 0) {                     // the operands are there long before the weights
+            ok = wait_all(v_full + j % kStages, (j / kStages) & 1) && (j + 1 == n || wait_all(k_full + (j + 1) % kStages, ((j + 1) / kStages) & 1));
+            if (!ok) break;
           }
-        if (!ok) {                          // whatever was issued has ended before tensor memory is given back
-          umma::commit(drain);
-          umma::mbar_wait(drain, 0);
+          if (!(ok = wait_all(p_ready + t, (j + 1) & 1))) break;
+          if (a.test_drop_mma && (blockIdx.x | blockIdx.y | blockIdx.z) == 0 && t == 0 && j == 1) continue;      // test hook
+          umma::fence_after_sync();
+          values(t, j);
+          if (j + 1 < n) scores(t, j + 1);
         }
+      if (!ok) {                            // whatever was issued has ended before tensor memory is given back
+        if (leader) umma::commit(drain);
+        for (int i = 0; i < 400 && !sleep_on(drain, 0); ++i) {}
       }
     } else {
       // ---- codes to operands ----
       // Unit u of a tile (32 chunks of 16 codes): block u / 16 of 64 coordinates, group (u / 2) % 8 of 16 tokens, eight of
-      // whose tokens are four lanes' each.  This warp has units w, w + 3, ...
+      // whose tokens are four lanes' each.  This warp has units w, w + 7, ...  A thread converts the chunks that it copied.
       const int w = warp - 9, sub = lane >> 2, c = lane & 3;
+      constexpr int kMine = (P::kUnits + kConverters - 1) / kConverters;
       const int32_t* row = a.table + seq * a.table_stride;
-      const uint8_t* k_head = a.p.k_codes + h * a.p.k_stride[1];
-      const uint8_t* v_head = a.p.v_codes + h * a.p.v_stride[1];
       const uint32_t to0 = sub * 128 + (((2 * c) ^ sub) << 4), to1 = sub * 128 + (((2 * c + 1) ^ sub) << 4);
-      // group `lane` (of the first eight) of tile j: its page, the offset inside it, its scales
+      // group `lane` (of the first eight) of tile j: its page and the offset inside it
       auto page_of = [&](int j) -> int {
         const int64_t tok = begin + static_cast<int64_t>(j) * kTok + 16 * (lane & 7);
         if (tok >= stop) return -1;
@@ -190,25 +311,39 @@ __global__ void __launch_bounds__(384, 1) paged8_prefill_kernel(Attn8Args a) {
         const int64_t tok = begin + static_cast<int64_t>(j) * kTok + 16 * (lane & 7);
         return static_cast<int>(a.bs_shift >= 0 ? tok & ((1 << a.bs_shift) - 1) : tok % a.p.block_size);
       };
-      auto issue = [&](const uint8_t* head, const int64_t* stride, unsigned char* dst, int j, int id, int off) {
-#pragma unroll 4
-        for (int u = w; u < P::kUnits; u += 3) {
-          const int g = (u >> 1) & 7, in = 8 * (u & 1) + sub;
-          const int pg = __shfl_sync(QKV_FULL_MASK, id, g), at = __shfl_sync(QKV_FULL_MASK, off, g);
-          const bool there = pg >= 0 && begin + static_cast<int64_t>(j) * kTok + 16 * g + in < s.len;
-          const uint8_t* src = head + (there ? pg : 0) * stride[0] + (there ? (at + in) * stride[2] + (u >> 4) * 64 + 16 * c : 0);
-          cp_async16(dst + u * 512 + lane * 16, src, there ? 16 : 0);      // what is not there is zeros
+      // The group's first byte: its address is computed once, by one lane, and handed round.
+      auto group_at = [&](const uint8_t* codes, const int64_t* stride, int id, int off) -> uint64_t {
+        return id < 0 ? 0 : reinterpret_cast<uint64_t>(codes + id * stride[0] + h * stride[1] + off * stride[2]);
+      };
+      auto issue = [&](uint64_t group, const uint8_t* any, int64_t stride, unsigned char* dst, int j) {
+        const int64_t held = s.len - begin - static_cast<int64_t>(j) * kTok;
+        const int valid = held < kTok ? static_cast<int>(held) : kTok;
+        const uint64_t mine = sub * stride + 16 * c;
+        uint64_t at[kMine];
+#pragma unroll
+        for (int i = 0; i < kMine; ++i) at[i] = __shfl_sync(QKV_FULL_MASK, group, ((w + kConverters * i) >> 1) & 7);
+#pragma unroll
+        for (int i = 0; i < kMine; ++i) {
+          const int u = w + kConverters * i;
+          if (u < P::kUnits) {
+            const bool there = at[i] != 0 && 8 * (u & 15) + sub < valid;
+            const uint64_t src = at[i] + mine + ((u & 1) ? 8 * stride : 0) + (u >> 4) * 64;
+            cp_async16(dst + u * 512 + lane * 16, there ? reinterpret_cast<const uint8_t*>(src) : any, there ? 16 : 0);      // else zeros
+          }
         }
         cp_async_commit();
       };
       auto convert = [&](const unsigned char* src, unsigned char* dst) {
-#pragma unroll 4
-        for (int u = w; u < P::kUnits; u += 3) {
-          const uint4 x = *reinterpret_cast<const uint4*>(src + u * 512 + lane * 16);
-          const uint32_t y[4] = {p8::biased<CODE>(x.x), p8::biased<CODE>(x.y), p8::biased<CODE>(x.z), p8::biased<CODE>(x.w)};
-          unsigned char* to = dst + (u >> 4) * (kTok * 128) + (u & 15) * 1024;
-          *reinterpret_cast<uint4*>(to + to0) = make_uint4(p8::halves_low<CODE>(y[0]), p8::halves_high<CODE>(y[0]), p8::halves_low<CODE>(y[1]), p8::halves_high<CODE>(y[1]));
-          *reinterpret_cast<uint4*>(to + to1) = make_uint4(p8::halves_low<CODE>(y[2]), p8::halves_high<CODE>(y[2]), p8::halves_low<CODE>(y[3]), p8::halves_high<CODE>(y[3]));
+#pragma unroll
+        for (int i = 0; i < kMine; ++i) {
+          const int u = w + kConverters * i;
+          if (u < P::kUnits) {
+            const uint4 x = *reinterpret_cast<const uint4*>(src + u * 512 + lane * 16);
+            const uint32_t y[4] = {p8::biased<CODE>(x.x), p8::biased<CODE>(x.y), p8::biased<CODE>(x.z), p8::biased<CODE>(x.w)};
+            unsigned char* to = dst + (u >> 4) * (kTok * 128) + (u & 15) * 1024;
+            *reinterpret_cast<uint4*>(to + to0) = make_uint4(p8::halves_low<CODE>(y[0]), p8::halves_high<CODE>(y[0]), p8::halves_low<CODE>(y[1]), p8::halves_high<CODE>(y[1]));
+            *reinterpret_cast<uint4*>(to + to1) = make_uint4(p8::halves_low<CODE>(y[2]), p8::halves_high<CODE>(y[2]), p8::halves_low<CODE>(y[3]), p8::halves_high<CODE>(y[3]));
+          }
         }
         umma::fence_smem_to_async();
       };
@@ -217,14 +352,15 @@ __global__ void __launch_bounds__(384, 1) paged8_prefill_kernel(Attn8Args a) {
       unsigned char* raw_v = raw_s + P::kRawBytes;
       int id = n > 0 ? page_of(0) : -1, id1 = n > 1 ? page_of(1) : -1;
       if (n > 0) {
-        issue(k_head, a.p.k_stride, raw_k, 0, id, offset_of(0));
-        issue(v_head, a.p.v_stride, raw_v, 0, id, offset_of(0));
+        issue(group_at(a.p.k_codes, a.p.k_stride, id, offset_of(0)), a.p.k_codes, a.p.k_stride[2], raw_k, 0);
+        issue(group_at(a.p.v_codes, a.p.v_stride, id, offset_of(0)), a.p.v_codes, a.p.v_stride[2], raw_v, 0);
       }
       float ks = scale_of(a.p.k_scales, a.p.ks_stride, id), vs = scale_of(a.p.v_scales, a.p.vs_stride, id);
       for (int j = 0; j < n; ++j) {
         const int st = j % kStages;
         const uint32_t par = ((j / kStages) & 1) ^ 1;
-        const int id2 = j + 2 < n ? page_of(j + 2) : -1;
+        const int id2 = j + 2 < n ? page_of(j + 2) : -1, off1 = offset_of(j + 1);
+        const uint64_t k1 = group_at(a.p.k_codes, a.p.k_stride, id1, off1), v1 = group_at(a.p.v_codes, a.p.v_stride, id1, off1);
         cp_async_wait<1>();                                // this thread's chunks of K
         if (j >= kStages && !wait_all(k_free + st, par)) break;
         if (w == 0) {
@@ -243,15 +379,14 @@ __global__ void __launch_bounds__(384, 1) paged8_prefill_kernel(Attn8Args a) {
         }
         convert(raw_k, k_s + st * P::kOpBytes);
         arrive(k_full + st);
-        const int off1 = offset_of(j + 1);
-        if (j + 1 < n) issue(k_head, a.p.k_stride, raw_k, j + 1, id1, off1); else cp_async_commit();
+        if (j + 1 < n) issue(k1, a.p.k_codes, a.p.k_stride[2], raw_k, j + 1); else cp_async_commit();
         ks = scale_of(a.p.k_scales, a.p.ks_stride, id1);
         vs = scale_of(a.p.v_scales, a.p.vs_stride, id1);
         cp_async_wait<1>();                                // this thread's chunks of V
         if (j >= kStages && !wait_all(v_free + st, par)) break;
         convert(raw_v, v_s + st * P::kOpBytes);
         arrive(v_full + st);
-        if (j + 1 < n) issue(v_head, a.p.v_stride, raw_v, j + 1, id1, off1); else cp_async_commit();
+        if (j + 1 < n) issue(v1, a.p.v_codes, a.p.v_stride[2], raw_v, j + 1); else cp_async_commit();
         id = id1;
         id1 = id2;
       }
@@ -259,38 +394,16 @@ __global__ void __launch_bounds__(384, 1) paged8_prefill_kernel(Attn8Args a) {
     }
   } else {
     // ---- a query row per thread ----
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 200;\n");
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 192;\n");
     const int t = warp >> 2, r = r0 + tid;
     if (t < nt) {
       const bool live = r < r_end;
       const uint32_t my = tmem + kTok * t + (static_cast<uint32_t>(32 * (warp & 3)) << 16);
-      float unit;                                          // score (base 2) per unit of the product
+      float unit;
       {
-        const int64_t at = live ? s.q_row0 + static_cast<int64_t>(r / a.G) * a.q_stride[1] + static_cast<int64_t>(h * a.G + r % a.G) * a.q_stride[2] : 0;
-        float mx = 0.f;
-#pragma unroll
-        for (int c = 0; c < D; c += 32) {
-          float v[32];
-          if (live) load_row8<32>(a.q, a.dtype, at + c, v);
-#pragma unroll
-          for (int i = 0; i < 32; ++i) mx = fmaxf(mx, live ? fabsf(v[i]) : 0.f);
-        }
-        const float up = scale_to8<13>(mx), sg = a.scale < 0.f ? -up : up;      // (a negative scale turns the query round)
-        unit = fabsf(a.scale) * 1.4426950408889634f * inverse8(up);
-        unsigned char* dst = q_s + t * P::kQBytes;
-        const int row = tid & 127;
-#pragma unroll
-        for (int c = 0; c < D; c += 32) {
-          float v[32];
-          if (live) load_row8<32>(a.q, a.dtype, at + c, v);
-#pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            uint32_t x[4];
-#pragma unroll
-            for (int e = 0; e < 4; ++e) x[e] = live ? pack_half2(v[8 * k + 2 * e] * sg, v[8 * k + 2 * e + 1] * sg) : 0u;
-            *reinterpret_cast<uint4*>(dst + umma::sw128_offset(row, c + 8 * k, kRowsT)) = make_uint4(x[0], x[1], x[2], x[3]);
-          }
-        }
+        const int row0 = 32 * (warp & 3), first = r0 + t * kRowsT + row0;
+        unit = a.dtype == QKV_BF16 ? stage_queries<D, true>(a, s, h, first, r_end, q_s + t * P::kQBytes, row0)
+                                   : stage_queries<D, false>(a, s, h, first, r_end, q_s + t * P::kQBytes, row0);
         umma::fence_smem_to_async();
         arrive(p_ready + t);
       }
@@ -299,19 +412,26 @@ __global__ void __launch_bounds__(384, 1) paged8_prefill_kernel(Attn8Args a) {
       float m = kNone, M = 0.5f * kNone, l = 0.f;
       bool ok = true;
       for (int j = 0; j < n; ++j) {
-        if (!(ok = wait_all(s_full + t, j & 1) && wait_all(m_full + j % kMetaSlots, (j / kMetaSlots) & 1))) break;
-        umma::fence_after_sync();
-        uint32_t x[2][64];
-        umma::tmem_ld64_issue(my, x[0]);
-        umma::tmem_ld64_issue(my + 64, x[1]);
+        if (!(ok = wait_all(m_full + j % kMetaSlots, (j / kMetaSlots) & 1))) break;
+        // factors of the scores, and of the weights as long as the references stay: while the scores come about
         const TileMeta& mt = meta[j % kMetaSlots];
-        float f[kGroups], ex[kGroups];
+        float f[kGroups], ex[kGroups], up[kGroups];
 #pragma unroll
         for (int g = 0; g < kGroups; ++g) {
           f[g] = mt.ks[g] * unit;
           ex[g] = mt.ex[g];
         }
+        auto factors = [&] {
+#pragma unroll
+          for (int g = 0; g < kGroups; ++g) up[g] = mt.mant[g] * ex2(fminf(m + ex[g] - M, 120.f));
+        };
+        factors();
         const uint32_t bad = mt.bad;
+        if (!(ok = wait_all(s_full + t, j & 1))) break;
+        umma::fence_after_sync();
+        uint32_t x[2][64];
+        umma::tmem_ld64_issue(my, x[0]);
+        umma::tmem_ld64_issue(my + 64, x[1]);
         const int left = lim - j * kTok;                   // tokens 0 .. left of the tile are visible
         const bool masked = __any_sync(QKV_FULL_MASK, left < kTok - 1) || bad != 0;
         umma::tmem_ld64_wait(x[0]);
@@ -336,10 +456,11 @@ __global__ void __launch_bounds__(384, 1) paged8_prefill_kernel(Attn8Args a) {
         } else {
 #pragma unroll
           for (int g = 0; g < kGroups; ++g) {
-            float top[2] = {-INFINITY, -INFINITY};
+            auto at = [&](int i) { return __uint_as_float(x[(16 * g + i) >> 6][(16 * g + i) & 63]); };
+            float top[4];
 #pragma unroll
-            for (int i = 0; i < 16; ++i) top[i & 1] = fmaxf(top[i & 1], __uint_as_float(x[(16 * g + i) >> 6][(16 * g + i) & 63]));
-            const float v = fmaxf(top[0], top[1]) * f[g];
+            for (int i = 0; i < 4; ++i) top[i] = max3(at(3 * i), at(3 * i + 1), at(3 * i + 2));
+            const float v = max3(max3(top[0], top[1], top[2]), max3(top[3], at(12), at(13)), fmaxf(at(14), at(15))) * f[g];
             tm = fmaxf(tm, v);
             tM = fmaxf(tM, v + ex[g]);
           }
@@ -351,6 +472,7 @@ __global__ void __launch_bounds__(384, 1) paged8_prefill_kernel(Attn8Args a) {
           const float alpha = ex2(M - M1);
           m = m1;
           M = M1;
+          factors();
           if (j > 0) {
 #pragma unroll 1
             for (int c = 0; c < D; c += 32) {
@@ -362,34 +484,52 @@ __global__ void __launch_bounds__(384, 1) paged8_prefill_kernel(Attn8Args a) {
             }
           }
         }
-        float ls[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int hf = 0; hf < 2; ++hf) {
-          uint32_t wt[32];
-#pragma unroll
-          for (int g4 = 0; g4 < 4; ++g4) {
-            const int g = 4 * hf + g4;
-            const float up = mt.mant[g] * ex2(fminf(m + ex[g] - M, 120.f));
-#pragma unroll
-            for (int i = 0; i < 16; i += 2) {
-              const float p0 = ex2(fmaf(__uint_as_float(x[hf][16 * g4 + i]), f[g], -m));
-              const float p1 = ex2(fmaf(__uint_as_float(x[hf][16 * g4 + i + 1]), f[g], -m));
-              ls[i & 2] += p0;
-              ls[(i & 2) + 1] += p1;
-              wt[8 * g4 + i / 2] = pack_half2(p0 * up, p1 * up);
-            }
-          }
+        // Sixteen tokens at a time in three steps (argument, exponential, product and rounding), one step apart, so that the
+        // exponentials, of which a scheduler starts one in eight cycles, have the other steps' instructions between them.
+        uint64_t ls[2] = {0, 0};
+        const uint64_t low = pair(-m, -m);
+        uint32_t wt[32];
+        auto el = [&](int k) -> uint32_t& { return x[k >> 6][k & 63]; };
+        auto argument = [&](int k) {
+          const float fg = f[k >> 4];
+          const float2 e = both(fma2(pair(__uint_as_float(el(k)), __uint_as_float(el(k + 1))), pair(fg, fg), low));
+          el(k) = __float_as_uint(e.x);
+          el(k + 1) = __float_as_uint(e.y);
+        };
+        auto weigh = [&](int k) {
+          const float u = up[k >> 4];
+          const uint64_t p = pair(__uint_as_float(el(k)), __uint_as_float(el(k + 1)));
+          ls[(k >> 1) & 1] = add2(ls[(k >> 1) & 1], p);
+          const float2 w = both(mul2(p, pair(u, u)));
+          wt[(k & 63) >> 1] = pack_half2(w.x, w.y);
+        };
+        auto store = [&](int hf) {
           if (masked) {                                    // a page of NaN weighs nothing where it is not seen
 #pragma unroll
             for (int i = 0; i < 64; i += 2) {
               const int k = 64 * hf + i;
-              const bool z0 = k > left || ((bad >> (k >> 4)) & 1u), z1 = k + 1 > left || ((bad >> (k >> 4)) & 1u);
-              wt[i / 2] &= (z0 ? 0u : 0xffffu) | (z1 ? 0u : 0xffff0000u);
+              const bool gone = (bad >> (k >> 4)) & 1u;
+              wt[i / 2] &= (k > left || gone ? 0u : 0xffffu) | (k + 1 > left || gone ? 0u : 0xffff0000u);
             }
           }
           tmem_st32(my + 32 * hf, wt);
+        };
+#pragma unroll
+        for (int i = 0; i < 16; i += 2) argument(i);
+#pragma unroll
+        for (int g = 0; g <= kGroups; ++g) {
+#pragma unroll
+          for (int i = 0; i < 16; i += 2) {
+            if (g < kGroups) el(16 * g + i) = ex2v(el(16 * g + i));
+            if (g + 1 < kGroups) argument(16 * (g + 1) + i);
+            if (g < kGroups) el(16 * g + i + 1) = ex2v(el(16 * g + i + 1));
+            if (g > 0) weigh(16 * (g - 1) + i);
+          }
+          if (g == 4) store(0);
+          if (g == 8) store(1);
         }
-        l += (ls[0] + ls[1]) + (ls[2] + ls[3]);
+        const float2 l2 = both(add2(ls[0], ls[1]));
+        l += l2.x + l2.y;
         umma::tmem_st_wait();
         umma::fence_before_sync();
         arrive(p_ready + t);
@@ -399,8 +539,11 @@ __global__ void __launch_bounds__(384, 1) paged8_prefill_kernel(Attn8Args a) {
         umma::fence_after_sync();
       }
       if (!ok) l = __int_as_float(0x7fc00000);             // (a wait that ran out: NaN)
-      const int64_t slot = part_row8(a, s, seq, h, r) * a.n_splits + blockIdx.z;
-#pragma unroll 1
+      // Rows leave through the place of the queries (every product that reads them has ended), so that D / 8 lanes write a row.
+      const int64_t slot = part_row8(a, s, seq, h, live ? r : 0) * a.n_splits + blockIdx.z;
+      const float by = l != 0.f ? ex2(M - m) / l : 0.f;    // a row that has seen nothing is zeros
+      unsigned char* rows_s = q_s + t * P::kQBytes + 32 * (warp & 3) * (2 * D);
+#pragma unroll
       for (int c = 0; c < D; c += 32) {
         uint32_t o[32];
         if (ok && n > 0) {
@@ -409,12 +552,34 @@ __global__ void __launch_bounds__(384, 1) paged8_prefill_kernel(Attn8Args a) {
 #pragma unroll
           for (int e = 0; e < 32; ++e) o[e] = ok ? 0u : 0x7fc00000u;
         }
-        if (!live) continue;
+        if (a.n_splits > 1) {
+          if (!live) continue;
 #pragma unroll
-        for (int e = 0; e < 32; e += 4) {
-          const float4 y = make_float4(__uint_as_float(o[e]), __uint_as_float(o[e + 1]), __uint_as_float(o[e + 2]), __uint_as_float(o[e + 3]));
-          if (a.n_splits == 1) store_out8(a, s, h, r, c + e, y, m, M, l);
-          else *reinterpret_cast<float4*>(a.part + slot * D + c + e) = y;
+          for (int e = 0; e < 32; e += 4) *reinterpret_cast<uint4*>(a.part + slot * D + c + e) = make_uint4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+          continue;
+        }
+#pragma unroll
+        for (int e = 0; e < 32; e += 8) {
+          uint32_t y[4];
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            const float v0 = __uint_as_float(o[e + 2 * k]) * by, v1 = __uint_as_float(o[e + 2 * k + 1]) * by;
+            const __nv_bfloat162 z = __floats2bfloat162_rn(v0, v1);
+            y[k] = a.dtype == QKV_BF16 ? *reinterpret_cast<const uint32_t*>(&z) : pack_half2(v0, v1);
+          }
+          *reinterpret_cast<uint4*>(rows_s + lane * (2 * D) + ((((c + e) >> 3) ^ (lane & 7)) << 4)) = make_uint4(y[0], y[1], y[2], y[3]);
+        }
+      }
+      if (a.n_splits == 1) {
+        constexpr int kLanes = D / 8, kRows = 32 / kLanes;
+        const int64_t mine = row_at(a, s.o_row0, a.o_stride, h, live ? r : r0);
+        __syncwarp();
+#pragma unroll 8
+        for (int i = 0; i < kLanes; ++i) {
+          const int k = kRows * i + lane / kLanes, c = lane % kLanes;
+          const int64_t at = __shfl_sync(QKV_FULL_MASK, mine, k);
+          const uint4 y = *reinterpret_cast<const uint4*>(rows_s + k * (2 * D) + ((c ^ (k & 7)) << 4));
+          if (r - lane + k < r_end) *(reinterpret_cast<uint4*>(static_cast<uint16_t*>(a.out) + at) + c) = y;
         }
       }
       if (live && a.n_splits > 1) *reinterpret_cast<float4*>(a.ref + slot * 4) = make_float4(m, M, l, 0.f);
@@ -423,14 +588,14 @@ __global__ void __launch_bounds__(384, 1) paged8_prefill_kernel(Attn8Args a) {
   umma::fence_before_sync();
   __syncthreads();
   umma::fence_after_sync();
-  if (warp == 0) umma::tmem_dealloc(tmem, 512);
+  if (warp == 0) umma::tmem_dealloc(*tmem_slot, 512);
 }
 
 template <int D, int CODE>
 int launch(const Attn8Args& a, dim3 grid, cudaStream_t st) {
   auto kernel = paged8_prefill_kernel<D, CODE>;
   if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(Pf8<D>::kSmem)) != cudaSuccess) return QKV_ELAUNCH;
-  kernel<<<grid, 384, Pf8<D>::kSmem, st>>>(a);
+  kernel<<<grid, kThreads, Pf8<D>::kSmem, st>>>(a);
   return check_launch();
 }
 
