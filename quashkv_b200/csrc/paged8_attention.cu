@@ -29,7 +29,7 @@ namespace qkv {
 namespace {
 
 constexpr int kWarps = 4;
-constexpr int kStages = 4;
+constexpr int kStages = 2;               // steps of 32 tokens in a warp's ring: one in work, one on its way
 constexpr float kNone = -1e30f;          // reference exponent before anything has been seen
 constexpr float kSlack = 4.f;
 constexpr float kLift = 10.f;            // the largest weight is near 2^kLift: fp16 then has 2^-35 of it as its least step
@@ -38,7 +38,7 @@ constexpr float kLift = 10.f;            // the largest weight is near 2^kLift: 
 template <int D> struct Pitch { static constexpr int kKey = D == 128 || D == 96 ? D + 16 : D, kVal = D + 16; };
 
 template <int D, int QT, int NG> struct Split {
-  static constexpr int kSlot = 16 * (Pitch<D>::kKey + Pitch<D>::kVal);
+  static constexpr int kGranule = 16 * (Pitch<D>::kKey + Pitch<D>::kVal), kSlot = 2 * kGranule;
   static constexpr int kRows = 8 * NG;
   static constexpr int kAccPitch = D + 4;
   static constexpr size_t kRing = static_cast<size_t>(kWarps) * kStages * kSlot;
@@ -66,8 +66,11 @@ template <int N> __device__ __forceinline__ void lds(uint32_t (&w)[N], const uns
   }
 }
 
+// CTAs on an SM that the registers allow for.
+template <int D, int NG> constexpr int resident() { return D > 64 ? (NG == 1 ? 3 : 2) : (NG == 1 ? 4 : 3); }
+
 template <int D, int CODE, int QT, int NG>
-__global__ void __launch_bounds__(kWarps * 32) paged8_split_kernel(Attn8Args a) {
+__global__ void __launch_bounds__(kWarps * 32, resident<D, NG>()) paged8_split_kernel(Attn8Args a) {
   using P = Split<D, QT, NG>;
   constexpr int kR = P::kRows, kKeyPitch = Pitch<D>::kKey, kValPitch = Pitch<D>::kVal;
   constexpr int kChunks = D;                               // 16-byte chunks of 16 rows of D bytes
@@ -146,71 +149,99 @@ __global__ void __launch_bounds__(kWarps * 32) paged8_split_kernel(Attn8Args a) 
     for (int e = 0; e < 2; ++e) { m[n][e] = kNone; M[n][e] = 0.5f * kNone; l[n][e] = 0.f; }
   }
 
-  // ---- granules: this warp has warp, warp + 4, ... of the chunk ----
-  const int granules = stop > begin ? static_cast<int>((stop - begin + 15) >> 4) : 0;
-  const int count = granules > warp ? (granules - warp + kWarps - 1) / kWarps : 0;
+  // ---- granules: this warp has the pairs warp, warp + 4, ... of the chunk ----
+  // Two granules a step: their products are independent of one another, and the test of the references, the waits and the
+  // bookkeeping are done once for both.
+  const int pairs = stop > begin ? static_cast<int>((stop - begin + 31) >> 5) : 0;
+  const int count = pairs > warp ? (pairs - warp + kWarps - 1) / kWarps : 0;
   const int stored = static_cast<int>(min(s.len - begin, a.chunk));        // tokens that the cache holds from `begin` on
   const int32_t* row = a.table + seq * a.table_stride;
   unsigned char* ring = smem + warp * kStages * P::kSlot;
-  // page and scales of granule 32 b + lane of the warp, for the batch b in work and the next one
-  auto page_of = [&](int i) -> int {
-    if (i >= count) return -1;
-    const int64_t tok = begin + 16 * (warp + kWarps * i);
+  // page and scales of granule `lane` of the batch of 16 steps in work, and of the next one
+  auto token_of = [&](int x) { return 32 * (warp + kWarps * (x >> 1)) + 16 * (x & 1); };      // x: granule of the warp, relative to begin
+  auto page_of = [&](int x) -> int {
+    const int rel = token_of(x);
+    if ((x >> 1) >= count || rel >= stored) return -1;
+    const int64_t tok = begin + rel;
     const int id = row[a.bs_shift >= 0 ? tok >> a.bs_shift : tok / a.p.block_size];
     return id >= 0 && id < a.p.num_blocks ? id : -1;
   };
   auto scale_k = [&](int id) { return id < 0 ? 0.f : a.p.k_scales[id * a.p.ks_stride[0] + h * a.p.ks_stride[1]]; };
   auto scale_v = [&](int id) { return id < 0 ? 0.f : a.p.v_scales[id * a.p.vs_stride[0] + h * a.p.vs_stride[1]]; };
-  int pg = page_of(lane), pg_next = -1;
+  // first byte of the granule's keys and values: computed by its lane, once
   const uint8_t* k_head = a.p.k_codes + h * a.p.k_stride[1];
   const uint8_t* v_head = a.p.v_codes + h * a.p.v_stride[1];
-  auto issue = [&](int i, int id) {                        // codes of granule i, page id (all lanes)
-    if (i < count && id >= 0) {
-      const int64_t tok = begin + 16 * (warp + kWarps * i);
-      const int off = static_cast<int>(a.bs_shift >= 0 ? tok & ((1 << a.bs_shift) - 1) : tok % a.p.block_size);
-      const uint8_t* ks = k_head + id * a.p.k_stride[0] + off * a.p.k_stride[2];
-      const uint8_t* vs = v_head + id * a.p.v_stride[0] + off * a.p.v_stride[2];
-      unsigned char* dst = ring + (i % kStages) * P::kSlot;
+  auto offset_of = [&](int x) {
+    const int64_t tok = begin + token_of(x);
+    return static_cast<int>(a.bs_shift >= 0 ? tok & ((1 << a.bs_shift) - 1) : tok % a.p.block_size);
+  };
+  auto key_at = [&](int x, int id) { return reinterpret_cast<uint64_t>(id < 0 ? nullptr : k_head + id * a.p.k_stride[0] + offset_of(x) * a.p.k_stride[2]); };
+  auto val_at = [&](int x, int id) { return reinterpret_cast<uint64_t>(id < 0 ? nullptr : v_head + id * a.p.v_stride[0] + offset_of(x) * a.p.v_stride[2]); };
+  int k_src[kCopies], dst_k[kCopies], dst_v[kCopies];      // this lane's chunks of a granule: row, then where they go
 #pragma unroll
-      for (int c = 0; c < kCopies; ++c) {
-        const int x = lane + 32 * c, rw = x / (D / 16), col = 16 * (x % (D / 16));
-        if (kChunks % 32 == 0 || x < kChunks) {
-          cp_async16(dst + rw * kKeyPitch + col, ks + rw * a.p.k_stride[2] + col, 16);
-          cp_async16(dst + 16 * kKeyPitch + rw * kValPitch + col, vs + rw * a.p.v_stride[2] + col, 16);
+  for (int c = 0; c < kCopies; ++c) {
+    const int x = lane + 32 * c, rw = x / (D / 16), col = 16 * (x % (D / 16));
+    k_src[c] = rw << 8 | col;
+    dst_k[c] = rw * kKeyPitch + col;
+    dst_v[c] = 16 * kKeyPitch + rw * kValPitch + col;
+  }
+  auto issue = [&](int i, uint64_t kat, uint64_t vat) {    // codes of step i; addresses of its batch, by lane
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      const int from = (2 * i + u) & 31;
+      const uint64_t kp = __shfl_sync(QKV_FULL_MASK, kat, from), vp = __shfl_sync(QKV_FULL_MASK, vat, from);
+      unsigned char* dst = ring + (i % kStages) * P::kSlot + u * P::kGranule;
+      if (i < count && kp) {
+#pragma unroll
+        for (int c = 0; c < kCopies; ++c) {
+          cp_async16(dst + dst_k[c], reinterpret_cast<const uint8_t*>(kp) + (k_src[c] >> 8) * a.p.k_stride[2] + (k_src[c] & 255), 16);
+          cp_async16(dst + dst_v[c], reinterpret_cast<const uint8_t*>(vp) + (k_src[c] >> 8) * a.p.v_stride[2] + (k_src[c] & 255), 16);
         }
       }
     }
-    cp_async_commit();                                     // one group a granule, empty ones too
+    cp_async_commit();                                     // one group a step, empty ones too
   };
-#pragma unroll
-  for (int i = 0; i < kStages - 1; ++i) issue(i, __shfl_sync(QKV_FULL_MASK, pg, i));
+  int pg = page_of(lane), pg_next = -1;
+  uint64_t kat = key_at(lane, pg), vat = val_at(lane, pg), kat_next = 0, vat_next = 0;
+  issue(0, kat, vat);
   float ksc = scale_k(pg), vsc = scale_v(pg), ksc_next = 0.f, vsc_next = 0.f;
 
   for (int i = 0; i < count; ++i) {
-    const int b = i & 31;
+    const int b = i & 15;
     if (b == 0) {
-      if (i > 0) { pg = pg_next; ksc = ksc_next; vsc = vsc_next; }
-      pg_next = page_of(i + 32 + lane);
+      if (i > 0) { pg = pg_next; ksc = ksc_next; vsc = vsc_next; kat = kat_next; vat = vat_next; }
+      pg_next = page_of(2 * i + 32 + lane);
     }
-    if (b == 16) { ksc_next = scale_k(pg_next); vsc_next = scale_v(pg_next); }
-    const int ahead = b + kStages - 1;
-    issue(i + kStages - 1, __shfl_sync(QKV_FULL_MASK, ahead < 32 ? pg : pg_next, ahead & 31));
-    cp_async_wait<kStages - 1>();
+    if (b == 8) {
+      ksc_next = scale_k(pg_next);
+      vsc_next = scale_v(pg_next);
+      kat_next = key_at(2 * (i - 8) + 32 + lane, pg_next);
+      vat_next = val_at(2 * (i - 8) + 32 + lane, pg_next);
+    }
+    if (b == 15) issue(i + 1, kat_next, vat_next); else issue(i + 1, kat, vat);
+    cp_async_wait<1>();
     __syncwarp();
 
     const unsigned char* slot = ring + (i % kStages) * P::kSlot;
-    const int tok = 16 * (warp + kWarps * i);              // relative to begin
-    const int id = __shfl_sync(QKV_FULL_MASK, pg, b);
-    const float ks = __shfl_sync(QKV_FULL_MASK, ksc, b), vs = __shfl_sync(QKV_FULL_MASK, vsc, b);
-    const int valid = id < 0 ? 0 : min(16, stored - tok);
-    const bool whole = valid == 16 && tok + 15 <= all_see; // every row sees every token
+    const int tok = 32 * (warp + kWarps * i);              // relative to begin
+    float ks[2], vs[2];
+    int valid[2];
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      const int id = __shfl_sync(QKV_FULL_MASK, pg, 2 * b + u);
+      ks[u] = __shfl_sync(QKV_FULL_MASK, ksc, 2 * b + u);
+      vs[u] = __shfl_sync(QKV_FULL_MASK, vsc, 2 * b + u);
+      valid[u] = id < 0 ? 0 : max(0, min(16, stored - tok - 16 * u));
+    }
+    const bool whole = valid[0] + valid[1] == 32 && tok + 31 <= all_see;   // every row sees every token
 
     // ---- scores ----
-    float sc[NG][4];
-    {
+    float sc[2][NG][4];
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
       uint32_t w0[kKW], w1[kKW];
-      lds<kKW>(w0, slot + g * kKeyPitch + t * (D / 4));
-      lds<kKW>(w1, slot + (g + 8) * kKeyPitch + t * (D / 4));
+      lds<kKW>(w0, slot + u * P::kGranule + g * kKeyPitch + t * (D / 4));
+      lds<kKW>(w1, slot + u * P::kGranule + (g + 8) * kKeyPitch + t * (D / 4));
       float part[NG][2][4];
 #pragma unroll
       for (int n = 0; n < NG; ++n)
@@ -229,43 +260,55 @@ __global__ void __launch_bounds__(kWarps * 32) paged8_split_kernel(Attn8Args a) 
 #pragma unroll
       for (int n = 0; n < NG; ++n)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) sc[n][e] = (part[n][0][e] + part[n][1][e]) * (ks * unit[n][e & 1]);
+        for (int e = 0; e < 4; ++e) sc[u][n][e] = (part[n][0][e] + part[n][1][e]) * (ks[u] * unit[n][e & 1]);
     }
     if (!whole) {
 #pragma unroll
-      for (int n = 0; n < NG; ++n)
+      for (int u = 0; u < 2; ++u)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int k = g + 8 * (e >> 1);
-          if (k >= valid || tok + k > lim[n][e & 1]) sc[n][e] = -INFINITY;
-        }
+        for (int n = 0; n < NG; ++n)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int k = g + 8 * (e >> 1);
+            if (k >= valid[u] || tok + 16 * u + k > lim[n][e & 1]) sc[u][n][e] = -INFINITY;
+          }
     }
 
     // ---- weights ----
     // vs = mant * 2^ex; a scale of 0 weighs nothing
-    const uint32_t vbits = __float_as_uint(vs);
-    const int vexp = static_cast<int>((vbits >> 23) & 255u);
-    const float ex = vexp ? static_cast<float>(vexp - 127) : kNone;
-    const float mant = vexp ? (vexp == 255 ? vs : __uint_as_float((vbits & 0x807fffffu) | 0x3f800000u)) : 0.f;
+    float ex[2], mant[2];
+    bool nan_page = false;
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      const uint32_t vbits = __float_as_uint(vs[u]);
+      const int vexp = static_cast<int>((vbits >> 23) & 255u);
+      ex[u] = vexp ? static_cast<float>(vexp - 127) : kNone;
+      mant[u] = vexp ? (vexp == 255 ? vs[u] : __uint_as_float((vbits & 0x807fffffu) | 0x3f800000u)) : 0.f;
+      nan_page |= vexp == 255;
+    }
     bool rise = false;
+    float top[NG][2], topM[NG][2];                         // of this lane's tokens
 #pragma unroll
     for (int n = 0; n < NG; ++n)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        rise |= sc[n][e] > m[n][e & 1] + kSlack;
-        rise |= sc[n][e] + ex > M[n][e & 1] + (kLift + kSlack);
+      for (int e = 0; e < 2; ++e) {
+        const float t0 = fmaxf(sc[0][n][e], sc[0][n][e + 2]), t1 = fmaxf(sc[1][n][e], sc[1][n][e + 2]);
+        top[n][e] = fmaxf(t0, t1);
+        topM[n][e] = fmaxf(t0 + ex[0], t1 + ex[1]);
+        rise |= top[n][e] > m[n][e] + kSlack || topM[n][e] > M[n][e] + (kLift + kSlack);
       }
     if (__any_sync(QKV_FULL_MASK, rise)) {
 #pragma unroll
       for (int n = 0; n < NG; ++n)
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          float top = fmaxf(sc[n][e], sc[n][e + 2]);
-          top = fmaxf(top, __shfl_xor_sync(QKV_FULL_MASK, top, 4));
-          top = fmaxf(top, __shfl_xor_sync(QKV_FULL_MASK, top, 8));
-          top = fmaxf(top, __shfl_xor_sync(QKV_FULL_MASK, top, 16));
-          top = ceilf(top);
-          const float m1 = fmaxf(m[n][e], top), M1 = fmaxf(M[n][e], top + ex - kLift);
+          float x = top[n][e], y = topM[n][e];
+#pragma unroll
+          for (int o = 4; o < 32; o <<= 1) {
+            x = fmaxf(x, __shfl_xor_sync(QKV_FULL_MASK, x, o));
+            y = fmaxf(y, __shfl_xor_sync(QKV_FULL_MASK, y, o));
+          }
+          const float m1 = fmaxf(m[n][e], ceilf(x)), M1 = fmaxf(M[n][e], ceilf(y) - kLift);
           l[n][e] *= ex2(m[n][e] - m1);
           const float f = ex2(M[n][e] - M1);
           m[n][e] = m1;
@@ -277,45 +320,48 @@ __global__ void __launch_bounds__(kWarps * 32) paged8_split_kernel(Attn8Args a) 
           }
         }
     }
-    uint32_t wh[NG][2], wl[NG][2];                         // operand B of the second product: tokens x rows
+    uint32_t wh[2][NG][2], wl[2][NG][2];                   // operand B of the second product: tokens x rows
 #pragma unroll
-    for (int n = 0; n < NG; ++n) {
-      float w[4];
+    for (int u = 0; u < 2; ++u)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        l[n][e & 1] += ex2(sc[n][e] - m[n][e & 1]);
-        w[e] = ex2(sc[n][e] - (M[n][e & 1] - ex)) * mant;
+      for (int n = 0; n < NG; ++n) {
+        float w[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          l[n][e & 1] += ex2(sc[u][n][e] - m[n][e & 1]);
+          w[e] = ex2(sc[u][n][e] - (M[n][e & 1] - ex[u])) * mant[u];
+        }
+        if (!whole && nan_page) {                          // a page of NaN: nothing from tokens that are not seen
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (sc[u][n][e] == -INFINITY) w[e] = 0.f;
+        }
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const __half2 hi = __floats2half2_rn(w[2 * e], w[2 * e + 1]);
+          const float2 f = __half22float2(hi);
+          wh[u][n][e] = movmatrix_trans(*reinterpret_cast<const uint32_t*>(&hi));
+          wl[u][n][e] = movmatrix_trans(pack_half2(w[2 * e] - f.x, w[2 * e + 1] - f.y));
+        }
       }
-      if (!whole && vexp == 255) {                         // a page of NaN: nothing from tokens that are not seen
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-          if (sc[n][e] == -INFINITY) w[e] = 0.f;
-      }
-#pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        const __half2 hi = __floats2half2_rn(w[2 * e], w[2 * e + 1]);
-        const float2 f = __half22float2(hi);
-        wh[n][e] = movmatrix_trans(*reinterpret_cast<const uint32_t*>(&hi));
-        wl[n][e] = movmatrix_trans(pack_half2(w[2 * e] - f.x, w[2 * e + 1] - f.y));
-      }
-    }
 
     // ---- values: row = coordinate, inner dimension = tokens 2t, 2t + 1, 2t + 8, 2t + 9 ----
-    {
-      const unsigned char* vp = slot + 16 * kKeyPitch + 2 * t * kValPitch + g * (D / 8);
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      const unsigned char* vp = slot + u * P::kGranule + 16 * kKeyPitch + 2 * t * kValPitch + g * (D / 8);
       uint32_t v0[kVW], v1[kVW], v8[kVW], v9[kVW];
       lds<kVW>(v0, vp);
       lds<kVW>(v1, vp + kValPitch);
       lds<kVW>(v8, vp + 8 * kValPitch);
       lds<kVW>(v9, vp + 9 * kValPitch);
-      if (valid < 16) {                                    // bytes behind the last token may be anything
+      if (valid[u] < 16) {                                 // bytes behind the last token may be anything
         const uint32_t z = 0;
 #pragma unroll
         for (int k = 0; k < kVW; ++k) {
-          v0[k] = 2 * t < valid ? v0[k] : z;
-          v1[k] = 2 * t + 1 < valid ? v1[k] : z;
-          v8[k] = 2 * t + 8 < valid ? v8[k] : z;
-          v9[k] = 2 * t + 9 < valid ? v9[k] : z;
+          v0[k] = 2 * t < valid[u] ? v0[k] : z;
+          v1[k] = 2 * t + 1 < valid[u] ? v1[k] : z;
+          v8[k] = 2 * t + 8 < valid[u] ? v8[k] : z;
+          v9[k] = 2 * t + 9 < valid[u] ? v9[k] : z;
         }
       }
 #pragma unroll
@@ -330,17 +376,17 @@ __global__ void __launch_bounds__(kWarps * 32) paged8_split_kernel(Attn8Args a) 
             // The tensor core truncates what it adds to an accumulator: over many granules that would show in fp32, so
             // each granule's sum is added in fp32.
             float c[4] = {0.f, 0.f, 0.f, 0.f}, d[4] = {0.f, 0.f, 0.f, 0.f};
-            mma16816(c, x, wl[n][0], wl[n][1]);
-            mma16816(d, y, wl[n][0], wl[n][1]);
-            mma16816(c, x, wh[n][0], wh[n][1]);
-            mma16816(d, y, wh[n][0], wh[n][1]);
+            mma16816(c, x, wl[u][n][0], wl[u][n][1]);
+            mma16816(d, y, wl[u][n][0], wl[u][n][1]);
+            mma16816(c, x, wh[u][n][0], wh[u][n][1]);
+            mma16816(d, y, wh[u][n][0], wh[u][n][1]);
 #pragma unroll
             for (int e = 0; e < 4; ++e) { acc[n][2 * k][e] += c[e]; acc[n][2 * k + 1][e] += d[e]; }
           } else {
-            mma16816(acc[n][2 * k], x, wl[n][0], wl[n][1]);
-            mma16816(acc[n][2 * k + 1], y, wl[n][0], wl[n][1]);
-            mma16816(acc[n][2 * k], x, wh[n][0], wh[n][1]);
-            mma16816(acc[n][2 * k + 1], y, wh[n][0], wh[n][1]);
+            mma16816(acc[n][2 * k], x, wl[u][n][0], wl[u][n][1]);
+            mma16816(acc[n][2 * k + 1], y, wl[u][n][0], wl[u][n][1]);
+            mma16816(acc[n][2 * k], x, wh[u][n][0], wh[u][n][1]);
+            mma16816(acc[n][2 * k + 1], y, wh[u][n][0], wh[u][n][1]);
           }
         }
       }
@@ -437,27 +483,35 @@ __global__ void __launch_bounds__(128) paged8_merge_kernel(Attn8Args a) {
   const int tile_end = min((rr / a.tile_rows + 1) * a.tile_rows, rows);
   const int64_t end = visible8(a, s, (tile_end - 1) / a.G);
   const int parts = end > a.chunk ? static_cast<int>((end + a.chunk - 1) / a.chunk) : 1;
+  // A lane holds the references of one part (two where there are more than 32), so that all of a row is in flight at once.
   const int64_t slot = job * a.n_splits;
+  float4 q[2];
   float mt = kNone, Mt = 0.5f * kNone;
-  for (int p = lane; p < parts; p += 32) {
-    mt = max_or_nan(mt, a.ref[(slot + p) * 4]);
-    Mt = max_or_nan(Mt, a.ref[(slot + p) * 4 + 1]);
+#pragma unroll
+  for (int u = 0; u < 2; ++u) {
+    q[u] = lane + 32 * u < parts ? *reinterpret_cast<const float4*>(a.ref + (slot + lane + 32 * u) * 4) : make_float4(kNone, 0.5f * kNone, 0.f, 0.f);
+    mt = max_or_nan(mt, q[u].x);
+    Mt = max_or_nan(Mt, q[u].y);
   }
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) {
     mt = max_or_nan(mt, __shfl_xor_sync(QKV_FULL_MASK, mt, o));
     Mt = max_or_nan(Mt, __shfl_xor_sync(QKV_FULL_MASK, Mt, o));
   }
-  float lt = 0.f;
+  float lt = fmaf(q[0].z, ex2(q[0].x - mt), q[1].z * ex2(q[1].x - mt));
+  const float f0 = ex2(q[0].y - Mt), f1 = ex2(q[1].y - Mt);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) lt += __shfl_xor_sync(QKV_FULL_MASK, lt, o);
   float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
-  for (int p = 0; p < parts; ++p) {
-    const float4 q = *reinterpret_cast<const float4*>(a.ref + (slot + p) * 4);
-    lt = fmaf(q.z, ex2(q.x - mt), lt);
-    const float f = ex2(q.y - Mt);
-    if (c < D) {
-      const float4 y = *reinterpret_cast<const float4*>(a.part + (slot + p) * D + c);
-      o.x = fmaf(y.x, f, o.x); o.y = fmaf(y.y, f, o.y); o.z = fmaf(y.z, f, o.z); o.w = fmaf(y.w, f, o.w);
+  for (int p0 = 0; p0 < parts; p0 += 8) {
+    float4 y[8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k)
+      y[k] = c < D && p0 + k < parts ? __ldcs(reinterpret_cast<const float4*>(a.part + (slot + p0 + k) * D + c)) : make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      const float f = __shfl_sync(QKV_FULL_MASK, p0 + k < 32 ? f0 : f1, (p0 + k) & 31);
+      o.x = fmaf(y[k].x, f, o.x); o.y = fmaf(y[k].y, f, o.y); o.z = fmaf(y[k].z, f, o.z); o.w = fmaf(y[k].w, f, o.w);
     }
   }
   if (c < D) store_out8(a, s, h, rr, c, o, mt, Mt, lt);
@@ -469,20 +523,21 @@ constexpr int kFewRows = 32;
 
 struct Plan8 { int ng, row_tiles, most_rows, n_splits; int64_t chunk, part_rows; size_t ws; };
 
-Plan8 plan_split(int n_seq, int Hkv, int most_rows, int64_t max_kv_len, int d, int dtype) {
+// `rows_used`: rows that sequences mostly have.
+Plan8 plan_split(int n_seq, int Hkv, int most_rows, int rows_used, int64_t max_kv_len, int d, int dtype) {
   Plan8 p;
   p.most_rows = most_rows;
-  p.ng = dtype != QKV_F32 && p.most_rows > 8 ? 2 : 1;
+  p.ng = dtype != QKV_F32 && rows_used > 8 ? 2 : 1;
   p.row_tiles = (p.most_rows + 8 * p.ng - 1) / (8 * p.ng);
-  const int64_t items = static_cast<int64_t>(n_seq) * Hkv * p.row_tiles, wave = 3 * kNumSMs;
-  int64_t splits = (2 * wave + items - 1) / items;
-  const int64_t most = (max_kv_len + 63) / 64;
-  if (splits > most) splits = most;
-  if (splits > 64) splits = 64;
-  if (splits < 1) splits = 1;
-  p.chunk = (max_kv_len + splits - 1) / splits;
-  p.chunk = (p.chunk + 63) / 64 * 64;
-  if (p.chunk < 64) p.chunk = 64;
+  const int tiles_used = (rows_used + 8 * p.ng - 1) / (8 * p.ng);
+  // Tokens of a split.  What fits one wave of resident CTAs is cut into one (each at least a step of its four warps); more
+  // is cut five times finer than a wave, so that the last CTAs to run, and sequences of different lengths, leave little
+  // of the chip idle.  Measured, 32 x 8 heads x 32768 tokens: 16384 tokens 440 us, 8192 384, 4096 367, 2048 376, 1024 404;
+  // 32 x 8 x up to 1278: 128 tokens 54 us (the whole step), 256 47, 512 and more 44; 8 heads x 1000: 64 tokens 11.6 us, 128 11.2, 512 13.7.
+  const int64_t wave = 3 * kNumSMs, per = (static_cast<int64_t>(n_seq) * Hkv * tiles_used * max_kv_len + wave - 1) / wave;
+  p.chunk = per <= 2048 ? (per < 128 ? 128 : per) : (per / 5 < 1024 ? 1024 : (per / 5 > 4096 ? 4096 : per / 5));
+  if (p.chunk < (max_kv_len + 63) / 64) p.chunk = (max_kv_len + 63) / 64;        // at most 64 splits
+  p.chunk = (p.chunk + 127) / 128 * 128;
   p.n_splits = static_cast<int>((max_kv_len + p.chunk - 1) / p.chunk);
   if (p.n_splits < 1) p.n_splits = 1;
   p.part_rows = static_cast<int64_t>(n_seq) * Hkv * p.most_rows;
@@ -518,7 +573,7 @@ Route8 route8(int n_seq, int Hkv, int G, int q_len, bool ragged, int64_t tokens,
   const int rows = G * q_len;
   r.prefill = rows > kFewRows && dtype != QKV_F32 && (d == 64 || d == 128);
   r.split = !r.prefill || (ragged && G <= kFewRows);
-  if (r.split) r.s = plan_split(n_seq, Hkv, r.prefill ? kFewRows : rows, max_kv_len, d, dtype);
+  if (r.split) r.s = plan_split(n_seq, Hkv, r.prefill ? kFewRows : rows, r.prefill ? G : rows, max_kv_len, d, dtype);
   if (r.prefill) r.p = plan_prefill(Hkv, G, q_len, tokens, max_kv_len, d);
   r.ws = r.s.ws > r.p.ws ? r.s.ws : r.p.ws;                // one after the other in the same place
   return r;
