@@ -421,7 +421,7 @@ int qkv_attention_paged8(const void* q, int q_dtype, const int64_t* q_strides, q
  * sequence has; slots[t] (of max_tokens) is block * block_size + offset of new token t, the sequences' tokens one
  * after the other, -1 behind them and for tokens that found no place (stack empty, row of the table full);
  * query_starts (n_seq + 1) are the exclusive sums of new_lens, none above max_tokens; seq_lens_out and pool_out
- * may be seq_lens and pool; start_lens_out (may be NULL) gets the lengths before.
+ * may be seq_lens and pool; start_lens_out gets the lengths before (NULL if not wanted, unless in place).
  * qkv_shrink_pages keeps the first min(keep_lens[i], seq_lens[i]) tokens and puts the blocks behind them back; after an
  * extend it restores the stack.  In place.
  * n_seq up to QKV_PAGES_MAX_SEQS; negative lengths count as 0. */

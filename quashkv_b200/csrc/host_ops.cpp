@@ -541,6 +541,14 @@ void check_pool(const Tensor& table, const Tensor& lens, const Tensor& other, co
                     "quashkv_b200: int32 lengths for ", lens.size(0), " sequences, int32 free pages, and pool (2) int32");
 }
 
+// A contiguous tensor on a part of another one's storage: a plan's small results come from one allocation.
+Tensor part_of(const Tensor& base, int64_t byte, at::IntArrayRef size, at::ScalarType type) {
+  Tensor t = at::detail::make_tensor<c10::TensorImpl>(c10::Storage(base.storage()), base.key_set(), c10::scalarTypeToTypeMeta(type));
+  t.unsafeGetTensorImpl()->set_storage_offset(byte / static_cast<int64_t>(c10::elementSize(type)));
+  t.unsafeGetTensorImpl()->set_sizes_contiguous(size);
+  return t;
+}
+
 // lens_out / pool_out: the tensors that get the new lengths and counts (those of the call: in place).
 void run_extend(const Tensor& table, const Tensor& lens, const Tensor& new_in, const Tensor& free_pages, const Tensor& pool, int64_t block_size,
                 const Tensor& slots, const Tensor& starts, const Tensor& lens_out, const Tensor* start_out, const Tensor& pool_out, void* stream) {
@@ -560,7 +568,10 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> extend_pages(Tensor table, const Tens
   check_pool(table, lens, new_lens, free_pages, pool);
   TORCH_CHECK_VALUE(max_tokens >= 0, "quashkv_b200: negative max_tokens");
   const int64_t n = lens.size(0);
-  Tensor slots = empty({max_tokens}, at::kLong, dev), starts = empty({n + 1}, at::kInt, dev), after = empty({n}, at::kInt, dev), count = empty({2}, at::kInt, dev);
+  const int64_t words = 2 * max_tokens;                    // of 32 bits; every part starts on eight bytes
+  const Tensor all = empty({8 * max_tokens + 4 * (2 * n + 8)}, at::kByte, dev);
+  Tensor slots = part_of(all, 0, {max_tokens}, at::kLong), starts = part_of(all, 4 * words, {n + 1}, at::kInt);
+  Tensor after = part_of(all, 4 * (words + (n + 2) / 2 * 2), {n}, at::kInt), count = part_of(all, 4 * (words + (n + 2) / 2 * 2 + (n + 1) / 2 * 2), {2}, at::kInt);
   run_extend(table, lens, new_lens, free_pages, pool, block_size, slots, starts, after, nullptr, count, call.stream);
   return {slots, starts, after, count};
 }
@@ -572,7 +583,10 @@ std::tuple<Tensor, Tensor, Tensor> extend_pages_(Tensor table, Tensor lens, cons
   check_pool(table, lens, new_lens, free_pages, pool);
   TORCH_CHECK_VALUE(max_tokens >= 0, "quashkv_b200: negative max_tokens");
   const int64_t n = lens.size(0);
-  Tensor slots = empty({max_tokens}, at::kLong, dev), starts = empty({n + 1}, at::kInt, dev), before = empty({n}, at::kInt, dev);
+  const int64_t words = 2 * max_tokens;
+  const Tensor all = empty({8 * max_tokens + 4 * (2 * n + 4)}, at::kByte, dev);
+  Tensor slots = part_of(all, 0, {max_tokens}, at::kLong), starts = part_of(all, 4 * words, {n + 1}, at::kInt);
+  Tensor before = part_of(all, 4 * (words + (n + 2) / 2 * 2), {n}, at::kInt);
   run_extend(table, lens, new_lens, free_pages, pool, block_size, slots, starts, lens, &before, pool, call.stream);
   return {slots, starts, before};
 }
@@ -631,11 +645,13 @@ extern "C" __attribute__((used, visibility("default"))) const char quashkv_host_
 #define QKV_FOR_EACH_OP(X)                                                                                          \
   X(compress_mse) X(compress_ip) X(compress_ip_into) X(compress_mixed) X(append_kv) X(append_records) X(append_paged) X(decompress) X(decompress_dense) \
   X(decompress_mixed) X(attention) X(attention_paged) X(attention_tiled) X(attention_tiled_out) X(index_scan_topk) \
-  X(append_paged8) X(attention_paged8) X(extend_pages) X(extend_pages_) X(shrink_pages_)
+  X(append_paged8) X(attention_paged8)
+#define QKV_FOR_EACH_TABLE_OP(X) X(extend_pages) X(extend_pages_) X(shrink_pages_)
 
 TORCH_LIBRARY_IMPL(quashkv_b200, CUDA, m) {
 #define QKV_IMPL(name) m.impl(#name, &name);
   QKV_FOR_EACH_OP(QKV_IMPL)
+  QKV_FOR_EACH_TABLE_OP(QKV_IMPL)
 #undef QKV_IMPL
 }
 
@@ -682,6 +698,9 @@ TORCH_LIBRARY_IMPL(quashkv_b200, Autograd, m) {
 #define QKV_NO_DERIVATIVE(name) m.impl(#name, torch::CppFunction::makeFromBoxedFunction<&without_derivative>());
   QKV_FOR_EACH_OP(QKV_NO_DERIVATIVE)
 #undef QKV_NO_DERIVATIVE
+#define QKV_WHOLE_NUMBERS(name) m.impl(#name, torch::CppFunction::makeFallthrough());      // nothing that could have one
+  QKV_FOR_EACH_TABLE_OP(QKV_WHOLE_NUMBERS)
+#undef QKV_WHOLE_NUMBERS
 }
 
 TORCH_LIBRARY_IMPL(quashkv_b200, ADInplaceOrView, m) {

@@ -527,7 +527,7 @@ struct Plan8 { int ng, row_tiles, most_rows, n_splits; int64_t chunk, part_rows;
 Plan8 plan_split(int n_seq, int Hkv, int most_rows, int rows_used, int64_t max_kv_len, int d, int dtype) {
   Plan8 p;
   p.most_rows = most_rows;
-  p.ng = dtype != QKV_F32 && rows_used > 8 ? 2 : 1;
+  p.ng = rows_used > 8 ? 2 : 1;
   p.row_tiles = (p.most_rows + 8 * p.ng - 1) / (8 * p.ng);
   const int tiles_used = (rows_used + 8 * p.ng - 1) / (8 * p.ng);
   // Tokens of a split.  What fits one wave of resident CTAs is cut into one (each at least a step of its four warps); more
@@ -611,7 +611,7 @@ int launch_split(const Attn8Args& a, int64_t items, cudaStream_t st) {
 
 template <int D, int CODE>
 int launch_types(const Attn8Args& a, int ng, int64_t items, cudaStream_t st) {
-  if (a.dtype == QKV_F32) return launch_split<D, CODE, 2, 1>(a, items, st);
+  if (a.dtype == QKV_F32) return ng == 2 ? launch_split<D, CODE, 2, 2>(a, items, st) : launch_split<D, CODE, 2, 1>(a, items, st);
   return ng == 2 ? launch_split<D, CODE, 1, 2>(a, items, st) : launch_split<D, CODE, 1, 1>(a, items, st);
 }
 template <int D>
