@@ -34,137 +34,181 @@ __device__ __forceinline__ int64_t slot_at(const Append8Args& a, int64_t t) {
   return p8::slot_of(a.table + i * a.table_stride, a.max_blocks, a.p.block_size, static_cast<int64_t>(a.start_lens[i]) + t % a.tokens);
 }
 
-// Eight coordinates as fp32.
-template <typename T> __device__ __forceinline__ void load8(const T* p, float (&v)[8]);
-template <> __device__ __forceinline__ void load8<float>(const float* p, float (&v)[8]) {
-  const float4 a = __ldg(reinterpret_cast<const float4*>(p)), b = __ldg(reinterpret_cast<const float4*>(p) + 1);
-  v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
-}
-template <> __device__ __forceinline__ void load8<__nv_bfloat16>(const __nv_bfloat16* p, float (&v)[8]) {
-  const uint4 w = __ldg(reinterpret_cast<const uint4*>(p));
-  const uint32_t x[4] = {w.x, w.y, w.z, w.w};
+// Eight coordinates of a row as they come, and how their magnitudes compare: as the bits of the largest (without signs an
+// infinity is above every number and a NaN above that).
+template <typename T> struct Raw;
+template <> struct Raw<float> {
+  uint4 w[2];
+  __device__ __forceinline__ void load(const float* p) { w[0] = __ldg(reinterpret_cast<const uint4*>(p)); w[1] = __ldg(reinterpret_cast<const uint4*>(p) + 1); }
+  __device__ __forceinline__ void clear() { w[0] = w[1] = make_uint4(0, 0, 0, 0); }
+  __device__ __forceinline__ uint32_t top() const {
+    const uint32_t x[8] = {w[0].x, w[0].y, w[0].z, w[0].w, w[1].x, w[1].y, w[1].z, w[1].w};
+    uint32_t m = 0;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    v[2 * i] = __uint_as_float(x[i] << 16);
-    v[2 * i + 1] = __uint_as_float(x[i] & 0xffff0000u);
+    for (int i = 0; i < 8; ++i) m = max(m, x[i] & 0x7fffffffu);
+    return m;
   }
-}
-template <> __device__ __forceinline__ void load8<__half>(const __half* p, float (&v)[8]) {
-  const uint4 w = __ldg(reinterpret_cast<const uint4*>(p));
-  const uint32_t x[4] = {w.x, w.y, w.z, w.w};
+  __device__ __forceinline__ void values(float (&v)[8]) const {
+    const uint32_t x[8] = {w[0].x, w[0].y, w[0].z, w[0].w, w[1].x, w[1].y, w[1].z, w[1].w};
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&x[i]));
-    v[2 * i] = f.x;
-    v[2 * i + 1] = f.y;
+    for (int i = 0; i < 8; ++i) v[i] = __uint_as_float(x[i]);
   }
-}
+  static __device__ __forceinline__ float magnitude(uint32_t bits) { return __uint_as_float(bits); }
+};
+template <typename T> struct Raw16 {
+  uint4 w;
+  __device__ __forceinline__ void load(const T* p) { w = __ldg(reinterpret_cast<const uint4*>(p)); }
+  __device__ __forceinline__ void clear() { w = make_uint4(0, 0, 0, 0); }
+  __device__ __forceinline__ uint32_t top() const {      // in the upper half of the word
+    const uint32_t x[4] = {w.x, w.y, w.z, w.w};
+    uint32_t m = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) m = max(m, max(x[i] & 0x7fff0000u, (x[i] << 16) & 0x7fff0000u));
+    return m;
+  }
+};
+template <> struct Raw<__nv_bfloat16> : Raw16<__nv_bfloat16> {
+  __device__ __forceinline__ void values(float (&v)[8]) const {
+    const uint32_t x[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      v[2 * i] = __uint_as_float(x[i] << 16);
+      v[2 * i + 1] = __uint_as_float(x[i] & 0xffff0000u);
+    }
+  }
+  static __device__ __forceinline__ float magnitude(uint32_t bits) { return __uint_as_float(bits); }
+};
+template <> struct Raw<__half> : Raw16<__half> {
+  __device__ __forceinline__ void values(float (&v)[8]) const {
+    const uint32_t x[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&x[i]));
+      v[2 * i] = f.x;
+      v[2 * i + 1] = f.y;
+    }
+  }
+  static __device__ __forceinline__ float magnitude(uint32_t bits) { return __half2float(__ushort_as_half(static_cast<unsigned short>(bits >> 16))); }
+};
 
-// One run: tokens t0 .. t0 + n of the call to rows at .. at + n of page `page`, head h, keys (which = 0) or values.
-template <typename T, int CODE, int D>
-__device__ __forceinline__ void store_run(const Append8Args& a, int which, int h, int64_t t0, int n, int64_t page, int at) {
-  constexpr int kLanes = D / 8, kRows = 32 / kLanes, kSteps = (16 + kRows - 1) / kRows;    // lanes a row, rows a step
-  const int lane = threadIdx.x & 31, row = lane / kLanes, col = 8 * (lane % kLanes);
-  const bool on = row < kRows;                                                 // D = 96: eight lanes have no row
-  const T* x = static_cast<const T*>(a.x[which]) + h * a.stride[which][2] + col;
-  const int64_t* ps = which ? a.p.v_stride : a.p.k_stride;
-  const int64_t* ss = which ? a.p.vs_stride : a.p.ks_stride;
-  uint8_t* codes = (which ? a.p.v_codes : a.p.k_codes) + page * ps[0] + h * ps[1] + col;
-  float* scale_p = (which ? a.p.v_scales : a.p.k_scales) + page * ss[0] + h * ss[1];
-  auto source = [&](int k) {
-    const int64_t t = t0 + k;
-    return x + (a.slots ? t * a.stride[which][1] : t / a.tokens * a.stride[which][0] + t % a.tokens * a.stride[which][1]);
-  };
-  const float old = at > 0 ? *scale_p : 0.f;
-  float v[kSteps][8];
-  float top = 0.f;
-  bool odd = false;                                                            // an infinity or a NaN
-  for (int k0 = 0; k0 < n; k0 += 16) {
+// A head's keys (which = 0) or values: lanes of a row, rows of a step, steps of sixteen rows.
+template <typename T, int CODE, int D> struct Head {
+  static constexpr int kLanes = D / 8, kRows = 32 / kLanes, kSteps = (16 + kRows - 1) / kRows;
+  const Append8Args& a;
+  int which, h, row, col;
+  const T* x;
+  __device__ __forceinline__ Head(const Append8Args& args, int w, int head) : a(args), which(w), h(head) {
+    const int lane = threadIdx.x & 31;
+    row = lane / kLanes;                               // D = 96: eight lanes have no row
+    col = 8 * (lane % kLanes);
+    x = static_cast<const T*>(a.x[which]) + h * a.stride[which][2] + col;
+  }
+  __device__ __forceinline__ bool has(int s, int n) const { return row < kRows && s * kRows + row < (n < 16 ? n : 16); }
+  __device__ __forceinline__ void load(Raw<T> (&v)[kSteps], int64_t t0, int n) const {      // rows t0 .. t0 + min(n, 16)
 #pragma unroll
     for (int s = 0; s < kSteps; ++s) {
-      const int k = k0 + s * kRows + row;
-#pragma unroll
-      for (int e = 0; e < 8; ++e) v[s][e] = 0.f;
-      if (on && k < n && s * kRows + row < 16) load8<T>(source(k), v[s]);
+      v[s].clear();
+      if (!has(s, n)) continue;
+      const int64_t t = t0 + s * kRows + row;
+      v[s].load(x + (a.slots ? t * a.stride[which][1] : t / a.tokens * a.stride[which][0] + t % a.tokens * a.stride[which][1]));
     }
+  }
+  // One run: tokens t0 .. t0 + n of the call to rows at .. at + n of page `page`; v holds its first sixteen rows.
+  __device__ __forceinline__ void store(Raw<T> (&v)[kSteps], int64_t t0, int n, int64_t page, int at) const {
+    const int64_t* ps = which ? a.p.v_stride : a.p.k_stride;
+    const int64_t* ss = which ? a.p.vs_stride : a.p.ks_stride;
+    uint8_t* codes = (which ? a.p.v_codes : a.p.k_codes) + page * ps[0] + h * ps[1] + col;
+    float* scale_p = (which ? a.p.v_scales : a.p.k_scales) + page * ss[0] + h * ss[1];
+    const float old = at > 0 ? *scale_p : 0.f;
+    uint32_t top = 0;
+    for (int k0 = 0;;) {
 #pragma unroll
-    for (int s = 0; s < kSteps; ++s)
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const float m = fabsf(v[s][e]);
-        odd |= !(m < INFINITY);
-        top = fmaxf(top, m);
+      for (int s = 0; s < kSteps; ++s) top = max(top, v[s].top());
+      if ((k0 += 16) >= n) break;
+      load(v, t0 + k0, n - k0);
+    }
+    top = __reduce_max_sync(QKV_FULL_MASK, top);
+    float scale = p8::scale_for<CODE>(Raw<T>::magnitude(top));
+    if (at > 0) scale = (old != old || scale != scale) ? __int_as_float(0x7fc00000) : fmaxf(old, scale);
+    const float inv = scale > 0.f ? 1.f / scale : 0.f;                         // 0 for NaN: codes are zeros
+    if (scale > 0.f && old != scale && at > 0) {                               // raised: what the page holds moves along
+      const float ratio = old / scale;
+      for (int k = row; k < at && row < kRows; k += kRows) {
+        uint2* c = reinterpret_cast<uint2*>(codes + k * ps[2]);
+        const uint2 w = *c;
+        const float4 p = p8::decode4<CODE>(w.x), q = p8::decode4<CODE>(w.y);
+        *c = make_uint2(p8::encode4<CODE>(p.x * ratio, p.y * ratio, p.z * ratio, p.w * ratio),
+                        p8::encode4<CODE>(q.x * ratio, q.y * ratio, q.z * ratio, q.w * ratio));
       }
-  }
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(QKV_FULL_MASK, top, o));
-  if (__any_sync(QKV_FULL_MASK, odd)) top = INFINITY;
-  float scale = p8::scale_for<CODE>(top);
-  if (at > 0) scale = (old != old || scale != scale) ? __int_as_float(0x7fc00000) : fmaxf(old, scale);
-  const float inv = scale > 0.f ? 1.f / scale : 0.f;                           // 0 for NaN: codes are zeros
-  if (scale > 0.f && old != scale && at > 0) {                                 // raised: what the page holds moves along
-    const float ratio = old / scale;
-    for (int k = row; k < at && on; k += kRows) {
-      uint2* c = reinterpret_cast<uint2*>(codes + k * ps[2]);
-      const uint2 w = *c;
-      const float4 p = p8::decode4<CODE>(w.x), q = p8::decode4<CODE>(w.y);
-      *c = make_uint2(p8::encode4<CODE>(p.x * ratio, p.y * ratio, p.z * ratio, p.w * ratio),
-                      p8::encode4<CODE>(q.x * ratio, q.y * ratio, q.z * ratio, q.w * ratio));
     }
-  }
-  for (int k0 = 0; k0 < n; k0 += 16) {
+    for (int k0 = 0; k0 < n; k0 += 16) {
+      if (n > 16) load(v, t0 + k0, n - k0);                                    // a short run is still in registers
 #pragma unroll
-    for (int s = 0; s < kSteps; ++s) {
-      const int k = k0 + s * kRows + row;
-      if (!on || k >= n || s * kRows + row >= 16) continue;
-      if (n > 16) load8<T>(source(k), v[s]);                                   // a short run is still in registers
-      uint2 w = make_uint2(0, 0);
-      if (inv > 0.f) {
-        w.x = p8::encode4<CODE>(v[s][0] * inv, v[s][1] * inv, v[s][2] * inv, v[s][3] * inv);
-        w.y = p8::encode4<CODE>(v[s][4] * inv, v[s][5] * inv, v[s][6] * inv, v[s][7] * inv);
+      for (int s = 0; s < kSteps; ++s) {
+        if (!has(s, n - k0)) continue;
+        uint2 w = make_uint2(0, 0);
+        if (inv > 0.f) {
+          float f[8];
+          v[s].values(f);
+          w.x = p8::encode4<CODE>(f[0] * inv, f[1] * inv, f[2] * inv, f[3] * inv);
+          w.y = p8::encode4<CODE>(f[4] * inv, f[5] * inv, f[6] * inv, f[7] * inv);
+        }
+        *reinterpret_cast<uint2*>(codes + (at + k0 + s * kRows + row) * ps[2]) = w;
       }
-      *reinterpret_cast<uint2*>(codes + (at + k) * ps[2]) = w;
     }
+    if ((threadIdx.x & 31) == 0) *scale_p = scale;
   }
-  if (lane == 0) *scale_p = scale;
-}
+};
 
 template <typename T, int CODE, int D>
 __global__ void __launch_bounds__(kWarps * 32) append8_kernel(Append8Args a) {
   const int lane = threadIdx.x & 31, bs = a.p.block_size;
   const int64_t job = static_cast<int64_t>(blockIdx.x) * kWarps + (threadIdx.x >> 5);
   const int64_t win = job / (2 * a.p.Hkv);
-  const int hw = static_cast<int>(job % (2 * a.p.Hkv)), which = hw & 1, h = hw >> 1;
+  const int hw = static_cast<int>(job - win * (2 * a.p.Hkv));
   const int64_t base = win * a.window;
   if (base >= a.total) return;
+  const Head<T, CODE, D> head(a, hw & 1, hw >> 1);
+  // The rows of the window travel while the slots do: nearly always they are one run, or its beginning.
+  Raw<T> v[Head<T, CODE, D>::kSteps];
+  const int64_t room = a.total - base;
+  const int ahead = static_cast<int>(room < a.window ? room : a.window);
+  head.load(v, base, ahead);
   // lane k holds the slot of token base - 1 + k; tokens 1 .. window of them begin runs where nothing continues
   const int64_t t = base - 1 + lane;
-  const bool here = lane >= 1 && lane <= a.window && t < a.total;
   const int64_t last_slot = a.p.num_blocks * bs;
-  const int64_t slot = (here || (lane == 0 && t >= 0)) ? slot_at(a, t) : -1;
+  const int64_t slot = t >= 0 && t < a.total ? slot_at(a, t) : -1;
   const int64_t prev = __shfl_up_sync(QKV_FULL_MASK, slot, 1);
+  const bool here = lane >= 1 && lane <= a.window && t < a.total;
   const bool lost = here && (slot >= last_slot || (slot < 0 && !a.slots));
-  if (which == 0) {
+  if (head.which == 0) {
     const unsigned dropped = __popc(__ballot_sync(QKV_FULL_MASK, lost));
     if (dropped && lane == 0) atomicAdd(&g_tokens_dropped, static_cast<unsigned long long>(dropped));
   }
-  const bool first = here && slot >= 0 && slot < last_slot && !(prev >= 0 && prev + 1 == slot && slot % bs != 0);
-  unsigned todo = __ballot_sync(QKV_FULL_MASK, first);
+  const bool goes_on = lane >= 1 && prev >= 0 && prev + 1 == slot && slot % bs != 0;
+  const unsigned on = __ballot_sync(QKV_FULL_MASK, goes_on);
+  unsigned todo = __ballot_sync(QKV_FULL_MASK, here && slot >= 0 && slot < last_slot && !goes_on);
+  bool first = true;                                       // v still holds the window's rows
   while (todo) {
     const int k = __ffs(todo) - 1;
     todo &= todo - 1;
     const int64_t t0 = base - 1 + k, s0 = __shfl_sync(QKV_FULL_MASK, slot, k);
     const int at = static_cast<int>(s0 % bs);
-    int n = 1;
-    for (;;) {                                                                 // how far it goes, 32 tokens at a time
-      const int64_t u = t0 + n + lane;
-      const bool more = u < a.total && at + n + lane < bs && slot_at(a, u) == s0 + n + lane;
-      const unsigned m = __ballot_sync(QKV_FULL_MASK, more);
-      if (m == QKV_FULL_MASK) { n += 32; continue; }
-      n += __ffs(~m) - 1;
-      break;
+    const unsigned more = k < 31 ? ~(on >> (k + 1)) : ~0u;
+    int n = __ffs(more);                                   // tokens of the run among the lanes: itself and those that go on
+    if (k + n == 32) {                                     // it may go on behind them, 32 tokens at a time
+      for (;;) {
+        const int64_t u = t0 + n + lane;
+        const bool yes = u < a.total && at + n + lane < bs && slot_at(a, u) == s0 + n + lane;
+        const unsigned m = __ballot_sync(QKV_FULL_MASK, yes);
+        if (m == QKV_FULL_MASK) { n += 32; continue; }
+        n += __ffs(~m) - 1;
+        break;
+      }
     }
-    store_run<T, CODE, D>(a, which, h, t0, n, s0 / bs, at);
+    if (!first || k != 1 || (n > ahead && ahead < 16) || n < ahead) head.load(v, t0, n);
+    first = false;
+    head.store(v, t0, n, s0 / bs, at);
   }
 }
 
