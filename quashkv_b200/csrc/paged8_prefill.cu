@@ -11,7 +11,7 @@
 //                into an accumulator that stays in tensor memory over the whole sequence
 //   warps 0-7    a thread per query row: scores of a tile from tensor memory, softmax, weights as fp16 in their place
 // The tensor core works for one row tile while the softmax of the other runs.  Rows hold two whole-number reference
-// exponents as in the split kernel, which rise only when a score passes them by 2^8; only then is the accumulator
+// exponents as in the split kernel, which rise only when a score passes them by 14; only then is the accumulator
 // rescaled (exactly), by the row's own thread.
 //
 // Precision: codes are exact in fp16, 16-bit queries too (scaled by a power of two per row); weights are rounded to
@@ -34,7 +34,7 @@ namespace {
 
 constexpr int kTok = 128, kRowsT = 128, kStages = 2, kMetaSlots = 4, kGroups = kTok / 16;
 constexpr int kThreads = 512, kConverters = 7;             // warps that turn codes into operands
-constexpr float kNone = -1e30f, kSlack = 8.f, kLift = 6.f;      // weights reach 2^15 and the largest is at least 2^5
+constexpr float kNone = -1e30f, kSlack = 14.f, kLift = 0.f;      // weights reach 2^15 and the largest is at least 1/2
 __device__ unsigned int g_prefill8_timeouts = 0;
 
 struct TileMeta { float ks[kGroups], ex[kGroups], mant[kGroups]; uint32_t bad; uint32_t pad[7]; };   // per group of 16 tokens
