@@ -240,8 +240,9 @@ __global__ void __launch_bounds__(kThreads, 1) paged8_prefill_kernel(Attn8Args a
   auto wait_all = [&](uint64_t* bar, uint32_t parity) { return __all_sync(QKV_FULL_MASK, wait(bar, parity)) != 0; };
 
   if (warp >= 8) {
-    // 512 threads start with 128 registers; 256 x 192 + 256 x 64 = 512 x 128
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 64;\n");
+    // 512 threads start with 128 registers; 256 x 192 + 256 x 64 = 256 x 200 + 256 x 56 = 512 x 128
+    if (D == 128) asm volatile("setmaxnreg.dec.sync.aligned.u32 64;\n");
+    else asm volatile("setmaxnreg.dec.sync.aligned.u32 56;\n");
     if (warp == 8) {
       // ---- MMAs: the warp goes through this as one, one of its threads issues ----
       constexpr uint32_t id_s = umma::instr_desc(umma::kFmtF16, 128, kTok), id_o = umma::instr_desc(umma::kFmtF16, 128, D) | kOuterB;
@@ -394,7 +395,8 @@ __global__ void __launch_bounds__(kThreads, 1) paged8_prefill_kernel(Attn8Args a
     }
   } else {
     // ---- a query row per thread ----
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 192;\n");
+    if (D == 128) asm volatile("setmaxnreg.inc.sync.aligned.u32 192;\n");
+    else asm volatile("setmaxnreg.inc.sync.aligned.u32 200;\n");
     const int t = warp >> 2, r = r0 + tid;
     if (t < nt) {
       const bool live = r < r_end;
