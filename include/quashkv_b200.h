@@ -396,8 +396,8 @@ int64_t qkv_dropped_paged8_tokens(void);
  *              contiguous elements; base and strides multiples of 16 bytes; out likewise, of q's dtype
  *   dense      query_starts == NULL: q_len tokens of every sequence
  *   ragged     tokens query_starts[i] .. query_starts[i+1]-1 (of total_q) are sequence i's, q_len the most of
- *              any (tokens beyond it are not attended); strides[0] is not used; rows of no sequence are left as
- *              they were
+ *              any; strides[0] is not used; starts ascend; rows of no sequence, and of a sequence beyond q_len,
+ *              are zeros
  *   seq_lens   tokens held, clamped to max_kv_len and to the table; a block number outside the pool hides
  *              its tokens; bytes behind the last token may be anything; codes within hold no NaN
  *   scale      any number;  scales of the pages: 0 or more, or NaN, which reaches what sees its page

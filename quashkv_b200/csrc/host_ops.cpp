@@ -509,8 +509,9 @@ Tensor attention_paged8(const Tensor& q_in, const Tensor& k_codes, const Tensor&
                       "quashkv_b200: int32 query_starts of ", n + 1, " entries, got ", starts.sizes());
   const Tensor q = rows16(dtype_code(q_in) < 0 ? q_in.to(at::kFloat) : q_in);
   Tensor out = empty(q.sizes(), q.scalar_type(), dev);
-  if (ragged) out.zero_();                                 // rows of no sequence
-  if (q.numel() == 0 || n == 0) return out;
+  if (q.numel() == 0) return out;
+  const int64_t q_len = ragged ? std::min(max_q_len, q.size(0)) : q.size(2);
+  if (n == 0 || q_len == 0) return out.zero_();            // rows of no sequence
   const int64_t dims[2][3] = {{0, 2, 1}, {-1, 0, 1}};      // sequence, token, head
   int64_t qs[3], os[3];
   for (int i = 0; i < 3; ++i) {
@@ -518,7 +519,7 @@ Tensor attention_paged8(const Tensor& q_in, const Tensor& k_codes, const Tensor&
     qs[i] = dim < 0 ? 0 : stride16(q, dim);
     os[i] = dim < 0 ? 0 : stride16(out, dim);
   }
-  const int64_t hq = q.size(1), q_len = ragged ? std::min(max_q_len, q.size(0)) : q.size(2);
+  const int64_t hq = q.size(1);
   TORCH_CHECK_VALUE(hq * std::max<int64_t>(q_len, 1) <= INT32_MAX && n <= INT32_MAX && max_kv_len < INT32_MAX - 64, "quashkv_b200: sizes beyond 32 bits");
   const int64_t need = api.qkv_attention_paged8_workspace_bytes(n, hq, pages.Hkv, q_len, ragged, ragged ? q.size(0) : 0, max_kv_len, pages.d, dtype_code(q));
   const Tensor ws = need > 0 ? empty({need}, at::kByte, dev) : Tensor();

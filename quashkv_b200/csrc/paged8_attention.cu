@@ -85,12 +85,17 @@ __global__ void __launch_bounds__(kWarps * 32, resident<D, NG>()) paged8_split_k
   item /= a.row_tiles;
   const int h = item % a.Hkv, seq = item / a.Hkv;
   const Span8 s = span8(a, seq);
+  // A launch that overlaps the prefill kernel in front of it ends after it: what follows may rely on both.
+  auto leave = [&] {
+    if (a.behind_prefill && blockIdx.x == 0 && blockIdx.y == 0) asm volatile("griddepcontrol.wait;\n" ::: "memory");
+  };
+  if (a.starts && rt == 0 && blockIdx.y == 0) zero_gaps8(a, s, seq, h);
   const int rows = a.G * s.q_len, r0 = rt * kR;
-  if (r0 >= rows || rows > a.most_rows) return;
+  if (r0 >= rows || rows > a.most_rows) return leave();
   const int r_end = min(r0 + kR, rows);
   const int64_t end = visible8(a, s, (r_end - 1) / a.G);
   const int64_t begin = static_cast<int64_t>(blockIdx.y) * a.chunk, stop = min(end, begin + a.chunk);
-  if (begin > 0 && begin >= end) return;
+  if (begin > 0 && begin >= end) return leave();
 
   // ---- queries: operand B of the scores, row r0 + 8 ng + g in column g ----
   uint32_t qf[NG][QT][kKW][2];
@@ -346,48 +351,62 @@ __global__ void __launch_bounds__(kWarps * 32, resident<D, NG>()) paged8_split_k
       }
 
     // ---- values: row = coordinate, inner dimension = tokens 2t, 2t + 1, 2t + 8, 2t + 9 ----
-#pragma unroll
-    for (int u = 0; u < 2; ++u) {
+    auto fetch = [&](int u, uint32_t (&v)[4][kVW]) {
       const unsigned char* vp = slot + u * P::kGranule + 16 * kKeyPitch + 2 * t * kValPitch + g * (D / 8);
-      uint32_t v0[kVW], v1[kVW], v8[kVW], v9[kVW];
-      lds<kVW>(v0, vp);
-      lds<kVW>(v1, vp + kValPitch);
-      lds<kVW>(v8, vp + 8 * kValPitch);
-      lds<kVW>(v9, vp + 9 * kValPitch);
-      if (valid[u] < 16) {                                 // bytes behind the last token may be anything
-        const uint32_t z = 0;
 #pragma unroll
-        for (int k = 0; k < kVW; ++k) {
-          v0[k] = 2 * t < valid[u] ? v0[k] : z;
-          v1[k] = 2 * t + 1 < valid[u] ? v1[k] : z;
-          v8[k] = 2 * t + 8 < valid[u] ? v8[k] : z;
-          v9[k] = 2 * t + 9 < valid[u] ? v9[k] : z;
+      for (int r = 0; r < 4; ++r) {
+        const int row_of = (r & 1) + 8 * (r >> 1);
+        lds<kVW>(v[r], vp + row_of * kValPitch);
+        if (valid[u] < 16 && 2 * t + row_of >= valid[u]) { // bytes behind the last token may be anything
+#pragma unroll
+          for (int k = 0; k < kVW; ++k) v[r][k] = 0;
         }
       }
+    };
+    auto operands = [&](const uint32_t (&v)[4][kVW], int k, uint32_t (&x)[4], uint32_t (&y)[4]) {      // coordinates 4 k, + 1 and + 2, + 3 of the lane's
+      const uint32_t a01 = p8::biased<CODE>(prmt(v[0][k], v[1][k], 0x5140)), a23 = p8::biased<CODE>(prmt(v[0][k], v[1][k], 0x7362));
+      const uint32_t b01 = p8::biased<CODE>(prmt(v[2][k], v[3][k], 0x5140)), b23 = p8::biased<CODE>(prmt(v[2][k], v[3][k], 0x7362));
+      x[0] = p8::halves_low<CODE>(a01); x[1] = p8::halves_high<CODE>(a01); x[2] = p8::halves_low<CODE>(b01); x[3] = p8::halves_high<CODE>(b01);
+      y[0] = p8::halves_low<CODE>(a23); y[1] = p8::halves_high<CODE>(a23); y[2] = p8::halves_low<CODE>(b23); y[3] = p8::halves_high<CODE>(b23);
+    };
+    if constexpr (QT == 1) {
 #pragma unroll
-      for (int k = 0; k < kVW; ++k) {
-        const uint32_t a01 = p8::biased<CODE>(prmt(v0[k], v1[k], 0x5140)), a23 = p8::biased<CODE>(prmt(v0[k], v1[k], 0x7362));
-        const uint32_t b01 = p8::biased<CODE>(prmt(v8[k], v9[k], 0x5140)), b23 = p8::biased<CODE>(prmt(v8[k], v9[k], 0x7362));
-        const uint32_t x[4] = {p8::halves_low<CODE>(a01), p8::halves_high<CODE>(a01), p8::halves_low<CODE>(b01), p8::halves_high<CODE>(b01)};
-        const uint32_t y[4] = {p8::halves_low<CODE>(a23), p8::halves_high<CODE>(a23), p8::halves_low<CODE>(b23), p8::halves_high<CODE>(b23)};
+      for (int u = 0; u < 2; ++u) {
+        uint32_t v[4][kVW];
+        fetch(u, v);
 #pragma unroll
-        for (int n = 0; n < NG; ++n) {
-          if (QT == 2) {
-            // The tensor core truncates what it adds to an accumulator: over many granules that would show in fp32, so
-            // each granule's sum is added in fp32.
-            float c[4] = {0.f, 0.f, 0.f, 0.f}, d[4] = {0.f, 0.f, 0.f, 0.f};
-            mma16816(c, x, wl[u][n][0], wl[u][n][1]);
-            mma16816(d, y, wl[u][n][0], wl[u][n][1]);
-            mma16816(c, x, wh[u][n][0], wh[u][n][1]);
-            mma16816(d, y, wh[u][n][0], wh[u][n][1]);
+        for (int k = 0; k < kVW; ++k) {
+          uint32_t x[4], y[4];
+          operands(v, k, x, y);
 #pragma unroll
-            for (int e = 0; e < 4; ++e) { acc[n][2 * k][e] += c[e]; acc[n][2 * k + 1][e] += d[e]; }
-          } else {
+          for (int n = 0; n < NG; ++n) {
             mma16816(acc[n][2 * k], x, wl[u][n][0], wl[u][n][1]);
             mma16816(acc[n][2 * k + 1], y, wl[u][n][0], wl[u][n][1]);
             mma16816(acc[n][2 * k], x, wh[u][n][0], wh[u][n][1]);
             mma16816(acc[n][2 * k + 1], y, wh[u][n][0], wh[u][n][1]);
           }
+        }
+      }
+    } else {
+      // The tensor core truncates what it adds to an accumulator: over many steps that would show in fp32, so each step's
+      // sum is added in fp32.
+      uint32_t v0[4][kVW], v1[4][kVW];
+      fetch(0, v0);
+      fetch(1, v1);
+#pragma unroll
+      for (int k = 0; k < kVW; ++k) {
+        uint32_t x[2][4], y[2][4];
+        operands(v0, k, x[0], y[0]);
+        operands(v1, k, x[1], y[1]);
+#pragma unroll
+        for (int n = 0; n < NG; ++n) {
+          float c[4] = {0.f, 0.f, 0.f, 0.f}, d[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int u = 0; u < 2; ++u) { mma16816(c, x[u], wl[u][n][0], wl[u][n][1]); mma16816(d, y[u], wl[u][n][0], wl[u][n][1]); }
+#pragma unroll
+          for (int u = 0; u < 2; ++u) { mma16816(c, x[u], wh[u][n][0], wh[u][n][1]); mma16816(d, y[u], wh[u][n][0], wh[u][n][1]); }
+#pragma unroll
+          for (int e = 0; e < 4; ++e) { acc[n][2 * k][e] += c[e]; acc[n][2 * k + 1][e] += d[e]; }
         }
       }
     }
@@ -442,19 +461,24 @@ __global__ void __launch_bounds__(kWarps * 32, resident<D, NG>()) paged8_split_k
       if (c == 0) *reinterpret_cast<float4*>(a.ref + slot * 4) = make_float4(mt, Mt, lt, 0.f);
     }
   }
+  leave();
 }
 
-// Splits of a row: a warp each; lane = four coordinates (D / 4 lanes).
-template <int D>
+// Parts of a row joined: lane = four coordinates (D / 4 lanes).  A warp joins one row, or (by_token, where rows are many and their
+// parts few) kTogether query heads of a token, all of whose loads are in flight at once.
+constexpr int kTogether = 4;
+
+template <int D, int R>
 __global__ void __launch_bounds__(128) paged8_merge_kernel(Attn8Args a) {
   const int lane = threadIdx.x & 31, c = 4 * lane;
   const int64_t job = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 5);
   asm volatile("griddepcontrol.wait;\n" ::: "memory");
-  int seq, h, rr;
+  int seq, h, rr, rows_here = 1;
+  int64_t row0;                                            // among the partial results
   Span8 s;
-  if (a.by_token) {
-    const int hq = a.Hkv * a.G, head = static_cast<int>(job % hq);
-    const int64_t tok = job / hq;
+  if (R > 1) {
+    const int hq = a.Hkv * a.G, groups = (hq + R - 1) / R, head = static_cast<int>(job % groups) * R;
+    const int64_t tok = job / groups;
     if (tok >= (a.starts ? a.total_q : static_cast<int64_t>(a.n_seq) * a.q_len)) return;
     if (a.starts) {                                        // the last sequence that starts at or in front of it
       int lo = 0, hi = a.n_seq;
@@ -470,6 +494,8 @@ __global__ void __launch_bounds__(128) paged8_merge_kernel(Attn8Args a) {
     if (tok < s.tok0 || tok - s.tok0 >= s.q_len) return;
     h = head / a.G;
     rr = static_cast<int>(tok - s.tok0) * a.G + head % a.G;
+    rows_here = min(R, hq - head);
+    row0 = tok * hq + head;
   } else {
     const int64_t head = job / a.most_rows;
     if (head >= static_cast<int64_t>(a.n_seq) * a.Hkv) return;
@@ -477,44 +503,73 @@ __global__ void __launch_bounds__(128) paged8_merge_kernel(Attn8Args a) {
     h = static_cast<int>(head % a.Hkv);
     seq = static_cast<int>(head / a.Hkv);
     s = span8(a, seq);
+    row0 = job;
   }
   const int rows = a.G * s.q_len;
   if (rr >= rows || rows > a.most_rows || rows <= a.few_rows) return;
   const int tile_end = min((rr / a.tile_rows + 1) * a.tile_rows, rows);
-  const int64_t end = visible8(a, s, (tile_end - 1) / a.G);
-  const int parts = end > a.chunk ? static_cast<int>((end + a.chunk - 1) / a.chunk) : 1;
-  // A lane holds the references of one part (two where there are more than 32), so that all of a row is in flight at once.
-  const int64_t slot = job * a.n_splits;
-  float4 q[2];
-  float mt = kNone, Mt = 0.5f * kNone;
+  // (rows of a token are of one tile or of neighbours, whose last tokens differ: the parts are counted for each)
+  float4 q[R][2];
+  float mt[R], Mt[R], lt[R];
+  int parts[R], most = 0;
 #pragma unroll
-  for (int u = 0; u < 2; ++u) {
-    q[u] = lane + 32 * u < parts ? *reinterpret_cast<const float4*>(a.ref + (slot + lane + 32 * u) * 4) : make_float4(kNone, 0.5f * kNone, 0.f, 0.f);
-    mt = max_or_nan(mt, q[u].x);
-    Mt = max_or_nan(Mt, q[u].y);
+  for (int r = 0; r < R; ++r) {
+    // head h * G + rr % G of the token, then the next ones (of the next KV heads, too)
+    const int in = rr % a.G + r, row = rr - rr % a.G + in % a.G;
+    const int te = R > 1 ? min((row / a.tile_rows + 1) * a.tile_rows, rows) : tile_end;
+    const int64_t end = visible8(a, s, (te - 1) / a.G);
+    parts[r] = r < rows_here ? (end > a.chunk ? static_cast<int>((end + a.chunk - 1) / a.chunk) : 1) : 0;
+    most = max(most, parts[r]);
   }
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    mt = max_or_nan(mt, __shfl_xor_sync(QKV_FULL_MASK, mt, o));
-    Mt = max_or_nan(Mt, __shfl_xor_sync(QKV_FULL_MASK, Mt, o));
-  }
-  float lt = fmaf(q[0].z, ex2(q[0].x - mt), q[1].z * ex2(q[1].x - mt));
-  const float f0 = ex2(q[0].y - Mt), f1 = ex2(q[1].y - Mt);
+  for (int r = 0; r < R; ++r)
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) lt += __shfl_xor_sync(QKV_FULL_MASK, lt, o);
-  float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-  for (int p0 = 0; p0 < parts; p0 += 8) {
-    float4 y[8];
+    for (int u = 0; u < 2; ++u)
+      q[r][u] = lane + 32 * u < parts[r] ? *reinterpret_cast<const float4*>(a.ref + ((row0 + r) * a.n_splits + lane + 32 * u) * 4) : make_float4(kNone, 0.5f * kNone, 0.f, 0.f);
+  float4 y[R][8 / (R > 1 ? 2 : 1)];
+  constexpr int kP = R > 1 ? 4 : 8;
+  auto fetch = [&](int p0) {
 #pragma unroll
-    for (int k = 0; k < 8; ++k)
-      y[k] = c < D && p0 + k < parts ? __ldcs(reinterpret_cast<const float4*>(a.part + (slot + p0 + k) * D + c)) : make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int r = 0; r < R; ++r)
 #pragma unroll
-    for (int k = 0; k < 8; ++k) {
-      const float f = __shfl_sync(QKV_FULL_MASK, p0 + k < 32 ? f0 : f1, (p0 + k) & 31);
-      o.x = fmaf(y[k].x, f, o.x); o.y = fmaf(y[k].y, f, o.y); o.z = fmaf(y[k].z, f, o.z); o.w = fmaf(y[k].w, f, o.w);
+      for (int k = 0; k < kP; ++k)
+        y[r][k] = c < D && p0 + k < parts[r] ? __ldcs(reinterpret_cast<const float4*>(a.part + ((row0 + r) * a.n_splits + p0 + k) * D + c)) : make_float4(0.f, 0.f, 0.f, 0.f);
+  };
+  fetch(0);
+  float4 o[R];
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    mt[r] = max_or_nan(q[r][0].x, q[r][1].x);
+    Mt[r] = max_or_nan(q[r][0].y, q[r][1].y);
+#pragma unroll
+    for (int x = 16; x > 0; x >>= 1) {
+      mt[r] = max_or_nan(mt[r], __shfl_xor_sync(QKV_FULL_MASK, mt[r], x));
+      Mt[r] = max_or_nan(Mt[r], __shfl_xor_sync(QKV_FULL_MASK, Mt[r], x));
     }
+    lt[r] = fmaf(q[r][0].z, ex2(q[r][0].x - mt[r]), q[r][1].z * ex2(q[r][1].x - mt[r]));
+    q[r][0].w = ex2(q[r][0].y - Mt[r]);
+    q[r][1].w = ex2(q[r][1].y - Mt[r]);
+#pragma unroll
+    for (int x = 16; x > 0; x >>= 1) lt[r] += __shfl_xor_sync(QKV_FULL_MASK, lt[r], x);
+    o[r] = make_float4(0.f, 0.f, 0.f, 0.f);
   }
-  if (c < D) store_out8(a, s, h, rr, c, o, mt, Mt, lt);
+  for (int p0 = 0;;) {
+#pragma unroll
+    for (int r = 0; r < R; ++r)
+#pragma unroll
+      for (int k = 0; k < kP; ++k) {
+        const float f = __shfl_sync(QKV_FULL_MASK, p0 + k < 32 ? q[r][0].w : q[r][1].w, (p0 + k) & 31);
+        o[r].x = fmaf(y[r][k].x, f, o[r].x); o[r].y = fmaf(y[r][k].y, f, o[r].y); o[r].z = fmaf(y[r][k].z, f, o[r].z); o[r].w = fmaf(y[r][k].w, f, o[r].w);
+      }
+    p0 += kP;
+    if (p0 >= most) break;
+    fetch(p0);
+  }
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    const int in = rr % a.G + r;
+    if (c < D && r < rows_here) store_out8(a, s, h + in / a.G, rr - rr % a.G + in % a.G, c, o[r], mt[r], Mt[r], lt[r]);
+  }
 }
 
 // How a call is carried out.  Sequences of up to `few` rows (query tokens x query heads of a KV head) go to the split kernel,
@@ -575,27 +630,32 @@ Route8 route8(int n_seq, int Hkv, int G, int q_len, bool ragged, int64_t tokens,
   r.split = !r.prefill || (ragged && G <= kFewRows);
   if (r.split) r.s = plan_split(n_seq, Hkv, r.prefill ? kFewRows : rows, r.prefill ? G : rows, max_kv_len, d, dtype);
   if (r.prefill) r.p = plan_prefill(Hkv, G, q_len, tokens, max_kv_len, d);
-  r.ws = r.s.ws > r.p.ws ? r.s.ws : r.p.ws;                // one after the other in the same place
+  r.ws = r.s.ws + r.p.ws;                                  // they overlap: each has a place of its own
   return r;
 }
 
-template <int D>
-int launch_merge(const Attn8Args& a, cudaStream_t st) {
-  if (a.n_splits == 1) return QKV_OK;
-  const int64_t rows = a.by_token ? (a.starts ? a.total_q : static_cast<int64_t>(a.n_seq) * a.q_len) * a.Hkv * a.G
-                                  : static_cast<int64_t>(a.n_seq) * a.Hkv * a.most_rows;
-  if ((rows + 3) / 4 > 0x7fffffffLL) return QKV_EDIM;
+// A launch, with `early` as a programmatic dependent of the one in front of it.
+int launch_behind(void (*kernel)(Attn8Args), dim3 grid, int threads, size_t smem, const Attn8Args& a, bool early, cudaStream_t st) {
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(static_cast<unsigned>((rows + 3) / 4));
-  cfg.blockDim = dim3(128);
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
   cfg.stream = st;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  if (cudaLaunchKernelEx(&cfg, paged8_merge_kernel<D>, a) != cudaSuccess) return QKV_ELAUNCH;
-  return check_launch();
+  cfg.numAttrs = early ? 1 : 0;
+  return cudaLaunchKernelEx(&cfg, kernel, a) == cudaSuccess ? check_launch() : QKV_ELAUNCH;
+}
+
+template <int D>
+int launch_merge(const Attn8Args& a, cudaStream_t st) {
+  if (a.n_splits == 1) return QKV_OK;
+  const int64_t rows = a.by_token ? (a.starts ? a.total_q : static_cast<int64_t>(a.n_seq) * a.q_len) * ((a.Hkv * a.G + kTogether - 1) / kTogether)
+                                  : static_cast<int64_t>(a.n_seq) * a.Hkv * a.most_rows;      // a warp each
+  if ((rows + 3) / 4 > 0x7fffffffLL) return QKV_EDIM;
+  return launch_behind(a.by_token ? paged8_merge_kernel<D, kTogether> : paged8_merge_kernel<D, 1>, dim3(static_cast<unsigned>((rows + 3) / 4)), 128, 0, a, true, st);
 }
 
 template <int D, int CODE, int QT, int NG>
@@ -604,8 +664,8 @@ int launch_split(const Attn8Args& a, int64_t items, cudaStream_t st) {
   auto kernel = paged8_split_kernel<D, CODE, QT, NG>;
   if (P::kSmem > 48 * 1024 && cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(P::kSmem)) != cudaSuccess)
     return QKV_ELAUNCH;
-  kernel<<<dim3(static_cast<unsigned>(items), a.n_splits), kWarps * 32, P::kSmem, st>>>(a);
-  if (const int rc = check_launch()) return rc;
+  // Behind the prefill kernel of the same call, which it shares nothing with, it starts as soon as that one's CTAs have.
+  if (const int rc = launch_behind(kernel, dim3(static_cast<unsigned>(items), a.n_splits), kWarps * 32, P::kSmem, a, a.behind_prefill != 0, st)) return rc;
   return launch_merge<D>(a, st);
 }
 
@@ -677,34 +737,39 @@ extern "C" int qkv_attention_paged8(const void* q, int q_dtype, const int64_t* q
   if (r.ws > workspace_bytes || (r.ws > 0 && !workspace)) return QKV_EWORKSPACE;
   if (reinterpret_cast<uintptr_t>(workspace) & 15u) return QKV_EALIGN;
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
-  auto with = [&](const Plan8& p) {
+  auto with = [&](const Plan8& p, size_t at) {
     Attn8Args b = a;
     b.row_tiles = p.row_tiles;
     b.most_rows = p.most_rows;
     b.n_splits = p.n_splits;
     b.chunk = p.chunk;
-    b.part = static_cast<float*>(workspace);
+    b.part = reinterpret_cast<float*>(static_cast<char*>(workspace) + at);
     b.ref = b.part + static_cast<size_t>(p.part_rows) * p.n_splits * pages.d;
     return b;
   };
+  Attn8Args p = with(r.p, r.s.ws), b = with(r.s, 0);
   if (r.prefill) {
-    Attn8Args b = with(r.p);
-    b.tile_rows = 256;
-    b.by_token = 1;
-    b.few_rows = r.split ? kFewRows : 0;
-    if (static_cast<int64_t>(n_seq) * a.Hkv > 0x7fffffffLL || b.row_tiles > 65535) return QKV_EDIM;
-    if (const int rc = launch_prefill8(b, st)) return rc;
-    if (const int rc = pages.d == 64 ? launch_merge<64>(b, st) : launch_merge<128>(b, st)) return rc;
+    p.tile_rows = 256;
+    p.by_token = 1;
+    p.few_rows = r.split ? kFewRows : 0;
+    p.zeros = !r.split;
+    if (static_cast<int64_t>(n_seq) * a.Hkv > 0x7fffffffLL || p.row_tiles > 65535) return QKV_EDIM;
+    if (const int rc = launch_prefill8(p, st)) return rc;
   }
-  if (!r.split) return QKV_OK;
-  Attn8Args b = with(r.s);
-  b.tile_rows = 8 * r.s.ng;
-  const int64_t items = static_cast<int64_t>(n_seq) * a.Hkv * r.s.row_tiles;
-  if (items > 0x7fffffffLL) return QKV_EDIM;
-  switch (pages.d) {
-    case 32: return launch_codes<32>(b, r.s.ng, items, st);
-    case 64: return launch_codes<64>(b, r.s.ng, items, st);
-    case 96: return launch_codes<96>(b, r.s.ng, items, st);
-    default: return launch_codes<128>(b, r.s.ng, items, st);
+  if (r.split) {
+    b.tile_rows = 8 * r.s.ng;
+    b.behind_prefill = r.prefill;
+    const int64_t items = static_cast<int64_t>(n_seq) * a.Hkv * r.s.row_tiles;
+    if (items > 0x7fffffffLL) return QKV_EDIM;
+    int rc;
+    switch (pages.d) {
+      case 32: rc = launch_codes<32>(b, r.s.ng, items, st); break;
+      case 64: rc = launch_codes<64>(b, r.s.ng, items, st); break;
+      case 96: rc = launch_codes<96>(b, r.s.ng, items, st); break;
+      default: rc = launch_codes<128>(b, r.s.ng, items, st); break;
+    }
+    if (rc) return rc;
   }
+  if (!r.prefill) return QKV_OK;
+  return pages.d == 64 ? launch_merge<64>(p, st) : launch_merge<128>(p, st);
 }

@@ -22,6 +22,8 @@ struct Attn8Args {
   float* part; float* ref;                  // [row][n_splits] sums, and their (m, M, l, -); rows as part_row8 numbers them
   int few_rows;                             // sequences of no more rows (query tokens x heads of a KV head) are not this kernel's,
   int by_token;                             // most_rows: nor are those of more.  by_token: see part_row8
+  int behind_prefill;                       // split kernel: it overlaps the prefill kernel and has to end after it
+  int zeros;                                // prefill kernel: rows of no sequence are its own to clear
   int test_drop_mma;                        // test hook of the prefill kernel
 };
 
@@ -56,6 +58,23 @@ __device__ __forceinline__ int64_t visible8(const Attn8Args& a, const Span8& s, 
   if (!a.causal) return s.len;
   const int64_t v = s.len - s.q_all + tok + 1;
   return v < 0 ? 0 : (v > s.len ? s.len : v);
+}
+
+// Ragged queries: output rows in front of the first sequence, behind the last one, and of a sequence beyond the promised
+// q_len are zeros.  By the CTA that comes first for (sequence, KV head).
+__device__ __forceinline__ void zero_gaps8(const Attn8Args& a, const Span8& s, int seq, int h) {
+  const int item = a.dtype == QKV_F32 ? 4 : 2, chunks = a.p.d * item / 16;
+  auto clear = [&](int64_t lo, int64_t hi) {               // tokens
+    for (int64_t x = threadIdx.x; x < (hi - lo) * a.G * chunks; x += blockDim.x) {
+      const int64_t row = x / chunks;
+      const int c = static_cast<int>(x - row * chunks);
+      char* at = static_cast<char*>(a.out) + ((lo + row / a.G) * a.o_stride[1] + (h * a.G + row % a.G) * a.o_stride[2]) * item;
+      reinterpret_cast<uint4*>(at)[c] = make_uint4(0, 0, 0, 0);
+    }
+  };
+  if (s.q_len < s.q_all) clear(s.tok0 + s.q_len, s.tok0 + s.q_all);
+  if (seq == 0 && s.tok0 > 0) clear(0, s.tok0);
+  if (seq == a.n_seq - 1 && s.tok0 + s.q_all < a.total_q) clear(s.tok0 + s.q_all, a.total_q);
 }
 
 // Row r of KV head h among the partial results: places for most_rows rows of every sequence and head, or, where sequences differ

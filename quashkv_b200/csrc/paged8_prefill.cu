@@ -216,6 +216,8 @@ __global__ void __launch_bounds__(kThreads, 1) paged8_prefill_kernel(Attn8Args a
 
   const int h = blockIdx.x % a.Hkv, seq = blockIdx.x / a.Hkv;
   const Span8 s = span8(a, seq);
+  asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");
+  if (a.starts && a.zeros && blockIdx.y == 0 && blockIdx.z == 0) zero_gaps8(a, s, seq, h);
   const int rows = a.G * s.q_len, r0 = (gridDim.y - 1 - blockIdx.y) * 2 * kRowsT;      // long rows first
   if (r0 >= rows || rows <= a.few_rows) return;
   const int r_end = min(r0 + 2 * kRowsT, rows), nt = r_end - r0 > kRowsT ? 2 : 1;
