@@ -646,13 +646,13 @@ extern "C" __attribute__((used, visibility("default"))) const char quashkv_host_
 #define QKV_FOR_EACH_OP(X)                                                                                          \
   X(compress_mse) X(compress_ip) X(compress_ip_into) X(compress_mixed) X(append_kv) X(append_records) X(append_paged) X(decompress) X(decompress_dense) \
   X(decompress_mixed) X(attention) X(attention_paged) X(attention_tiled) X(attention_tiled_out) X(index_scan_topk) \
-  X(append_paged8) X(attention_paged8)
-#define QKV_FOR_EACH_TABLE_OP(X) X(extend_pages) X(extend_pages_) X(shrink_pages_)
+  X(attention_paged8)
+#define QKV_FOR_EACH_PAGE_WRITER(X) X(append_paged8) X(extend_pages) X(extend_pages_) X(shrink_pages_)
 
 TORCH_LIBRARY_IMPL(quashkv_b200, CUDA, m) {
 #define QKV_IMPL(name) m.impl(#name, &name);
   QKV_FOR_EACH_OP(QKV_IMPL)
-  QKV_FOR_EACH_TABLE_OP(QKV_IMPL)
+  QKV_FOR_EACH_PAGE_WRITER(QKV_IMPL)
 #undef QKV_IMPL
 }
 
@@ -699,9 +699,9 @@ TORCH_LIBRARY_IMPL(quashkv_b200, Autograd, m) {
 #define QKV_NO_DERIVATIVE(name) m.impl(#name, torch::CppFunction::makeFromBoxedFunction<&without_derivative>());
   QKV_FOR_EACH_OP(QKV_NO_DERIVATIVE)
 #undef QKV_NO_DERIVATIVE
-#define QKV_WHOLE_NUMBERS(name) m.impl(#name, torch::CppFunction::makeFallthrough());      // nothing that could have one
-  QKV_FOR_EACH_TABLE_OP(QKV_WHOLE_NUMBERS)
-#undef QKV_WHOLE_NUMBERS
+#define QKV_NO_RESULT(name) m.impl(#name, torch::CppFunction::makeFallthrough());      // no floating-point results
+  QKV_FOR_EACH_PAGE_WRITER(QKV_NO_RESULT)
+#undef QKV_NO_RESULT
 }
 
 TORCH_LIBRARY_IMPL(quashkv_b200, ADInplaceOrView, m) {

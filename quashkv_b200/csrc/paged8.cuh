@@ -5,6 +5,8 @@
 
 #include <cuda_fp8.h>
 
+#include <atomic>
+
 #include "common.cuh"
 
 namespace qkv {
@@ -94,6 +96,21 @@ template <int CODE> __device__ __forceinline__ float4 decode4(uint32_t w) {
 #endif
 
 }  // namespace p8
+
+// Allows a kernel `smem` bytes of dynamic shared memory on the current device: once for each device, since the call costs
+// as much host time as a launch.
+template <auto kernel>
+int allow_smem(size_t smem) {
+  static std::atomic<uint64_t> done{0};
+  int dev = 0;
+  if (smem <= 48 * 1024) return QKV_OK;
+  if (cudaGetDevice(&dev) != cudaSuccess) return QKV_ELAUNCH;
+  const uint64_t bit = dev < 64 ? uint64_t(1) << dev : 0;
+  if (done.load(std::memory_order_relaxed) & bit) return QKV_OK;
+  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)) != cudaSuccess) return QKV_ELAUNCH;
+  done.fetch_or(bit, std::memory_order_relaxed);
+  return QKV_OK;
+}
 
 // What the entry points check of a pool before anything is launched.
 inline int check_pages8(const qkv_pages8_t& p) {

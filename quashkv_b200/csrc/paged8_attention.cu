@@ -20,6 +20,8 @@
 // Bound by the bytes of the pages: (2 D + 8 / block_size) a token and KV head.
 #include <math.h>
 
+#include <cooperative_groups.h>
+
 #include "mma_decode.cuh"
 #include "paged8.cuh"
 #include "paged8_attention.cuh"
@@ -31,6 +33,7 @@ namespace {
 constexpr int kWarps = 4;
 constexpr int kStages = 2;               // steps of 32 tokens in a warp's ring: one in work, one on its way
 constexpr float kNone = -1e30f;          // reference exponent before anything has been seen
+constexpr int kMostCluster = 8;          // CTAs of a cluster (the portable size)
 constexpr float kSlack = 4.f;
 constexpr float kLift = 10.f;            // the largest weight is near 2^kLift: fp16 then has 2^-35 of it as its least step
 
@@ -42,7 +45,8 @@ template <int D, int QT, int NG> struct Split {
   static constexpr int kRows = 8 * NG;
   static constexpr int kAccPitch = D + 4;
   static constexpr size_t kRing = static_cast<size_t>(kWarps) * kStages * kSlot;
-  static constexpr size_t kMerge = static_cast<size_t>(kWarps) * kRows * (kAccPitch + 4) * 4;
+  static constexpr size_t kOwn = static_cast<size_t>(kWarps) * kRows * (kAccPitch + 4) * 4;      // where the CTA's sums stand for its cluster
+  static constexpr size_t kMerge = kOwn + static_cast<size_t>(kRows) * (D + 4) * 4;
   static constexpr size_t kSmem = kRing > kMerge ? kRing : kMerge;
 };
 
@@ -95,7 +99,7 @@ __global__ void __launch_bounds__(kWarps * 32, resident<D, NG>()) paged8_split_k
   const int r_end = min(r0 + kR, rows);
   const int64_t end = visible8(a, s, (r_end - 1) / a.G);
   const int64_t begin = static_cast<int64_t>(blockIdx.y) * a.chunk, stop = min(end, begin + a.chunk);
-  if (begin > 0 && begin >= end) return leave();
+  if (begin > 0 && begin >= end && !a.in_cluster) return leave();      // (in a cluster it goes on with nothing to add)
 
   // ---- queries: operand B of the scores, row r0 + 8 ng + g in column g ----
   uint32_t qf[NG][QT][kKW][2];
@@ -455,11 +459,48 @@ __global__ void __launch_bounds__(kWarps * 32, resident<D, NG>()) paged8_split_k
     const int rr = r0 + r;
     if (a.n_splits == 1) {
       store_out8(a, s, h, rr, c, o, mt, Mt, lt);
+    } else if (a.in_cluster) {
+      float* own = reinterpret_cast<float*>(smem + P::kOwn);
+      *reinterpret_cast<float4*>(own + r * D + c) = o;
+      if (c == 0) *reinterpret_cast<float4*>(own + kR * D + r * 4) = make_float4(mt, Mt, lt, 0.f);
     } else {
       const int64_t slot = part_row8(a, s, seq, h, rr) * a.n_splits + blockIdx.y;
       *reinterpret_cast<float4*>(a.part + slot * D + c) = o;
       if (c == 0) *reinterpret_cast<float4*>(a.ref + slot * 4) = make_float4(mt, Mt, lt, 0.f);
     }
+  }
+  if (a.in_cluster) {                                      // the splits of these rows are one cluster: joined through shared memory
+    namespace cg = cooperative_groups;
+    cg::cluster_group cluster = cg::this_cluster();
+    cluster.sync();
+    const int parts = end > a.chunk ? static_cast<int>((end + a.chunk - 1) / a.chunk) : 1;
+    float* own = reinterpret_cast<float*>(smem + P::kOwn);
+    for (int x = blockIdx.y * (kWarps * 32) + threadIdx.x; x < n_rows * (D / 4); x += a.n_splits * (kWarps * 32)) {
+      const int r = x / (D / 4), c = 4 * (x % (D / 4));
+      float4 q[kMostCluster], y[kMostCluster];
+#pragma unroll
+      for (int p = 0; p < kMostCluster; ++p) {
+        const float* theirs = cluster.map_shared_rank(own, p < parts ? p : 0);
+        q[p] = p < parts ? *reinterpret_cast<const float4*>(theirs + kR * D + r * 4) : make_float4(kNone, 0.5f * kNone, 0.f, 0.f);
+        y[p] = *reinterpret_cast<const float4*>(theirs + r * D + c);
+      }
+      float mt = kNone, Mt = 0.5f * kNone, lt = 0.f;
+#pragma unroll
+      for (int p = 0; p < kMostCluster; ++p) {
+        mt = max_or_nan(mt, q[p].x);
+        Mt = max_or_nan(Mt, q[p].y);
+      }
+      float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+      for (int p = 0; p < kMostCluster; ++p) {
+        if (p >= parts) continue;
+        lt = fmaf(q[p].z, ex2(q[p].x - mt), lt);
+        const float f = ex2(q[p].y - Mt);
+        o.x = fmaf(y[p].x, f, o.x); o.y = fmaf(y[p].y, f, o.y); o.z = fmaf(y[p].z, f, o.z); o.w = fmaf(y[p].w, f, o.w);
+      }
+      store_out8(a, s, h, r0 + r, c, o, mt, Mt, lt);
+    }
+    cluster.sync();                                        // nobody leaves while others read
   }
   leave();
 }
@@ -576,11 +617,11 @@ __global__ void __launch_bounds__(128) paged8_merge_kernel(Attn8Args a) {
 // those of more to the prefill kernel where it exists (head size 64 and 128, 16-bit queries).
 constexpr int kFewRows = 32;
 
-struct Plan8 { int ng, row_tiles, most_rows, n_splits; int64_t chunk, part_rows; size_t ws; };
+struct Plan8 { int ng, row_tiles, most_rows, n_splits; bool cluster; int64_t chunk, part_rows; size_t ws; };
 
 // `rows_used`: rows that sequences mostly have.
 Plan8 plan_split(int n_seq, int Hkv, int most_rows, int rows_used, int64_t max_kv_len, int d, int dtype) {
-  Plan8 p;
+  Plan8 p{};
   p.most_rows = most_rows;
   p.ng = rows_used > 8 ? 2 : 1;
   p.row_tiles = (p.most_rows + 8 * p.ng - 1) / (8 * p.ng);
@@ -591,12 +632,19 @@ Plan8 plan_split(int n_seq, int Hkv, int most_rows, int rows_used, int64_t max_k
   // 32 x 8 x up to 1278: 128 tokens 54 us (the whole step), 256 47, 512 and more 44; 8 heads x 1000: 64 tokens 11.6 us, 128 11.2, 512 13.7.
   const int64_t wave = 3 * kNumSMs, per = (static_cast<int64_t>(n_seq) * Hkv * tiles_used * max_kv_len + wave - 1) / wave;
   p.chunk = per <= 2048 ? (per < 128 ? 128 : per) : (per / 5 < 1024 ? 1024 : (per / 5 > 4096 ? 4096 : per / 5));
-  if (p.chunk < (max_kv_len + 63) / 64) p.chunk = (max_kv_len + 63) / 64;        // at most 64 splits
+  // Few rows over a short cache: the splits of a row tile are one cluster, whose CTAs join their sums through shared memory:
+  // no second launch and no workspace (8 heads x 1000 tokens 12.0 -> 10.3 us, 8 x 4 heads of 64 x 1277 12.1 -> 10.9).  Not where
+  // there are CTAs for more than two an SM: a cluster is held up by its longest split and by those that have nothing
+  // (32 x 8 x up to 1278 in two splits 39 -> 48 us for the whole step).
+  const int64_t items = static_cast<int64_t>(n_seq) * Hkv * p.row_tiles;
+  const int64_t finest = max_kv_len <= 4096 && items * kMostCluster <= 2 * kNumSMs ? kMostCluster : 64;
+  if (p.chunk < (max_kv_len + finest - 1) / finest) p.chunk = (max_kv_len + finest - 1) / finest;
   p.chunk = (p.chunk + 127) / 128 * 128;
   p.n_splits = static_cast<int>((max_kv_len + p.chunk - 1) / p.chunk);
   if (p.n_splits < 1) p.n_splits = 1;
   p.part_rows = static_cast<int64_t>(n_seq) * Hkv * p.most_rows;
-  p.ws = p.n_splits > 1 ? static_cast<size_t>(p.part_rows) * p.n_splits * (d + 4) * sizeof(float) : 0;
+  p.cluster = p.n_splits > 1 && p.n_splits <= kMostCluster && items * p.n_splits <= 2 * kNumSMs;
+  p.ws = p.n_splits > 1 && !p.cluster ? static_cast<size_t>(p.part_rows) * p.n_splits * (d + 4) * sizeof(float) : 0;
   return p;
 }
 
@@ -634,38 +682,45 @@ Route8 route8(int n_seq, int Hkv, int G, int q_len, bool ragged, int64_t tokens,
   return r;
 }
 
-// A launch, with `early` as a programmatic dependent of the one in front of it.
-int launch_behind(void (*kernel)(Attn8Args), dim3 grid, int threads, size_t smem, const Attn8Args& a, bool early, cudaStream_t st) {
+// A launch: as a programmatic dependent of the one in front of it (`early`), in clusters of `cluster` CTAs along y.
+int launch_as(void (*kernel)(Attn8Args), dim3 grid, int threads, size_t smem, const Attn8Args& a, bool early, int cluster, cudaStream_t st) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = grid;
   cfg.blockDim = dim3(threads);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = st;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchAttribute attr[2];
   cfg.attrs = attr;
-  cfg.numAttrs = early ? 1 : 0;
+  if (early) {
+    attr[cfg.numAttrs].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[cfg.numAttrs++].val.programmaticStreamSerializationAllowed = 1;
+  }
+  if (cluster > 1) {
+    attr[cfg.numAttrs].id = cudaLaunchAttributeClusterDimension;
+    attr[cfg.numAttrs].val.clusterDim.x = 1;
+    attr[cfg.numAttrs].val.clusterDim.y = cluster;
+    attr[cfg.numAttrs++].val.clusterDim.z = 1;
+  }
   return cudaLaunchKernelEx(&cfg, kernel, a) == cudaSuccess ? check_launch() : QKV_ELAUNCH;
 }
 
 template <int D>
 int launch_merge(const Attn8Args& a, cudaStream_t st) {
-  if (a.n_splits == 1) return QKV_OK;
+  if (a.n_splits == 1 || a.in_cluster) return QKV_OK;
   const int64_t rows = a.by_token ? (a.starts ? a.total_q : static_cast<int64_t>(a.n_seq) * a.q_len) * ((a.Hkv * a.G + kTogether - 1) / kTogether)
                                   : static_cast<int64_t>(a.n_seq) * a.Hkv * a.most_rows;      // a warp each
   if ((rows + 3) / 4 > 0x7fffffffLL) return QKV_EDIM;
-  return launch_behind(a.by_token ? paged8_merge_kernel<D, kTogether> : paged8_merge_kernel<D, 1>, dim3(static_cast<unsigned>((rows + 3) / 4)), 128, 0, a, true, st);
+  return launch_as(a.by_token ? paged8_merge_kernel<D, kTogether> : paged8_merge_kernel<D, 1>, dim3(static_cast<unsigned>((rows + 3) / 4)), 128, 0, a, true, 1, st);
 }
 
 template <int D, int CODE, int QT, int NG>
 int launch_split(const Attn8Args& a, int64_t items, cudaStream_t st) {
   using P = Split<D, QT, NG>;
-  auto kernel = paged8_split_kernel<D, CODE, QT, NG>;
-  if (P::kSmem > 48 * 1024 && cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(P::kSmem)) != cudaSuccess)
-    return QKV_ELAUNCH;
+  constexpr auto kernel = paged8_split_kernel<D, CODE, QT, NG>;
+  if (const int rc = allow_smem<kernel>(P::kSmem)) return rc;
   // Behind the prefill kernel of the same call, which it shares nothing with, it starts as soon as that one's CTAs have.
-  if (const int rc = launch_behind(kernel, dim3(static_cast<unsigned>(items), a.n_splits), kWarps * 32, P::kSmem, a, a.behind_prefill != 0, st)) return rc;
+  if (const int rc = launch_as(kernel, dim3(static_cast<unsigned>(items), a.n_splits), kWarps * 32, P::kSmem, a, a.behind_prefill != 0, a.in_cluster ? a.n_splits : 1, st))
+    return rc;
   return launch_merge<D>(a, st);
 }
 
@@ -758,6 +813,7 @@ extern "C" int qkv_attention_paged8(const void* q, int q_dtype, const int64_t* q
   }
   if (r.split) {
     b.tile_rows = 8 * r.s.ng;
+    b.in_cluster = r.s.cluster;
     b.behind_prefill = r.prefill;
     const int64_t items = static_cast<int64_t>(n_seq) * a.Hkv * r.s.row_tiles;
     if (items > 0x7fffffffLL) return QKV_EDIM;

@@ -22,6 +22,7 @@ struct Attn8Args {
   float* part; float* ref;                  // [row][n_splits] sums, and their (m, M, l, -); rows as part_row8 numbers them
   int few_rows;                             // sequences of no more rows (query tokens x heads of a KV head) are not this kernel's,
   int by_token;                             // most_rows: nor are those of more.  by_token: see part_row8
+  int in_cluster;                           // split kernel: the splits of a row tile are one cluster
   int behind_prefill;                       // split kernel: it overlaps the prefill kernel and has to end after it
   int zeros;                                // prefill kernel: rows of no sequence are its own to clear
   int test_drop_mma;                        // test hook of the prefill kernel

@@ -597,8 +597,8 @@ __global__ void __launch_bounds__(kThreads, 1) paged8_prefill_kernel(Attn8Args a
 
 template <int D, int CODE>
 int launch(const Attn8Args& a, dim3 grid, cudaStream_t st) {
-  auto kernel = paged8_prefill_kernel<D, CODE>;
-  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(Pf8<D>::kSmem)) != cudaSuccess) return QKV_ELAUNCH;
+  constexpr auto kernel = paged8_prefill_kernel<D, CODE>;
+  if (const int rc = allow_smem<kernel>(Pf8<D>::kSmem)) return rc;
   kernel<<<grid, kThreads, Pf8<D>::kSmem, st>>>(a);
   return check_launch();
 }

@@ -229,11 +229,7 @@ int threads_for(int64_t items) {
   return threads;
 }
 
-template <typename Args>
-int prepare(void (*kernel)(Args), size_t smem) {
-  if (smem <= 48 * 1024) return QKV_OK;
-  return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)) == cudaSuccess ? QKV_OK : QKV_ELAUNCH;
-}
+constexpr size_t kMostSmem = (3 * static_cast<size_t>(kMaxSeqs) + 2) * 4;
 
 int shift_of(int bs) { return (bs & (bs - 1)) == 0 ? __builtin_ctz(bs) : -1; }
 
@@ -268,12 +264,12 @@ extern "C" int qkv_extend_pages(int32_t* block_table, int64_t table_stride, int 
   const int threads = threads_for(max_tokens > n_seq ? max_tokens : n_seq);
   const unsigned grid = static_cast<unsigned>(ctas < 4 * kNumSMs ? ctas : 4 * kNumSMs);
   if (!in_place || grid == 1) {            // (one CTA has read what it overwrites)
-    if (const int rc = prepare(extend_kernel<true, true>, smem)) return rc;
+    if (const int rc = allow_smem<extend_kernel<true, true>>(kMostSmem)) return rc;
     extend_kernel<true, true><<<grid, threads, smem, st>>>(a);
     return check_launch();
   }
-  if (const int rc = prepare(extend_kernel<true, false>, smem)) return rc;
-  if (const int rc = prepare(extend_kernel<false, true>, smem)) return rc;
+  if (const int rc = allow_smem<extend_kernel<true, false>>(kMostSmem)) return rc;
+  if (const int rc = allow_smem<extend_kernel<false, true>>(kMostSmem)) return rc;
   extend_kernel<true, false><<<grid, threads, smem, st>>>(a);
   if (const int rc = check_launch()) return rc;
   a.lens = start_lens_out;
@@ -290,7 +286,7 @@ extern "C" int qkv_shrink_pages(const int32_t* block_table, int64_t table_stride
   const ShrinkArgs a{block_table, table_stride, max_blocks, seq_lens, keep_lens, free_pages, n_free_pages, pool, n_seq, block_size, shift_of(block_size)};
   // How many pages come back is known on the device only: the portable eight CTAs of a cluster where there can be many.
   const size_t smem = (2 * static_cast<size_t>(n_seq) + 1) * 4;
-  if (const int rc = prepare(shrink_kernel, smem)) return rc;
+  if (const int rc = allow_smem<shrink_kernel>(kMostSmem)) return rc;
   const int64_t most = static_cast<int64_t>(n_seq) * max_blocks;
   const int ctas = most > 4096 ? 8 : 1;
   cudaLaunchConfig_t cfg = {};

@@ -68,10 +68,10 @@ def test_bad_arguments_are_refused_without_launching():
     assert attend(q=None) == -1 and attend(lens=None) == -1 and attend(table=None) == -1 and attend(out=None) == -1
     assert attend(dtype=7) == -4 and attend(hq=7) == -2 and attend(hq=0) == -2 and attend(blocks=0) == -2 and attend(stride=3) == -2
     assert attend(kv=-1) == -2 and attend(kv=1 << 31) == -2 and attend(total=-1) == -2 and attend(q_len=-1) == -2
-    assert attend(q=at8) == -5 and attend(os_=odd3) == -5 and attend(ws=at8, kv=4096) == -5
-    assert attend(kv=4096, size=16) == -6 and attend(kv=4096, ws=None) == -6
+    assert attend(q=at8) == -5 and attend(os_=odd3) == -5 and attend(ws=at8, kv=9000) == -5
+    assert attend(kv=9000, size=16) == -6 and attend(kv=9000, ws=None) == -6
     assert attend(n=0) == 0 and attend(q_len=0) == 0                        # nothing to do
-    assert L.qkv_attention_paged8_workspace_bytes(1, 32, 8, 1, 0, 0, 4096, 128, 1) > 0
+    assert L.qkv_attention_paged8_workspace_bytes(1, 32, 8, 1, 0, 0, 9000, 128, 1) > 0
     assert L.qkv_attention_paged8_workspace_bytes(1, 7, 2, 1, 0, 0, 4096, 128, 1) == 0
 
     def extend(table=one, stride=8, blocks=8, n=4, bs=16, tokens=10, slots=one, pool=one, free=4):
