@@ -10,12 +10,13 @@
 // which coordinate stands at which place of the inner dimension is free as long as both operands agree, so each lane reads
 // contiguous bytes of a token's key and needs no transposition.  Values are transposed by pairing the bytes of two tokens.
 //
-// Precision.  Query rows are scaled by a power of two to below 2^14 and held as fp16, which is exact for 16-bit types, and as hi + lo for
-// fp32.  Weights go in as hi + lo (22 bits, or 2^-34 of the largest).  Softmax in base 2 with two whole-number reference
+// Precision.  Query rows are scaled by a power of two to below 2^14 and held as fp16, which is exact for 16-bit types, and
+// as hi + lo for fp32.  Weights go in as hi + lo (22 bits, or 2^-34 of the largest), with bf16 queries as hi alone: 2^-11
+// at most of each, an eighth of what the output's own rounding takes.  Softmax in base 2 with two whole-number reference
 // exponents a row, so that rescaling is exact: m for the scores t, M for t + log2 of the page's value scale.  The weights
-// of the second product, 2^(t - M) vs, are then at most 2^15 and the largest at least 2^9 whatever the scales are: a page of large
-// values that a row hardly weighs takes no bits from the others.  References rise when a score is 4 above them, which is
-// rare after the first granules.
+// of the second product, 2^(t - M) vs, are then at most 2^15 and the largest at least 2^9 whatever the scales are: a page
+// of large values that a row hardly weighs takes no bits from the others.  References rise when a score is 4 above them,
+// which is rare after the first granules.
 //
 // Bound by the bytes of the pages: (2 D + 8 / block_size) a token and KV head.
 #include <math.h>
@@ -33,6 +34,8 @@ namespace {
 constexpr int kWarps = 4;
 constexpr int kStages = 2;               // steps of 32 tokens in a warp's ring: one in work, one on its way
 constexpr float kNone = -1e30f;          // reference exponent before anything has been seen
+// What queries and weights are held as: fp16 once each (bf16), queries once and weights as hi + lo (fp16), both as hi + lo (fp32).
+enum { kBF16 = 0, kF16 = 1, kF32 = 2 };
 constexpr int kMostCluster = 8;          // CTAs of a cluster (the portable size)
 constexpr float kSlack = 4.f;
 constexpr float kLift = 10.f;            // the largest weight is near 2^kLift: fp16 then has 2^-35 of it as its least step
@@ -40,7 +43,7 @@ constexpr float kLift = 10.f;            // the largest weight is near 2^kLift: 
 // Bytes from one token's row to the next in the ring: without bank conflicts for both operands' reads.
 template <int D> struct Pitch { static constexpr int kKey = D == 128 || D == 96 ? D + 16 : D, kVal = D + 16; };
 
-template <int D, int QT, int NG> struct Split {
+template <int D, int NG> struct Split {
   static constexpr int kGranule = 16 * (Pitch<D>::kKey + Pitch<D>::kVal), kSlot = 2 * kGranule;
   static constexpr int kRows = 8 * NG;
   static constexpr int kAccPitch = D + 4;
@@ -73,9 +76,10 @@ template <int N> __device__ __forceinline__ void lds(uint32_t (&w)[N], const uns
 // CTAs on an SM that the registers allow for.
 template <int D, int NG> constexpr int resident() { return D > 64 ? (NG == 1 ? 3 : 2) : (NG == 1 ? 4 : 3); }
 
-template <int D, int CODE, int QT, int NG>
+template <int D, int CODE, int KIND, int NG>
 __global__ void __launch_bounds__(kWarps * 32, resident<D, NG>()) paged8_split_kernel(Attn8Args a) {
-  using P = Split<D, QT, NG>;
+  using P = Split<D, NG>;
+  constexpr int QT = KIND == kF32 ? 2 : 1, WT = KIND == kBF16 ? 1 : 2;      // terms of queries and weights
   constexpr int kR = P::kRows, kKeyPitch = Pitch<D>::kKey, kValPitch = Pitch<D>::kVal;
   constexpr int kChunks = D;                               // 16-byte chunks of 16 rows of D bytes
   constexpr int kCopies = (kChunks + 31) / 32;
@@ -350,7 +354,7 @@ __global__ void __launch_bounds__(kWarps * 32, resident<D, NG>()) paged8_split_k
           const __half2 hi = __floats2half2_rn(w[2 * e], w[2 * e + 1]);
           const float2 f = __half22float2(hi);
           wh[u][n][e] = movmatrix_trans(*reinterpret_cast<const uint32_t*>(&hi));
-          wl[u][n][e] = movmatrix_trans(pack_half2(w[2 * e] - f.x, w[2 * e + 1] - f.y));
+          if (WT == 2) wl[u][n][e] = movmatrix_trans(pack_half2(w[2 * e] - f.x, w[2 * e + 1] - f.y));
         }
       }
 
@@ -384,8 +388,10 @@ __global__ void __launch_bounds__(kWarps * 32, resident<D, NG>()) paged8_split_k
           operands(v, k, x, y);
 #pragma unroll
           for (int n = 0; n < NG; ++n) {
-            mma16816(acc[n][2 * k], x, wl[u][n][0], wl[u][n][1]);
-            mma16816(acc[n][2 * k + 1], y, wl[u][n][0], wl[u][n][1]);
+            if (WT == 2) {
+              mma16816(acc[n][2 * k], x, wl[u][n][0], wl[u][n][1]);
+              mma16816(acc[n][2 * k + 1], y, wl[u][n][0], wl[u][n][1]);
+            }
             mma16816(acc[n][2 * k], x, wh[u][n][0], wh[u][n][1]);
             mma16816(acc[n][2 * k + 1], y, wh[u][n][0], wh[u][n][1]);
           }
@@ -713,10 +719,10 @@ int launch_merge(const Attn8Args& a, cudaStream_t st) {
   return launch_as(a.by_token ? paged8_merge_kernel<D, kTogether> : paged8_merge_kernel<D, 1>, dim3(static_cast<unsigned>((rows + 3) / 4)), 128, 0, a, true, 1, st);
 }
 
-template <int D, int CODE, int QT, int NG>
+template <int D, int CODE, int KIND, int NG>
 int launch_split(const Attn8Args& a, int64_t items, cudaStream_t st) {
-  using P = Split<D, QT, NG>;
-  constexpr auto kernel = paged8_split_kernel<D, CODE, QT, NG>;
+  using P = Split<D, NG>;
+  constexpr auto kernel = paged8_split_kernel<D, CODE, KIND, NG>;
   if (const int rc = allow_smem<kernel>(P::kSmem)) return rc;
   // Behind the prefill kernel of the same call, which it shares nothing with, it starts as soon as that one's CTAs have.
   if (const int rc = launch_as(kernel, dim3(static_cast<unsigned>(items), a.n_splits), kWarps * 32, P::kSmem, a, a.behind_prefill != 0, a.in_cluster ? a.n_splits : 1, st))
@@ -724,10 +730,14 @@ int launch_split(const Attn8Args& a, int64_t items, cudaStream_t st) {
   return launch_merge<D>(a, st);
 }
 
+template <int D, int CODE, int KIND>
+int launch_groups(const Attn8Args& a, int ng, int64_t items, cudaStream_t st) {
+  return ng == 2 ? launch_split<D, CODE, KIND, 2>(a, items, st) : launch_split<D, CODE, KIND, 1>(a, items, st);
+}
 template <int D, int CODE>
 int launch_types(const Attn8Args& a, int ng, int64_t items, cudaStream_t st) {
-  if (a.dtype == QKV_F32) return ng == 2 ? launch_split<D, CODE, 2, 2>(a, items, st) : launch_split<D, CODE, 2, 1>(a, items, st);
-  return ng == 2 ? launch_split<D, CODE, 1, 2>(a, items, st) : launch_split<D, CODE, 1, 1>(a, items, st);
+  return a.dtype == QKV_F32 ? launch_groups<D, CODE, kF32>(a, ng, items, st)
+       : a.dtype == QKV_F16 ? launch_groups<D, CODE, kF16>(a, ng, items, st) : launch_groups<D, CODE, kBF16>(a, ng, items, st);
 }
 template <int D>
 int launch_codes(const Attn8Args& a, int ng, int64_t items, cudaStream_t st) {
