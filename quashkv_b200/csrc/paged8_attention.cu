@@ -658,8 +658,9 @@ Plan8 plan_split(int n_seq, int Hkv, int most_rows, int rows_used, int64_t max_k
 Plan8 plan_prefill(int Hkv, int G, int q_len, int64_t tokens, int64_t max_kv_len, int d) {
   Plan8 p{};
   p.most_rows = G * q_len;
-  p.row_tiles = (p.most_rows + 255) / 256;
-  const int64_t ctas = (tokens * G + 255) / 256 * Hkv;
+  const int rows = prefill8_rows(d);
+  p.row_tiles = (p.most_rows + rows - 1) / rows;
+  const int64_t ctas = (tokens * G + rows - 1) / rows * Hkv;
   int64_t splits = ctas > 0 ? kNumSMs / ctas : 1;
   const int64_t most = max_kv_len / 512;
   if (splits > most) splits = most;
@@ -814,7 +815,7 @@ extern "C" int qkv_attention_paged8(const void* q, int q_dtype, const int64_t* q
   };
   Attn8Args p = with(r.p, r.s.ws), b = with(r.s, 0);
   if (r.prefill) {
-    p.tile_rows = 256;
+    p.tile_rows = prefill8_rows(pages.d);
     p.by_token = 1;
     p.few_rows = r.split ? kFewRows : 0;
     p.zeros = !r.split;

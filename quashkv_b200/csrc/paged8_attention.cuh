@@ -28,6 +28,7 @@ struct Attn8Args {
   int test_drop_mma;                        // test hook of the prefill kernel
 };
 
+int prefill8_rows(int d);                   // query rows of a CTA of the prefill kernel
 int launch_prefill8(const Attn8Args& a, cudaStream_t st);
 unsigned int prefill8_timeouts();
 

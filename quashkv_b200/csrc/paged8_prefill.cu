@@ -1,16 +1,16 @@
 // Attention of many query rows over 8-bit pages on the fifth-generation tensor cores: head_dim 64 and 128, queries of 16 bits.
 // Formulas as in paged8_attention.cu.
 //
-// A CTA holds 256 query rows of one (sequence, KV head), a row being a query token and one of the head's query heads, as
-// two row tiles of 128 (the M of an MMA), and goes over tokens in tiles of 128:
-//   warps 9-15   bring the codes of a tile from their pages (cp.async) and turn them into fp16 operands in the swizzled
-//                order of the tensor core; both K and V as they lie in memory, a row a token: the scores read K with the
-//                inner dimension contiguous, the second product reads V with the outer one contiguous, so nothing is
-//                transposed
-//   warp 8       one thread issues every MMA: scores of a row tile into tensor memory, and weights (tensor memory) times V
-//                into an accumulator that stays in tensor memory over the whole sequence
-//   warps 0-7    a thread per query row: scores of a tile from tensor memory, softmax, weights as fp16 in their place
-// The tensor core works for one row tile while the softmax of the other runs.  Rows hold two whole-number reference
+// A CTA holds query rows of one (sequence, KV head), a row being a query token and one of the head's query heads, as row
+// tiles of 128 (the M of an MMA), and goes over tokens: operands in tiles of 128, scores in tiles of 128 or 64 (below).
+//   softmax warps   a thread per query row: scores of a tile from tensor memory, softmax, weights as fp16 in their place
+//   one MMA warp    one of its threads issues every MMA: scores of a row tile into tensor memory, and weights (tensor
+//                   memory) times V into an accumulator that stays in tensor memory over the whole sequence
+//   converters      bring the codes of a tile from their pages (cp.async) and turn them into fp16 operands in the swizzled
+//                   order of the tensor core; both K and V as they lie in memory, a row a token: the scores read K with the
+//                   inner dimension contiguous, the second product reads V with the outer one contiguous, so nothing is
+//                   transposed
+// The tensor core works for one row tile while the softmax of the others runs.  Rows hold two whole-number reference
 // exponents as in the split kernel, which rise only when a score passes them by 14; only then is the accumulator
 // rescaled (exactly), by the row's own thread.
 //
@@ -18,8 +18,15 @@
 // fp16 once, 2^-12 on average of each, which is less than the rounding of the output (2^-9 or, fp16, as much), and the sum of weights is
 // fp32 of the unrounded ones.
 //
-// Bound by the chain of one tile: scores (512 cycles of the tensor core), 128 exponentials a thread (1024 cycles of a
-// quarter's unit), second product.
+// Bound by the chain of a row tile: its scores, its softmax, its weights times V, none of which can overlap another of
+// the same row tile, since scores and weights share their columns.  At head_dim 128 a round of 128 tokens takes about
+// 4400 cycles: 2900 of softmax (two warps on a quarter of the SM, whose exponentials alone take 2048) and 1400 of tensor core
+// and hand-over.  512 columns of tensor memory are two row tiles of 128 scores and 128 sums.  At head_dim 64 they are
+// four of 64 and 64, which lets another row tile's softmax run meanwhile: 130 -> 100 us at 8 x 1024 tokens, 32 heads.
+// Measured (causal, bf16, e4m3): 2 x 4096 tokens, 32 heads of 128 over 8: 350 us, 785 TFLOP/s; 8 x 1024, 32 heads
+// of 64 over 4: 100 us, 344 TFLOP/s counted over visible pairs.
+// Slower at head_dim 128: score tiles of 64 tokens in two buffers each; two threads a row (490 us); rows read twice from
+// tensor memory in place of held in registers (470); arithmetic on single numbers in place of pairs (386).
 //
 // Every wait is bounded; one that runs out is counted (qkv_tensor_core_timeouts) and makes the CTA's rows NaN.
 #include <math.h>
@@ -33,7 +40,6 @@ namespace qkv {
 namespace {
 
 constexpr int kTok = 128, kRowsT = 128, kStages = 2, kMetaSlots = 4, kGroups = kTok / 16;
-constexpr int kThreads = 512, kConverters = 7;             // warps that turn codes into operands
 constexpr float kNone = -1e30f, kSlack = 14.f, kLift = 0.f;      // weights reach 2^15 and the largest is at least 1/2
 __device__ unsigned int g_prefill8_timeouts = 0;
 
@@ -43,9 +49,17 @@ static_assert(sizeof(TileMeta) % 16 == 0, "read as 16-byte words");
 template <int D> struct Pf8 {
   static constexpr int kQBytes = kRowsT * D * 2, kOpBytes = kTok * D * 2, kRawBytes = kTok * D;
   static constexpr int kUnits = kRawBytes / 512;           // 32 chunks of 16 codes
-  static constexpr size_t kSmem = 2 * kQBytes + 2 * kStages * kOpBytes + 2 * kRawBytes + kMetaSlots * sizeof(TileMeta) + 256;
+  // Row tiles, and tokens of a score tile: what 512 columns of tensor memory hold, scores at kSub t and sums at 256 + D t.
+  // Four row tiles of 64 tokens keep more softmax warps at work than two of 128, where the sums leave room for them.
+  static constexpr int NT = D == 64 ? 4 : 2, kSub = D == 64 ? 64 : 128, kRowsC = NT * kRowsT;
+  static constexpr int kConverters = D == 64 ? 3 : 7;      // warps that turn codes into operands
+  static constexpr int kSoft = 4 * NT, kThreads = 32 * (kSoft + 1 + kConverters);
+  // Registers of a softmax thread and of the others: within what the CTA starts with (640 threads of 96, 512 of 128).
+  static constexpr int kSoftRegs = D == 64 ? 104 : 192, kOtherRegs = 64, kStartRegs = D == 64 ? 96 : 128;
+  static_assert(32 * (kSoft * kSoftRegs + (1 + kConverters) * kOtherRegs) <= kThreads * kStartRegs, "setmaxnreg would wait for ever");
+  static constexpr size_t kSmem = NT * kQBytes + 2 * kStages * kOpBytes + 2 * kRawBytes + kMetaSlots * sizeof(TileMeta) + 256;
   static_assert(kSmem <= 232448, "shared memory of one CTA");
-  static constexpr int kO = 256;                           // tensor memory: scores at 0 and 128, sums at 256 and 256 + 128
+  static constexpr int kO = 256;
 };
 
 __device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t* v) {
@@ -55,6 +69,16 @@ __device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t* v) {
       "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15]),
       "r"(v[16]), "r"(v[17]), "r"(v[18]), "r"(v[19]), "r"(v[20]), "r"(v[21]), "r"(v[22]), "r"(v[23]), "r"(v[24]), "r"(v[25]),
       "r"(v[26]), "r"(v[27]), "r"(v[28]), "r"(v[29]), "r"(v[30]), "r"(v[31])
+      : "memory");
+}
+
+__device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&v)[16]) {      // and its wait
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];\n\t"
+      "tcgen05.wait::ld.sync.aligned;\n"
+      : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]), "=r"(v[9]),
+        "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15])
+      : "r"(taddr)
       : "memory");
 }
 
@@ -192,11 +216,12 @@ __device__ __forceinline__ float stage_queries(const Attn8Args& a, const Span8& 
 }
 
 template <int D, int CODE>
-__global__ void __launch_bounds__(kThreads, 1) paged8_prefill_kernel(Attn8Args a) {
+__global__ void __launch_bounds__(Pf8<D>::kThreads, 1) paged8_prefill_kernel(Attn8Args a) {
   using P = Pf8<D>;
   extern __shared__ __align__(1024) unsigned char smem[];
-  unsigned char* q_s = smem;                                               // [2]
-  unsigned char* k_s = q_s + 2 * P::kQBytes;                               // [kStages]
+  constexpr int NT = P::NT, kSub = P::kSub, kParts = kTok / kSub, kConverters = P::kConverters, kSoft = P::kSoft;
+  unsigned char* q_s = smem;                                               // [NT]
+  unsigned char* k_s = q_s + NT * P::kQBytes;                               // [kStages]
   unsigned char* v_s = k_s + kStages * P::kOpBytes;                        // [kStages]
   unsigned char* raw_s = v_s + kStages * P::kOpBytes;                      // codes of one K and one V tile
   TileMeta* meta = reinterpret_cast<TileMeta*>(raw_s + 2 * P::kRawBytes);  // [kMetaSlots]
@@ -205,12 +230,13 @@ __global__ void __launch_bounds__(kThreads, 1) paged8_prefill_kernel(Attn8Args a
   uint64_t* v_full = bars + 2;              // [2]
   uint64_t* k_free = bars + 4;              // [2] its MMAs have read it
   uint64_t* v_free = bars + 6;              // [2]
-  uint64_t* s_full = bars + 8;              // [2] scores of a row tile; everything issued before has ended, too
-  uint64_t* p_ready = bars + 10;            // [2] queries (phase 0), then weights of tile j (phase j + 1)
-  uint64_t* o_full = bars + 12;             // [2] all sums
-  uint64_t* m_full = bars + 14;             // [4] scales of a tile
-  uint64_t* drain = bars + 18;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 19);
+  uint64_t* m_full = bars + 8;              // [4] scales of a tile
+  uint64_t* p_ready = bars + 12;            // [NT] queries (phase 0), then weights of score tile i (phase i + 1)
+  uint64_t* s_full = p_ready + NT;          // [NT] scores of a row tile; everything issued before has ended, too
+  uint64_t* o_full = s_full + NT;           // [NT] all sums
+  uint64_t* drain = o_full + NT;
+  constexpr int kBars = 13 + 3 * NT;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + kBars);
   volatile int* dead = reinterpret_cast<volatile int*>(tmem_slot + 1);
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
 
@@ -218,16 +244,17 @@ __global__ void __launch_bounds__(kThreads, 1) paged8_prefill_kernel(Attn8Args a
   const Span8 s = span8(a, seq);
   asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");
   if (a.starts && a.zeros && blockIdx.y == 0 && blockIdx.z == 0) zero_gaps8(a, s, seq, h);
-  const int rows = a.G * s.q_len, r0 = (gridDim.y - 1 - blockIdx.y) * 2 * kRowsT;      // long rows first
+  const int rows = a.G * s.q_len, r0 = (gridDim.y - 1 - blockIdx.y) * P::kRowsC;      // long rows first
   if (r0 >= rows || rows <= a.few_rows) return;
-  const int r_end = min(r0 + 2 * kRowsT, rows), nt = r_end - r0 > kRowsT ? 2 : 1;
+  const int r_end = min(r0 + P::kRowsC, rows), nt = (r_end - r0 + kRowsT - 1) / kRowsT;
   const int64_t seen = visible8(a, s, (r_end - 1) / a.G);
   const int64_t begin = static_cast<int64_t>(blockIdx.z) * a.chunk, stop = min(seen, begin + a.chunk);
   if (begin > 0 && begin >= seen) return;
-  const int n = stop > begin ? static_cast<int>((stop - begin + kTok - 1) / kTok) : 0;
+  const int n_sub = stop > begin ? static_cast<int>((stop - begin + kSub - 1) / kSub) : 0;      // score tiles of kSub tokens
+  const int n = (n_sub + kParts - 1) / kParts;                                                // operand tiles of kTok
 
   if (tid == 0) {
-    for (int i = 0; i < 19; ++i) umma::mbar_init(bars + i, i < 4 ? 32 * kConverters : (i == 10 || i == 11 ? kRowsT : 1));
+    for (int i = 0; i < kBars; ++i) umma::mbar_init(bars + i, i < 4 ? 32 * kConverters : (i >= 12 && i < 12 + NT ? kRowsT : 1));
     asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
     *dead = 0;
   }
@@ -235,41 +262,41 @@ __global__ void __launch_bounds__(kThreads, 1) paged8_prefill_kernel(Attn8Args a
   umma::fence_before_sync();
   __syncthreads();
   umma::fence_after_sync();
-  constexpr uint32_t tmem = 0;              // all 512 columns of it are this CTA's
+  // (all 512 columns of tensor memory are this CTA's: addresses start at 0)
   auto wait = [&](uint64_t* bar, uint32_t parity) {                        // bounded; false when it, or another one, ran out
     return sleep_on(bar, parity) || wait_on(bar, parity, dead);
   };
   auto wait_all = [&](uint64_t* bar, uint32_t parity) { return __all_sync(QKV_FULL_MASK, wait(bar, parity)) != 0; };
 
-  if (warp >= 8) {
-    // 512 threads start with 128 registers; 256 x 192 + 256 x 64 = 256 x 200 + 256 x 56 = 512 x 128
-    if (D == 128) asm volatile("setmaxnreg.dec.sync.aligned.u32 64;\n");
-    else asm volatile("setmaxnreg.dec.sync.aligned.u32 56;\n");
-    if (warp == 8) {
+  if (warp >= kSoft) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;\n" ::"n"(P::kOtherRegs));
+    if (warp == kSoft) {
       // ---- MMAs: the warp goes through this as one, one of its threads issues ----
-      constexpr uint32_t id_s = umma::instr_desc(umma::kFmtF16, 128, kTok), id_o = umma::instr_desc(umma::kFmtF16, 128, D) | kOuterB;
+      constexpr uint32_t id_s = umma::instr_desc(umma::kFmtF16, 128, kSub), id_o = umma::instr_desc(umma::kFmtF16, 128, D) | kOuterB;
       const bool leader = elect_one();
       const uint64_t q_desc = umma::smem_desc_sw128(umma::smem_u32(q_s)), k_desc = umma::smem_desc_sw128(umma::smem_u32(k_s));
       const uint64_t v_desc = smem_desc_outer(umma::smem_u32(v_s), kTok * 128);
-      auto scores = [&](int t, int j) {
-        const uint64_t qd = q_desc + t * (P::kQBytes >> 4), kd = k_desc + (j % kStages) * (P::kOpBytes >> 4);
+      auto scores = [&](int t, int i) {     // score tile i: part i % kParts of operand tile i / kParts
+        const int st = (i / kParts) % kStages, part = i % kParts;
+        const uint64_t qd = q_desc + t * (P::kQBytes >> 4), kd = k_desc + ((st * P::kOpBytes + part * (kSub * 128)) >> 4);
         if (leader) {
 #pragma unroll
           for (int k = 0; k < D / 16; ++k)
-            umma::mma_f16(kTok * t, qd + (((k >> 2) * (kRowsT * 128) + (k & 3) * 32) >> 4), kd + (((k >> 2) * (kTok * 128) + (k & 3) * 32) >> 4), id_s, k != 0);
+            umma::mma_f16(kSub * t, qd + (((k >> 2) * (kRowsT * 128) + (k & 3) * 32) >> 4), kd + (((k >> 2) * (kTok * 128) + (k & 3) * 32) >> 4), id_s, k != 0);
           umma::commit(s_full + t);
-          if (t == nt - 1) umma::commit(k_free + j % kStages);
+          if (t == nt - 1 && part == kParts - 1) umma::commit(k_free + st);
         }
         __syncwarp();
       };
-      auto values = [&](int t, int j) {
-        const uint64_t vd = v_desc + (j % kStages) * (P::kOpBytes >> 4);
+      auto values = [&](int t, int i) {
+        const int st = (i / kParts) % kStages, part = i % kParts;
+        const uint64_t vd = v_desc + ((st * P::kOpBytes + part * (kSub * 128)) >> 4);
         if (leader) {
 #pragma unroll
-          for (int k = 0; k < kTok / 16; ++k)
-            umma::mma_f16_ts(P::kO + kTok * t, kTok * t + 8 * k, vd + (k * 2048 >> 4), id_o, j != 0 || k != 0);
-          if (t == nt - 1) umma::commit(v_free + j % kStages);
-          if (j + 1 == n) umma::commit(o_full + t);
+          for (int k = 0; k < kSub / 16; ++k)
+            umma::mma_f16_ts(P::kO + D * t, kSub * t + 8 * k, vd + (k * 2048 >> 4), id_o, i != 0 || k != 0);
+          if (t == nt - 1 && part == kParts - 1) umma::commit(v_free + st);
+          if (i + 1 == n_sub) umma::commit(o_full + t);
         }
         __syncwarp();
       };
@@ -279,18 +306,19 @@ __global__ void __launch_bounds__(kThreads, 1) paged8_prefill_kernel(Attn8Args a
         umma::fence_after_sync();
         for (int t = 0; t < nt; ++t) scores(t, 0);
       }
-      for (int j = 0; j < n && ok; ++j)
+      for (int i = 0; i < n_sub && ok; ++i) {
+        // the operands are there long before the weights
+        const int j = i / kParts, j1 = (i + 1) / kParts;
+        if (i % kParts == 0) ok = wait_all(v_full + j % kStages, (j / kStages) & 1);
+        if (ok && j1 != j && i + 1 < n_sub) ok = wait_all(k_full + j1 % kStages, (j1 / kStages) & 1);
         for (int t = 0; t < nt && ok; ++t) {
-          if (t == 0) {                     // the operands are there long before the weights
-            ok = wait_all(v_full + j % kStages, (j / kStages) & 1) && (j + 1 == n || wait_all(k_full + (j + 1) % kStages, ((j + 1) / kStages) & 1));
-            if (!ok) break;
-          }
-          if (!(ok = wait_all(p_ready + t, (j + 1) & 1))) break;
-          if (a.test_drop_mma && (blockIdx.x | blockIdx.y | blockIdx.z) == 0 && t == 0 && j == 1) continue;      // test hook
+          if (!(ok = wait_all(p_ready + t, (i + 1) & 1))) break;
+          if (a.test_drop_mma && (blockIdx.x | blockIdx.y | blockIdx.z) == 0 && t == 0 && i == 1) continue;      // test hook
           umma::fence_after_sync();
-          values(t, j);
-          if (j + 1 < n) scores(t, j + 1);
+          values(t, i);
+          if (i + 1 < n_sub) scores(t, i + 1);
         }
+      }
       if (!ok) {                            // whatever was issued has ended before tensor memory is given back
         if (leader) umma::commit(drain);
         for (int i = 0; i < 400 && !sleep_on(drain, 0); ++i) {}
@@ -298,8 +326,8 @@ __global__ void __launch_bounds__(kThreads, 1) paged8_prefill_kernel(Attn8Args a
     } else {
       // ---- codes to operands ----
       // Unit u of a tile (32 chunks of 16 codes): block u / 16 of 64 coordinates, group (u / 2) % 8 of 16 tokens, eight of
-      // whose tokens are four lanes' each.  This warp has units w, w + 7, ...  A thread converts the chunks that it copied.
-      const int w = warp - 9, sub = lane >> 2, c = lane & 3;
+      // whose tokens are four lanes' each.  This warp has units w, w + kConverters, ...  A thread converts the chunks that it copied.
+      const int w = warp - kSoft - 1, sub = lane >> 2, c = lane & 3;
       constexpr int kMine = (P::kUnits + kConverters - 1) / kConverters;
       const int32_t* row = a.table + seq * a.table_stride;
       const uint32_t to0 = sub * 128 + (((2 * c) ^ sub) << 4), to1 = sub * 128 + (((2 * c + 1) ^ sub) << 4);
@@ -397,12 +425,11 @@ __global__ void __launch_bounds__(kThreads, 1) paged8_prefill_kernel(Attn8Args a
     }
   } else {
     // ---- a query row per thread ----
-    if (D == 128) asm volatile("setmaxnreg.inc.sync.aligned.u32 192;\n");
-    else asm volatile("setmaxnreg.inc.sync.aligned.u32 200;\n");
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;\n" ::"n"(P::kSoftRegs));
     const int t = warp >> 2, r = r0 + tid;
     if (t < nt) {
       const bool live = r < r_end;
-      const uint32_t my = tmem + kTok * t + (static_cast<uint32_t>(32 * (warp & 3)) << 16);
+      const uint32_t lanes = static_cast<uint32_t>(32 * (warp & 3)) << 16, my = kSub * t + lanes, sums = P::kO + D * t + lanes;
       float unit;
       {
         const int row0 = 32 * (warp & 3), first = r0 + t * kRowsT + row0;
@@ -415,39 +442,41 @@ __global__ void __launch_bounds__(kThreads, 1) paged8_prefill_kernel(Attn8Args a
       const int lim = live ? static_cast<int>(max(min(visible8(a, s, r / a.G) - begin, a.chunk), static_cast<int64_t>(0))) - 1 : -1;
       float m = kNone, M = 0.5f * kNone, l = 0.f;
       bool ok = true;
-      for (int j = 0; j < n; ++j) {
-        if (!(ok = wait_all(m_full + j % kMetaSlots, (j / kMetaSlots) & 1))) break;
+      constexpr int kG = kSub / 16;
+      for (int i = 0; i < n_sub; ++i) {
+        const int j = i / kParts, g0 = i % kParts * kG;    // groups g0 .. of operand tile j
+        if (i % kParts == 0 && !(ok = wait_all(m_full + j % kMetaSlots, (j / kMetaSlots) & 1))) break;
         // factors of the scores, and of the weights as long as the references stay: while the scores come about
         const TileMeta& mt = meta[j % kMetaSlots];
-        float f[kGroups], ex[kGroups], up[kGroups];
+        float f[kG], ex[kG], up[kG];
 #pragma unroll
-        for (int g = 0; g < kGroups; ++g) {
-          f[g] = mt.ks[g] * unit;
-          ex[g] = mt.ex[g];
+        for (int g = 0; g < kG; ++g) {
+          f[g] = mt.ks[g0 + g] * unit;
+          ex[g] = mt.ex[g0 + g];
         }
         auto factors = [&] {
 #pragma unroll
-          for (int g = 0; g < kGroups; ++g) up[g] = mt.mant[g] * ex2(fminf(m + ex[g] - M, 120.f));
+          for (int g = 0; g < kG; ++g) up[g] = mt.mant[g0 + g] * ex2(fminf(m + ex[g] - M, 120.f));
         };
         factors();
-        const uint32_t bad = mt.bad;
-        if (!(ok = wait_all(s_full + t, j & 1))) break;
+        const uint32_t bad = (mt.bad >> g0) & ((1u << kG) - 1u);
+        if (!(ok = wait_all(s_full + t, i & 1))) break;
         umma::fence_after_sync();
-        uint32_t x[2][64];
-        umma::tmem_ld64_issue(my, x[0]);
-        umma::tmem_ld64_issue(my + 64, x[1]);
-        const int left = lim - j * kTok;                   // tokens 0 .. left of the tile are visible
-        const bool masked = __any_sync(QKV_FULL_MASK, left < kTok - 1) || bad != 0;
-        umma::tmem_ld64_wait(x[0]);
-        umma::tmem_ld64_wait(x[1]);
+        uint32_t x[kSub / 64][64];
+        const int left = lim - i * kSub;                   // tokens 0 .. left of the tile are visible
+        const bool masked = __any_sync(QKV_FULL_MASK, left < kSub - 1) || bad != 0;
+#pragma unroll
+        for (int hf = 0; hf < kSub / 64; ++hf) umma::tmem_ld64_issue(my + 64 * hf, x[hf]);
+#pragma unroll
+        for (int hf = 0; hf < kSub / 64; ++hf) umma::tmem_ld64_wait(x[hf]);
         float tm = -INFINITY, tM = -INFINITY;
         if (masked) {
 #pragma unroll
-          for (int g = 0; g < kGroups; ++g) {
+          for (int g = 0; g < kG; ++g) {
             float top = -INFINITY;
 #pragma unroll
-            for (int i = 0; i < 16; ++i) {
-              const int k = 16 * g + i;
+            for (int e = 0; e < 16; ++e) {
+              const int k = 16 * g + e;
               uint32_t& y = x[k >> 6][k & 63];
               const float v = (k > left || ((bad >> g) & 1u)) ? -INFINITY : __uint_as_float(y) * f[g];
               y = __float_as_uint(v);
@@ -459,11 +488,11 @@ __global__ void __launch_bounds__(kThreads, 1) paged8_prefill_kernel(Attn8Args a
           }
         } else {
 #pragma unroll
-          for (int g = 0; g < kGroups; ++g) {
-            auto at = [&](int i) { return __uint_as_float(x[(16 * g + i) >> 6][(16 * g + i) & 63]); };
+          for (int g = 0; g < kG; ++g) {
+            auto at = [&](int e) { return __uint_as_float(x[(16 * g + e) >> 6][(16 * g + e) & 63]); };
             float top[4];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) top[i] = max3(at(3 * i), at(3 * i + 1), at(3 * i + 2));
+            for (int e = 0; e < 4; ++e) top[e] = max3(at(3 * e), at(3 * e + 1), at(3 * e + 2));
             const float v = max3(max3(top[0], top[1], top[2]), max3(top[3], at(12), at(13)), fmaxf(at(14), at(15))) * f[g];
             tm = fmaxf(tm, v);
             tM = fmaxf(tM, v + ex[g]);
@@ -477,14 +506,14 @@ __global__ void __launch_bounds__(kThreads, 1) paged8_prefill_kernel(Attn8Args a
           m = m1;
           M = M1;
           factors();
-          if (j > 0) {
+          if (i > 0) {
 #pragma unroll 1
-            for (int c = 0; c < D; c += 32) {
-              uint32_t o[32];
-              umma::tmem_ld32(my + (P::kO + c), o);        // the sums of row tile t are kO columns behind its scores
+            for (int c = 0; c < D; c += 16) {
+              uint32_t o[16];
+              tmem_ld16(sums + c, o);
 #pragma unroll
-              for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * alpha);
-              tmem_st32(my + (P::kO + c), o);
+              for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * alpha);
+              umma::tmem_st16(sums + c, o);
             }
           }
         }
@@ -519,15 +548,15 @@ __global__ void __launch_bounds__(kThreads, 1) paged8_prefill_kernel(Attn8Args a
           tmem_st32(my + 32 * hf, wt);
         };
 #pragma unroll
-        for (int i = 0; i < 16; i += 2) argument(i);
+        for (int e = 0; e < 16; e += 2) argument(e);
 #pragma unroll
-        for (int g = 0; g <= kGroups; ++g) {
+        for (int g = 0; g <= kG; ++g) {
 #pragma unroll
-          for (int i = 0; i < 16; i += 2) {
-            if (g < kGroups) el(16 * g + i) = ex2v(el(16 * g + i));
-            if (g + 1 < kGroups) argument(16 * (g + 1) + i);
-            if (g < kGroups) el(16 * g + i + 1) = ex2v(el(16 * g + i + 1));
-            if (g > 0) weigh(16 * (g - 1) + i);
+          for (int e = 0; e < 16; e += 2) {
+            if (g < kG) el(16 * g + e) = ex2v(el(16 * g + e));
+            if (g + 1 < kG) argument(16 * (g + 1) + e);
+            if (g < kG) el(16 * g + e + 1) = ex2v(el(16 * g + e + 1));
+            if (g > 0) weigh(16 * (g - 1) + e);
           }
           if (g == 4) store(0);
           if (g == 8) store(1);
@@ -538,7 +567,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged8_prefill_kernel(Attn8Args a
         umma::fence_before_sync();
         arrive(p_ready + t);
       }
-      if (ok && n > 0) {
+      if (ok && n_sub > 0) {
         ok = wait_all(o_full + t, 0);
         umma::fence_after_sync();
       }
@@ -550,8 +579,8 @@ __global__ void __launch_bounds__(kThreads, 1) paged8_prefill_kernel(Attn8Args a
 #pragma unroll
       for (int c = 0; c < D; c += 32) {
         uint32_t o[32];
-        if (ok && n > 0) {
-          umma::tmem_ld32(my + (P::kO + c), o);
+        if (ok && n_sub > 0) {
+          umma::tmem_ld32(sums + c, o);
         } else {
 #pragma unroll
           for (int e = 0; e < 32; ++e) o[e] = ok ? 0u : 0x7fc00000u;
@@ -599,7 +628,7 @@ template <int D, int CODE>
 int launch(const Attn8Args& a, dim3 grid, cudaStream_t st) {
   constexpr auto kernel = paged8_prefill_kernel<D, CODE>;
   if (const int rc = allow_smem<kernel>(Pf8<D>::kSmem)) return rc;
-  kernel<<<grid, kThreads, Pf8<D>::kSmem, st>>>(a);
+  kernel<<<grid, Pf8<D>::kThreads, Pf8<D>::kSmem, st>>>(a);
   return check_launch();
 }
 
@@ -610,6 +639,8 @@ unsigned int prefill8_timeouts() {
   cudaMemcpyFromSymbol(&v, g_prefill8_timeouts, sizeof(v));
   return v;
 }
+
+int prefill8_rows(int d) { return d == 64 ? Pf8<64>::kRowsC : Pf8<128>::kRowsC; }
 
 int launch_prefill8(const Attn8Args& a_in, cudaStream_t st) {
   Attn8Args a = a_in;
