@@ -2,6 +2,9 @@
 arithmetic allows, and the three together as a serving loop uses them."""
 
 import math
+import os
+import subprocess
+import sys
 
 import numpy as np
 import pytest
@@ -315,24 +318,33 @@ def test_pieces_of_prompts_over_a_long_cache(d, H, G, q_len, x_dtype):
     _check_attention(flat, pages, table, _i32(lens), starts=starts, max_q_len=q_len)
 
 
-def test_a_wait_that_runs_out_gives_nan_and_is_counted(monkeypatch):
-    """The first CTA leaves out the products of one tile (nothing is left in flight): its waits give up, its rows are NaN
-    and no others, and the context stays usable."""
+def _a_wait_runs_out(d):
     from quashkv_b200 import _lib
     g = torch.Generator(device=DEV).manual_seed(1)
-    pages = ref.random_pages(g, 80, 2, 16, 128, E4M3)
+    pages = ref.random_pages(g, 80, 2, 16, d, E4M3)
     table = ref.random_tables([600, 500], 16, 80, 1).to(DEV)
-    q = torch.randn(2, 4, 300, 128, generator=g, device=DEV).bfloat16()
+    q = torch.randn(2, 4, 300, d, generator=g, device=DEV).bfloat16()
     want = paged8.attention_paged8(q, *pages, table, _i32([600, 500]), 600, causal=True)
     before = _lib.lib().qkv_tensor_core_timeouts()
-    monkeypatch.setenv("QUASHKV_B200_TEST_DROP_MMA", "1")
+    os.environ["QUASHKV_B200_TEST_DROP_MMA"] = "1"
     got = paged8.attention_paged8(q, *pages, table, _i32([600, 500]), 600, causal=True)
     torch.cuda.synchronize()
-    monkeypatch.delenv("QUASHKV_B200_TEST_DROP_MMA")
+    del os.environ["QUASHKV_B200_TEST_DROP_MMA"]
     assert _lib.lib().qkv_tensor_core_timeouts() > before
     bad = got.isnan().all(-1)
     assert bad.any() and not bad[1].any() and not bad[0, 2:].any() and torch.equal(got[~bad], want[~bad])
     assert torch.equal(paged8.attention_paged8(q, *pages, table, _i32([600, 500]), 600, causal=True), want)
+
+
+@pytest.mark.parametrize("d", [64, 128])
+def test_a_wait_that_runs_out_gives_nan_and_is_counted(d):
+    """The first CTA leaves out the products of one tile (nothing is left in flight): its waits give up, its rows are NaN
+    and no others, and the context stays usable.  In a process of its own: others count the waits of this one."""
+    here = os.path.dirname(os.path.abspath(__file__))
+    path = os.pathsep.join([here, os.path.dirname(here), os.environ.get("PYTHONPATH", "")])
+    child = subprocess.run([sys.executable, "-c", f"import test_gpu_paged8 as t; t._a_wait_runs_out({d})"], timeout=300, capture_output=True,
+                           text=True, env={**os.environ, "PYTHONPATH": path})
+    assert child.returncode == 0, child.stderr
 
 
 @pytest.mark.parametrize("q_len", [1, 90])
