@@ -140,9 +140,9 @@ __global__ void __launch_bounds__(kMostThreads) extend_kernel(ExtendArgs a) {
     return static_cast<int32_t>(max(static_cast<int64_t>(0), min(static_cast<int64_t>(start[i + 1] - start[i]), room)));
   };
   if (SLOTS) {
-    for (int32_t p = blockIdx.x * T + tid; p < given; p += gridDim.x * T) {
-      const int i = owner(page, a.n, p);
-      const int j = bs.pages(len[i], a.max_blocks) + p - page[i];
+    for (int64_t p = static_cast<int64_t>(blockIdx.x) * T + tid; p < given; p += static_cast<int64_t>(gridDim.x) * T) {
+      const int i = owner(page, a.n, static_cast<int32_t>(p));
+      const int j = bs.pages(len[i], a.max_blocks) + static_cast<int32_t>(p) - page[i];
       a.table[i * a.table_stride + j] = a.free_pages[left - 1 - p];
     }
     const int32_t total = start[a.n];
@@ -208,9 +208,9 @@ __global__ void __launch_bounds__(kMostThreads) shrink_kernel(ShrinkArgs a) {
   __syncthreads();
   scan_cta(page, a.n);
   const int64_t now = left + page[a.n];
-  for (int32_t p = blockIdx.x * T + tid; p < page[a.n]; p += gridDim.x * T) {
-    const int i = owner(page, a.n, p);
-    const int j = bs.pages(len[i], a.max_blocks) + p - page[i];
+  for (int64_t p = static_cast<int64_t>(blockIdx.x) * T + tid; p < page[a.n]; p += static_cast<int64_t>(gridDim.x) * T) {
+    const int i = owner(page, a.n, static_cast<int32_t>(p));
+    const int j = bs.pages(len[i], a.max_blocks) + static_cast<int32_t>(p) - page[i];
     const int64_t at = now - 1 - p;
     if (at < a.n_pages) a.free_pages[at] = a.table[i * a.table_stride + j];
   }
