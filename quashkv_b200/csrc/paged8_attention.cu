@@ -619,9 +619,13 @@ __global__ void __launch_bounds__(128) paged8_merge_kernel(Attn8Args a) {
   }
 }
 
-// How a call is carried out.  Sequences of up to `few` rows (query tokens x query heads of a KV head) go to the split kernel,
-// those of more to the prefill kernel where it exists (head size 64 and 128, 16-bit queries).
-constexpr int kFewRows = 32;
+// How a call is carried out.  Sequences of few rows (query tokens x query heads of a KV head) go to the split kernel, those of
+// more to the prefill kernel where it exists (head size 64 and 128, 16-bit queries).  us, split / prefill, 16 sequences of 16384
+// tokens: 8 KV heads of 128: 48 rows 350 / 520, 64 rows 444 / 525, 96 rows 647 / 533; 4 of 64: 64 rows 160 / 220, 96 rows 222 / 220, 128
+// rows 272 / 181; 64 x 1024 tokens: 64 rows 157 / 155 and 53 / 69, 96 rows 229 / 157 and 73 / 69.  In a ragged batch the
+// split kernel has CTAs for the most rows of every sequence, which mostly end at once: 63 single tokens and a
+// piece of 1985 over 4096 tokens 340 us with CTAs for 32 rows, 352 for 64.
+constexpr int kFewRows = 64, kFewRagged = 32;
 
 struct Plan8 { int ng, row_tiles, most_rows, n_splits; bool cluster; int64_t chunk, part_rows; size_t ws; };
 
@@ -654,13 +658,13 @@ Plan8 plan_split(int n_seq, int Hkv, int most_rows, int rows_used, int64_t max_k
   return p;
 }
 
-// `tokens`: query tokens of all sequences.
-Plan8 plan_prefill(int Hkv, int G, int q_len, int64_t tokens, int64_t max_kv_len, int d) {
+// `tokens`: query tokens of all sequences, of which a ragged batch may have a few that are long (counted as if they were one).
+Plan8 plan_prefill(int n_seq, int Hkv, int G, int q_len, bool ragged, int64_t tokens, int64_t max_kv_len, int d) {
   Plan8 p{};
   p.most_rows = G * q_len;
   const int rows = prefill8_rows(d);
   p.row_tiles = (p.most_rows + rows - 1) / rows;
-  const int64_t ctas = (tokens * G + rows - 1) / rows * Hkv;
+  const int64_t ctas = (ragged ? (tokens * G + rows - 1) / rows : static_cast<int64_t>(n_seq) * p.row_tiles) * Hkv;
   int64_t splits = ctas > 0 ? kNumSMs / ctas : 1;
   const int64_t most = max_kv_len / 512;
   if (splits > most) splits = most;
@@ -681,10 +685,11 @@ struct Route8 { bool split, prefill; Plan8 s, p; size_t ws; };
 Route8 route8(int n_seq, int Hkv, int G, int q_len, bool ragged, int64_t tokens, int64_t max_kv_len, int d, int dtype) {
   Route8 r{};
   const int rows = G * q_len;
-  r.prefill = rows > kFewRows && dtype != QKV_F32 && (d == 64 || d == 128);
-  r.split = !r.prefill || (ragged && G <= kFewRows);
-  if (r.split) r.s = plan_split(n_seq, Hkv, r.prefill ? kFewRows : rows, r.prefill ? G : rows, max_kv_len, d, dtype);
-  if (r.prefill) r.p = plan_prefill(Hkv, G, q_len, tokens, max_kv_len, d);
+  const int few = ragged ? kFewRagged : kFewRows;
+  r.prefill = rows > few && dtype != QKV_F32 && (d == 64 || d == 128);
+  r.split = !r.prefill || ragged;                          // (it clears the rows of no sequence, too)
+  if (r.split) r.s = plan_split(n_seq, Hkv, r.prefill ? few : rows, r.prefill ? G : rows, r.prefill && G > few ? 0 : max_kv_len, d, dtype);
+  if (r.prefill) r.p = plan_prefill(n_seq, Hkv, G, q_len, ragged, tokens, max_kv_len, d);
   r.ws = r.s.ws + r.p.ws;                                  // they overlap: each has a place of its own
   return r;
 }
@@ -817,8 +822,7 @@ extern "C" int qkv_attention_paged8(const void* q, int q_dtype, const int64_t* q
   if (r.prefill) {
     p.tile_rows = prefill8_rows(pages.d);
     p.by_token = 1;
-    p.few_rows = r.split ? kFewRows : 0;
-    p.zeros = !r.split;
+    p.few_rows = r.split ? kFewRagged : 0;
     if (static_cast<int64_t>(n_seq) * a.Hkv > 0x7fffffffLL || p.row_tiles > 65535) return QKV_EDIM;
     if (const int rc = launch_prefill8(p, st)) return rc;
   }

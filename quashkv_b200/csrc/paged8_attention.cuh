@@ -24,7 +24,6 @@ struct Attn8Args {
   int by_token;                             // most_rows: nor are those of more.  by_token: see part_row8
   int in_cluster;                           // split kernel: the splits of a row tile are one cluster
   int behind_prefill;                       // split kernel: it overlaps the prefill kernel and has to end after it
-  int zeros;                                // prefill kernel: rows of no sequence are its own to clear
   int test_drop_mma;                        // test hook of the prefill kernel
 };
 
@@ -63,20 +62,20 @@ __device__ __forceinline__ int64_t visible8(const Attn8Args& a, const Span8& s, 
 }
 
 // Ragged queries: output rows in front of the first sequence, behind the last one, and of a sequence beyond the promised
-// q_len are zeros.  By the CTA that comes first for (sequence, KV head).
+// q_len are zeros.  By the CTA that comes first for (sequence, KV head); all of a head's clear what is behind the last sequence.
 __device__ __forceinline__ void zero_gaps8(const Attn8Args& a, const Span8& s, int seq, int h) {
   const int item = a.dtype == QKV_F32 ? 4 : 2, chunks = a.p.d * item / 16;
-  auto clear = [&](int64_t lo, int64_t hi) {               // tokens
-    for (int64_t x = threadIdx.x; x < (hi - lo) * a.G * chunks; x += blockDim.x) {
+  auto clear = [&](int64_t lo, int64_t hi, int part, int parts) {      // tokens
+    for (int64_t x = part * static_cast<int64_t>(blockDim.x) + threadIdx.x; x < (hi - lo) * a.G * chunks; x += parts * static_cast<int64_t>(blockDim.x)) {
       const int64_t row = x / chunks;
       const int c = static_cast<int>(x - row * chunks);
       char* at = static_cast<char*>(a.out) + ((lo + row / a.G) * a.o_stride[1] + (h * a.G + row % a.G) * a.o_stride[2]) * item;
       reinterpret_cast<uint4*>(at)[c] = make_uint4(0, 0, 0, 0);
     }
   };
-  if (s.q_len < s.q_all) clear(s.tok0 + s.q_len, s.tok0 + s.q_all);
-  if (seq == 0 && s.tok0 > 0) clear(0, s.tok0);
-  if (seq == a.n_seq - 1 && s.tok0 + s.q_all < a.total_q) clear(s.tok0 + s.q_all, a.total_q);
+  if (s.q_len < s.q_all) clear(s.tok0 + s.q_len, s.tok0 + s.q_all, 0, 1);
+  if (seq == 0 && s.tok0 > 0) clear(0, s.tok0, 0, 1);
+  clear(min(static_cast<int64_t>(max(a.starts[a.n_seq], 0)), a.total_q), a.total_q, seq, a.n_seq);
 }
 
 // Row r of KV head h among the partial results: places for most_rows rows of every sequence and head, or, where sequences differ

@@ -157,6 +157,26 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
   return d;
 }
 
+// A ragged batch as one row of tiles: a sequence's first one is its rows' place among all, in tiles, plus its number, which
+// leaves each room enough for its own (ceil(b - a) <= floor(b) - floor(a) + 1).
+__device__ __forceinline__ int first_tile(const Attn8Args& a, int seq, int rows) {
+  const int64_t tok = min(static_cast<int64_t>(max(a.starts[seq], 0)), a.total_q);
+  return static_cast<int>(tok * a.G / rows) + seq;
+}
+// The last sequence whose first tile is not behind `tile` (or 0), by a warp: 32 at a time.
+__device__ __forceinline__ int owner_of(const Attn8Args& a, int tile, int rows) {
+  const int lane = threadIdx.x & 31;
+  int lo = 0, n = a.n_seq;
+  while (n > 1) {
+    const int step = (n + 31) / 32, k = lane * step;
+    const uint32_t in = __ballot_sync(QKV_FULL_MASK, k < n && first_tile(a, lo + (k < n ? k : 0), rows) <= tile);
+    const int skip = in ? (__popc(in) - 1) * step : 0;
+    lo += skip;
+    n = min(step, n - skip);
+  }
+  return lo;
+}
+
 // Where row r of a CTA's (sequence, KV head) lies in the queries or the output, in elements.
 __device__ __forceinline__ int64_t row_at(const Attn8Args& a, int64_t row0, const int64_t* stride, int h, int r) {
   const int tok = r / a.G;
@@ -215,7 +235,8 @@ __device__ __forceinline__ float stage_queries(const Attn8Args& a, const Span8& 
   return unit;
 }
 
-template <int D, int CODE>
+// PACKED: a ragged batch's tiles behind one another.
+template <int D, int CODE, bool PACKED>
 __global__ void __launch_bounds__(Pf8<D>::kThreads, 1) paged8_prefill_kernel(Attn8Args a) {
   using P = Pf8<D>;
   extern __shared__ __align__(1024) unsigned char smem[];
@@ -240,12 +261,12 @@ __global__ void __launch_bounds__(Pf8<D>::kThreads, 1) paged8_prefill_kernel(Att
   volatile int* dead = reinterpret_cast<volatile int*>(tmem_slot + 1);
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
 
-  const int h = blockIdx.x % a.Hkv, seq = blockIdx.x / a.Hkv;
+  const int order = gridDim.y - 1 - blockIdx.y, h = blockIdx.x % a.Hkv;      // long rows first
+  const int seq = PACKED ? owner_of(a, order, P::kRowsC) : blockIdx.x / a.Hkv;
   const Span8 s = span8(a, seq);
   asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");
-  if (a.starts && a.zeros && blockIdx.y == 0 && blockIdx.z == 0) zero_gaps8(a, s, seq, h);
-  const int rows = a.G * s.q_len, r0 = (gridDim.y - 1 - blockIdx.y) * P::kRowsC;      // long rows first
-  if (r0 >= rows || rows <= a.few_rows) return;
+  const int rows = a.G * s.q_len, r0 = (PACKED ? order - first_tile(a, seq, P::kRowsC) : order) * P::kRowsC;
+  if ((PACKED && r0 < 0) || r0 >= rows || rows <= a.few_rows) return;
   const int r_end = min(r0 + P::kRowsC, rows), nt = (r_end - r0 + kRowsT - 1) / kRowsT;
   const int64_t seen = visible8(a, s, (r_end - 1) / a.G);
   const int64_t begin = static_cast<int64_t>(blockIdx.z) * a.chunk, stop = min(seen, begin + a.chunk);
@@ -624,12 +645,16 @@ __global__ void __launch_bounds__(Pf8<D>::kThreads, 1) paged8_prefill_kernel(Att
   if (warp == 0) umma::tmem_dealloc(*tmem_slot, 512);
 }
 
-template <int D, int CODE>
-int launch(const Attn8Args& a, dim3 grid, cudaStream_t st) {
-  constexpr auto kernel = paged8_prefill_kernel<D, CODE>;
+template <int D, int CODE, bool PACKED>
+int launch_as_is(const Attn8Args& a, dim3 grid, cudaStream_t st) {
+  constexpr auto kernel = paged8_prefill_kernel<D, CODE, PACKED>;
   if (const int rc = allow_smem<kernel>(Pf8<D>::kSmem)) return rc;
   kernel<<<grid, Pf8<D>::kThreads, Pf8<D>::kSmem, st>>>(a);
   return check_launch();
+}
+template <int D, int CODE>
+int launch(const Attn8Args& a, dim3 grid, bool packed, cudaStream_t st) {
+  return packed ? launch_as_is<D, CODE, true>(a, grid, st) : launch_as_is<D, CODE, false>(a, grid, st);
 }
 
 }  // namespace
@@ -646,9 +671,12 @@ int launch_prefill8(const Attn8Args& a_in, cudaStream_t st) {
   Attn8Args a = a_in;
   const char* e = getenv("QUASHKV_B200_TEST_DROP_MMA");
   a.test_drop_mma = e && e[0] == '1';
-  const dim3 grid(static_cast<unsigned>(a.n_seq) * a.Hkv, a.row_tiles, a.n_splits);
-  if (a.p.d == 64) return a.p.code == QKV_E4M3 ? launch<64, p8::kE4M3>(a, grid, st) : launch<64, p8::kInt8>(a, grid, st);
-  return a.p.code == QKV_E4M3 ? launch<128, p8::kE4M3>(a, grid, st) : launch<128, p8::kInt8>(a, grid, st);
+  // A ragged batch is one row of tiles where that is fewer than the most rows for each sequence, whose CTAs have mostly nothing.
+  const int64_t tiles = a.total_q * a.G / a.tile_rows + a.n_seq;
+  const bool packed = a.starts && tiles < static_cast<int64_t>(a.n_seq) * a.row_tiles && tiles <= 65535;
+  const dim3 grid(static_cast<unsigned>(packed ? 1 : a.n_seq) * a.Hkv, static_cast<unsigned>(packed ? tiles : a.row_tiles), a.n_splits);
+  if (a.p.d == 64) return a.p.code == QKV_E4M3 ? launch<64, p8::kE4M3>(a, grid, packed, st) : launch<64, p8::kInt8>(a, grid, packed, st);
+  return a.p.code == QKV_E4M3 ? launch<128, p8::kE4M3>(a, grid, packed, st) : launch<128, p8::kInt8>(a, grid, packed, st);
 }
 
 }  // namespace qkv

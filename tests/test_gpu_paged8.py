@@ -77,6 +77,24 @@ def test_extend_at_its_limits():
     _check_extend(rs, 7, 600, 16, rs.randint(0, 9000, 7), 4000)                           # long ones
 
 
+@pytest.mark.parametrize("spare", [40, 900])
+def test_a_large_step_updates_lengths_in_place(spare):
+    """More tokens than one CTA takes: lengths and counts change behind all that read them, pages lasting and not."""
+    n, w, bs, most = 50, 60, 16, 9000
+    tables = paged8.PageTables(spare, n, w, block_size=bs)
+    rs, free = np.random.RandomState(spare), tables.free_pages.cpu().numpy()
+    held, pool, table = [0] * n, tables.pool.tolist(), tables.block_table.cpu().numpy()
+    for _ in range(3):
+        new = rs.randint(0, 200, n)
+        plan = tables.extend(_i32(new), most)
+        table, slots, starts, after, pool = ref.extend(table, held, new.tolist(), free, pool, bs, most)
+        assert plan.slots.tolist() == slots and plan.query_starts.tolist() == starts and plan.start_lens.tolist() == held
+        assert tables.seq_lens.tolist() == after and tables.pool.tolist() == pool
+        have = [-(-x // bs) for x in after]
+        assert all(np.array_equal(tables.block_table[i, :k].cpu().numpy(), table[i, :k]) for i, k in enumerate(have))
+        held = after
+
+
 @pytest.mark.parametrize("n,bs", [(1, 16), (33, 16), (700, 1), (16384, 48)])
 def test_shrink_restores_what_extend_took(n, bs):
     rs = np.random.RandomState(n)
@@ -146,6 +164,25 @@ def test_append_equals_the_definition(d, H, bs, layout, x_dtype, dtype):
         x = x.to(x_dtype)
         keys, values = x[:, :H], x[:, H:2 * H]                     # strided, as a projection gives them
         _check_append(keys, values, pages, slots, bs, dtype, lambda: paged8.append_paged8(keys, values, *pages, torch.from_numpy(slots).to(DEV)))
+
+
+@pytest.mark.parametrize("total", [300, 900, 1500, 2600, 5000])
+def test_append_of_runs_of_any_length(total):
+    """Runs of 1 to 20 tokens on pages of their own, in calls whose warps look for the runs of few or many tokens."""
+    rs, g = np.random.RandomState(total), torch.Generator(device=DEV).manual_seed(total)
+    H, d, bs = 4, 32, 32
+    slots, page = [], 0
+    while len(slots) < total:
+        n, at = rs.randint(1, 21), rs.randint(0, 12)
+        slots += list(range(page * bs + at, page * bs + at + n))
+        page += 1
+    slots = np.array(slots[:total])
+    order = rs.permutation(page)                             # pages in any order
+    slots = order[slots // bs] * bs + slots % bs
+    slots[slots // bs == slots[total // 2] // bs] = -1       # a page that is left out
+    k, v = (torch.randn(total, H, d, generator=g, device=DEV).bfloat16() for _ in range(2))
+    pages = _pool(page, H, bs, d, E4M3, "hnd")
+    _check_append(k, v, pages, slots.tolist(), bs, E4M3, lambda: paged8.append_paged8(k, v, *pages, torch.from_numpy(slots).to(DEV)))
 
 
 @pytest.mark.parametrize("dtype", [E4M3, INT8])
@@ -334,6 +371,67 @@ def _a_wait_runs_out(d):
     bad = got.isnan().all(-1)
     assert bad.any() and not bad[1].any() and not bad[0, 2:].any() and torch.equal(got[~bad], want[~bad])
     assert torch.equal(paged8.attention_paged8(q, *pages, table, _i32([600, 500]), 600, causal=True), want)
+
+
+@pytest.mark.parametrize("d,H,G", [(128, 2, 4), (64, 3, 5), (128, 1, 32)])
+def test_a_padded_ragged_batch(d, H, G):
+    """Many sequences, most of one token, some of pieces that end anywhere in a tile of rows; rows in front of the first
+    sequence and far behind the last; more rows allowed for a sequence than any has, and fewer."""
+    g = torch.Generator(device=DEV).manual_seed(G)
+    for new, front, behind in (([1] * 30 + [9, 500, 1, 0, 65, 64, 63, 0, 1], 0, 700), ([300] + [1] * 70, 3, 1), ([1] * 40 + [128] * 3, 5, 0), ([40] * 33, 0, 2000)):
+        lens = [n + (37 * i) % 900 for i, n in enumerate(new)]
+        total = sum(-(-n // 16) for n in lens) + 1
+        pages = ref.random_pages(g, total, H, 16, d, INT8, "nhd")
+        table = ref.random_tables(lens, 16, total, 5).to(DEV)
+        starts = (front + np.r_[0, np.cumsum(new)]).tolist()
+        q = torch.randn(starts[-1] + behind, H * G, d, generator=g, device=DEV).bfloat16()
+        torch.full_like(q, math.nan)                         # (what the result's memory may hold)
+        _check_attention(q, pages, table, _i32(lens), starts=starts)
+        torch.full_like(q, math.nan)
+        got = paged8.attention_paged8(q, *pages, table, _i32(lens), max(lens), query_starts=_i32(starts), max_q_len=60, causal=True)
+        exact, bound = ref.attention(q, pages, table, _i32(lens), 1 / math.sqrt(d), True, starts)
+        for i, n in enumerate(new):                          # the rows that are allowed for see what they saw
+            kept = slice(starts[i], starts[i] + min(n, 60))
+            assert ((got[kept].double() - exact[kept]).abs() <= bound[kept]).all()
+            assert not got[starts[i] + min(n, 60):starts[i + 1]].any()
+        assert not got[:front].any() and not got[starts[-1]:].any()
+
+
+def test_graphs_of_a_mixed_batch_on_two_streams():
+    """Prompt pieces and single tokens over caches long enough that both are split, captured twice and replayed side by
+    side with lengths that change between replays."""
+    g = torch.Generator(device=DEV).manual_seed(3)
+    H, G, d, bs, n, T = 2, 4, 128, 16, 12, 160
+    pages = ref.random_pages(g, n * 400, H, bs, d, E4M3)
+    table = ref.random_tables([6400] * n, bs, n * 400, 1).to(DEV)
+    sides = []
+    for _ in range(2):
+        q, lens, starts = torch.randn(T, H * G, d, generator=g, device=DEV).bfloat16(), _i32([1] * n), _i32([0] * (n + 1))
+        call = lambda q=q, lens=lens, starts=starts: paged8.attention_paged8(q, *pages, table, lens, 6400, causal=True, query_starts=starts)      # noqa: E731
+        stream, graph = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+        with torch.cuda.stream(stream):
+            call()
+        stream.synchronize()
+        with torch.cuda.graph(graph):
+            out = call()
+        sides.append((q, lens, starts, call, stream, graph, out))
+    rs = np.random.RandomState(0)
+    for step in range(6):
+        for q, lens, starts, call, stream, graph, out in sides:
+            new = np.ones(n, dtype=np.int64)
+            new[rs.randint(n)] = [1, 40, 149, 9, 100, 0][step]
+            lens.copy_(_i32(rs.randint(149, 6400, n)))
+            starts.copy_(_i32(np.r_[0, np.cumsum(new)]))
+        want = [side[3]() for side in sides]
+        torch.cuda.synchronize()
+        for _ in range(3):
+            for side in sides:
+                with torch.cuda.stream(side[4]):
+                    side[5].replay()
+        torch.cuda.synchronize()
+        for side, exact in zip(sides, want):
+            assert torch.equal(side[6], exact)
+            _check_attention(side[0], pages, table, side[1], starts=side[2].tolist(), max_kv_len=6400)
 
 
 @pytest.mark.parametrize("d", [64, 128])
