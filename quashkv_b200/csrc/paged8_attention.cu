@@ -517,64 +517,64 @@ constexpr int kTogether = 4;
 
 template <int D, int R>
 __global__ void __launch_bounds__(128) paged8_merge_kernel(Attn8Args a) {
+  constexpr int kU = R > 1 ? 1 : 2, kP = R > 1 ? 4 : 8;    // a lane's parts (the prefill kernel makes up to 32); parts in flight
   const int lane = threadIdx.x & 31, c = 4 * lane;
-  const int64_t job = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 5);
+  const uint32_t job = blockIdx.x * 4 + (threadIdx.x >> 5), chunk = static_cast<uint32_t>(a.chunk);      // (32 bits: divisions of 64 took most of the time)
   asm volatile("griddepcontrol.wait;\n" ::: "memory");
   int seq, h, rr, rows_here = 1;
   int64_t row0;                                            // among the partial results
   Span8 s;
   if (R > 1) {
-    const int hq = a.Hkv * a.G, groups = (hq + R - 1) / R, head = static_cast<int>(job % groups) * R;
-    const int64_t tok = job / groups;
+    const uint32_t hq = a.Hkv * a.G, groups = (hq + R - 1) / R, tok = job / groups, head = (job - tok * groups) * R;
     if (tok >= (a.starts ? a.total_q : static_cast<int64_t>(a.n_seq) * a.q_len)) return;
-    if (a.starts) {                                        // the last sequence that starts at or in front of it
-      int lo = 0, hi = a.n_seq;
-      while (hi - lo > 1) {
-        const int mid = (lo + hi) >> 1;
-        if (a.starts[mid] <= tok) lo = mid; else hi = mid;
+    if (a.starts) {                                        // the last sequence that starts at or in front of it: 32 at a time
+      int lo = 0, n = a.n_seq;
+      while (n > 1) {
+        const int step = (n + 31) / 32, k = lane * step;
+        const uint32_t in = __ballot_sync(QKV_FULL_MASK, k < n && a.starts[lo + (k < n ? k : 0)] <= static_cast<int64_t>(tok));
+        const int skip = in ? (__popc(in) - 1) * step : 0;
+        lo += skip;
+        n = min(step, n - skip);
       }
       seq = lo;
     } else {
-      seq = static_cast<int>(tok / a.q_len);
+      seq = static_cast<int>(tok / static_cast<uint32_t>(a.q_len));
     }
     s = span8(a, seq);
     if (tok < s.tok0 || tok - s.tok0 >= s.q_len) return;
     h = head / a.G;
     rr = static_cast<int>(tok - s.tok0) * a.G + head % a.G;
-    rows_here = min(R, hq - head);
-    row0 = tok * hq + head;
+    rows_here = min(static_cast<uint32_t>(R), hq - head);
+    row0 = static_cast<int64_t>(tok) * hq + head;
   } else {
-    const int64_t head = job / a.most_rows;
+    const uint32_t head = job / static_cast<uint32_t>(a.most_rows);
     if (head >= static_cast<int64_t>(a.n_seq) * a.Hkv) return;
-    rr = static_cast<int>(job % a.most_rows);
-    h = static_cast<int>(head % a.Hkv);
+    rr = static_cast<int>(job - head * a.most_rows);
     seq = static_cast<int>(head / a.Hkv);
+    h = static_cast<int>(head - seq * static_cast<uint32_t>(a.Hkv));
     s = span8(a, seq);
     row0 = job;
   }
   const int rows = a.G * s.q_len;
   if (rr >= rows || rows > a.most_rows || rows <= a.few_rows) return;
-  const int tile_end = min((rr / a.tile_rows + 1) * a.tile_rows, rows);
   // (rows of a token are of one tile or of neighbours, whose last tokens differ: the parts are counted for each)
-  float4 q[R][2];
+  const int in_head = rr % a.G, first = rr - in_head;      // head h * G + in_head of the token, then the next ones (of the next KV heads, too)
+  float4 q[R][kU];
   float mt[R], Mt[R], lt[R];
   int parts[R], most = 0;
 #pragma unroll
   for (int r = 0; r < R; ++r) {
-    // head h * G + rr % G of the token, then the next ones (of the next KV heads, too)
-    const int in = rr % a.G + r, row = rr - rr % a.G + in % a.G;
-    const int te = R > 1 ? min((row / a.tile_rows + 1) * a.tile_rows, rows) : tile_end;
-    const int64_t end = visible8(a, s, (te - 1) / a.G);
-    parts[r] = r < rows_here ? (end > a.chunk ? static_cast<int>((end + a.chunk - 1) / a.chunk) : 1) : 0;
+    const int row = first + (in_head + r) % a.G, te = min((row / a.tile_rows + 1) * a.tile_rows, rows);
+    const uint32_t end = static_cast<uint32_t>(visible8(a, s, (te - 1) / a.G));
+    parts[r] = r < rows_here ? (end > chunk ? static_cast<int>((end + chunk - 1) / chunk) : 1) : 0;
     most = max(most, parts[r]);
   }
 #pragma unroll
   for (int r = 0; r < R; ++r)
 #pragma unroll
-    for (int u = 0; u < 2; ++u)
+    for (int u = 0; u < kU; ++u)
       q[r][u] = lane + 32 * u < parts[r] ? *reinterpret_cast<const float4*>(a.ref + ((row0 + r) * a.n_splits + lane + 32 * u) * 4) : make_float4(kNone, 0.5f * kNone, 0.f, 0.f);
-  float4 y[R][8 / (R > 1 ? 2 : 1)];
-  constexpr int kP = R > 1 ? 4 : 8;
+  float4 y[R][kP];
   auto fetch = [&](int p0) {
 #pragma unroll
     for (int r = 0; r < R; ++r)
@@ -584,28 +584,48 @@ __global__ void __launch_bounds__(128) paged8_merge_kernel(Attn8Args a) {
   };
   fetch(0);
   float4 o[R];
+  // lanes that hold parts: the first ones, a power of two
+  const int width = most > 16 ? 32 : (most > 8 ? 16 : (most > 4 ? 8 : (most > 2 ? 4 : 2)));
 #pragma unroll
   for (int r = 0; r < R; ++r) {
-    mt[r] = max_or_nan(q[r][0].x, q[r][1].x);
-    Mt[r] = max_or_nan(q[r][0].y, q[r][1].y);
+    mt[r] = q[r][0].x;
+    Mt[r] = q[r][0].y;
+    if (kU > 1) {
+      mt[r] = max_or_nan(mt[r], q[r][kU - 1].x);
+      Mt[r] = max_or_nan(Mt[r], q[r][kU - 1].y);
+    }
+  }
+#pragma unroll 1
+  for (int x = width >> 1; x > 0; x >>= 1)
 #pragma unroll
-    for (int x = 16; x > 0; x >>= 1) {
+    for (int r = 0; r < R; ++r) {
       mt[r] = max_or_nan(mt[r], __shfl_xor_sync(QKV_FULL_MASK, mt[r], x));
       Mt[r] = max_or_nan(Mt[r], __shfl_xor_sync(QKV_FULL_MASK, Mt[r], x));
     }
-    lt[r] = fmaf(q[r][0].z, ex2(q[r][0].x - mt[r]), q[r][1].z * ex2(q[r][1].x - mt[r]));
-    q[r][0].w = ex2(q[r][0].y - Mt[r]);
-    q[r][1].w = ex2(q[r][1].y - Mt[r]);
 #pragma unroll
-    for (int x = 16; x > 0; x >>= 1) lt[r] += __shfl_xor_sync(QKV_FULL_MASK, lt[r], x);
+  for (int r = 0; r < R; ++r) {
+    mt[r] = __shfl_sync(QKV_FULL_MASK, mt[r], 0);
+    Mt[r] = __shfl_sync(QKV_FULL_MASK, Mt[r], 0);
+    lt[r] = 0.f;
+#pragma unroll
+    for (int u = 0; u < kU; ++u) {
+      lt[r] = fmaf(q[r][u].z, ex2(q[r][u].x - mt[r]), lt[r]);
+      q[r][u].w = ex2(q[r][u].y - Mt[r]);
+    }
     o[r] = make_float4(0.f, 0.f, 0.f, 0.f);
   }
+#pragma unroll 1
+  for (int x = width >> 1; x > 0; x >>= 1)
+#pragma unroll
+    for (int r = 0; r < R; ++r) lt[r] += __shfl_xor_sync(QKV_FULL_MASK, lt[r], x);
+#pragma unroll
+  for (int r = 0; r < R; ++r) lt[r] = __shfl_sync(QKV_FULL_MASK, lt[r], 0);
   for (int p0 = 0;;) {
 #pragma unroll
     for (int r = 0; r < R; ++r)
 #pragma unroll
       for (int k = 0; k < kP; ++k) {
-        const float f = __shfl_sync(QKV_FULL_MASK, p0 + k < 32 ? q[r][0].w : q[r][1].w, (p0 + k) & 31);
+        const float f = __shfl_sync(QKV_FULL_MASK, p0 + k < 32 ? q[r][0].w : q[r][kU - 1].w, (p0 + k) & 31);
         o[r].x = fmaf(y[r][k].x, f, o[r].x); o[r].y = fmaf(y[r][k].y, f, o[r].y); o[r].z = fmaf(y[r][k].z, f, o[r].z); o[r].w = fmaf(y[r][k].w, f, o[r].w);
       }
     p0 += kP;
@@ -614,8 +634,8 @@ __global__ void __launch_bounds__(128) paged8_merge_kernel(Attn8Args a) {
   }
 #pragma unroll
   for (int r = 0; r < R; ++r) {
-    const int in = rr % a.G + r;
-    if (c < D && r < rows_here) store_out8(a, s, h + in / a.G, rr - rr % a.G + in % a.G, c, o[r], mt[r], Mt[r], lt[r]);
+    const int in = in_head + r;
+    if (c < D && r < rows_here) store_out8(a, s, h + in / a.G, first + in % a.G, c, o[r], mt[r], Mt[r], lt[r]);
   }
 }
 
@@ -721,7 +741,7 @@ int launch_merge(const Attn8Args& a, cudaStream_t st) {
   if (a.n_splits == 1 || a.in_cluster) return QKV_OK;
   const int64_t rows = a.by_token ? (a.starts ? a.total_q : static_cast<int64_t>(a.n_seq) * a.q_len) * ((a.Hkv * a.G + kTogether - 1) / kTogether)
                                   : static_cast<int64_t>(a.n_seq) * a.Hkv * a.most_rows;      // a warp each
-  if ((rows + 3) / 4 > 0x7fffffffLL) return QKV_EDIM;
+  if (rows > 0x7fffffffLL) return QKV_EDIM;
   return launch_as(a.by_token ? paged8_merge_kernel<D, kTogether> : paged8_merge_kernel<D, 1>, dim3(static_cast<unsigned>((rows + 3) / 4)), 128, 0, a, true, 1, st);
 }
 
