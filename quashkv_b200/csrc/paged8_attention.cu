@@ -18,7 +18,10 @@
 // of large values that a row hardly weighs takes no bits from the others.  References rise when a score is 4 above them,
 // which is rare after the first granules.
 //
-// Bound by the bytes of the pages: (2 D + 8 / block_size) a token and KV head.
+// Bound by the bytes of the pages: (2 D + 8 / block_size) a token and KV head.  Measured, 32 x 8 KV heads x 32768 tokens of 128, four
+// bf16 queries a head: 370 us, 5.8 TB/s; the schedulers' issue slots are 48 % busy, their three warps mostly wait for results of their own.
+// fp32 queries take four MMAs in place of one, and 16 rows fill the registers (two CTAs an SM): 32 sequences of up to 16384
+// tokens, 16 rows a head: 236 us, 2.6 TB/s, bound by the latency of a warp's own chain.
 #include <math.h>
 
 #include <cooperative_groups.h>
@@ -653,7 +656,7 @@ struct Plan8 { int ng, row_tiles, most_rows, n_splits; bool cluster; int64_t chu
 Plan8 plan_split(int n_seq, int Hkv, int most_rows, int rows_used, int64_t max_kv_len, int d, int dtype) {
   Plan8 p{};
   p.most_rows = most_rows;
-  p.ng = rows_used > 8 ? 2 : 1;
+  p.ng = rows_used > 8 ? 2 : 1;                            // groups of eight rows in a CTA (16 fp32 rows a head: 236 us in one, 288 in two)
   p.row_tiles = (p.most_rows + 8 * p.ng - 1) / (8 * p.ng);
   const int tiles_used = (rows_used + 8 * p.ng - 1) / (8 * p.ng);
   // Tokens of a split.  What fits one wave of resident CTAs is cut into one (each at least a step of its four warps); more
@@ -662,6 +665,8 @@ Plan8 plan_split(int n_seq, int Hkv, int most_rows, int rows_used, int64_t max_k
   // 32 x 8 x up to 1278: 128 tokens 54 us (the whole step), 256 47, 512 and more 44; 8 heads x 1000: 64 tokens 11.6 us, 128 11.2, 512 13.7.
   const int64_t wave = 3 * kNumSMs, per = (static_cast<int64_t>(n_seq) * Hkv * tiles_used * max_kv_len + wave - 1) / wave;
   p.chunk = per <= 2048 ? (per < 128 ? 128 : per) : (per / 5 < 1024 ? 1024 : (per / 5 > 4096 ? 4096 : per / 5));
+  // Rows for more than eight waves need no splits (fp32, 8 KV heads of 128: 8192 x 4 rows 4702 us in two, 4382 whole).
+  if (static_cast<int64_t>(n_seq) * Hkv * tiles_used > 8 * wave) p.chunk = max_kv_len > 0 ? max_kv_len : 1;
   // Few rows over a short cache: the splits of a row tile are one cluster, whose CTAs join their sums through shared memory:
   // no second launch and no workspace (8 heads x 1000 tokens 12.0 -> 10.3 us, 8 x 4 heads of 64 x 1277 12.1 -> 10.9).  Not where
   // there are CTAs for more than two an SM: a cluster is held up by its longest split and by those that have nothing
@@ -686,8 +691,14 @@ Plan8 plan_prefill(int n_seq, int Hkv, int G, int q_len, bool ragged, int64_t to
   p.row_tiles = (p.most_rows + rows - 1) / rows;
   const int64_t ctas = (ragged ? (tokens * G + rows - 1) / rows : static_cast<int64_t>(n_seq) * p.row_tiles) * Hkv;
   int64_t splits = ctas > 0 ? kNumSMs / ctas : 1;
-  const int64_t most = max_kv_len / 512;
+  // What leaves SMs idle is split over its tokens, into parts of at least 512 (one sequence, 8 KV heads of 128, bf16: 32 x 4 rows
+  // over 4096 tokens 30 us, 81 whole, 30 at 256 tokens, 37 at 1024; 512 x 4 over 8192 107, 164 whole).  In a ragged batch of at least 2048, and two
+  // parts only from 8192 tokens on, because other sequences use those SMs too and the join is not free: 15 single tokens
+  // and a piece of 512 over 1024 tokens 50 us whole, 61 in parts of 512; 31 and 512 over 4096 118 whole, 137 in two; 15 and 256 over
+  // 4096 114 whole, 83 in parts of 2048; 3 and 512 over 8192 180 whole, 122 in two.
+  const int64_t most = max_kv_len / (ragged ? 2048 : 512);
   if (splits > most) splits = most;
+  if (ragged && splits == 2 && max_kv_len < 8192) splits = 1;
   if (splits > 32) splits = 32;
   if (splits < 1) splits = 1;
   p.chunk = (max_kv_len + splits - 1) / splits;

@@ -23,7 +23,7 @@
 // 4400 cycles: 2900 of softmax (two warps on a quarter of the SM, whose exponentials alone take 2048) and 1400 of tensor core
 // and hand-over.  512 columns of tensor memory are two row tiles of 128 scores and 128 sums.  At head_dim 64 they are
 // four of 64 and 64, which lets another row tile's softmax run meanwhile: 130 -> 100 us at 8 x 1024 tokens, 32 heads.
-// Measured (causal, bf16, e4m3): 2 x 4096 tokens, 32 heads of 128 over 8: 350 us, 785 TFLOP/s; 8 x 1024, 32 heads
+// Measured (causal, bf16, e4m3): 2 x 4096 tokens, 32 heads of 128 over 8: 344 us, 800 TFLOP/s; 8 x 1024, 32 heads
 // of 64 over 4: 100 us, 344 TFLOP/s counted over visible pairs.
 // Slower at head_dim 128: score tiles of 64 tokens in two buffers each; two threads a row (490 us); rows read twice from
 // tensor memory in place of held in registers (470); arithmetic on single numbers in place of pairs (386).
