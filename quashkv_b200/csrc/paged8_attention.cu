@@ -692,13 +692,13 @@ Plan8 plan_prefill(int n_seq, int Hkv, int G, int q_len, bool ragged, int64_t to
   const int64_t ctas = (ragged ? (tokens * G + rows - 1) / rows : static_cast<int64_t>(n_seq) * p.row_tiles) * Hkv;
   int64_t splits = ctas > 0 ? kNumSMs / ctas : 1;
   // What leaves SMs idle is split over its tokens, into parts of at least 512 (one sequence, 8 KV heads of 128, bf16: 32 x 4 rows
-  // over 4096 tokens 30 us, 81 whole, 30 at 256 tokens, 37 at 1024; 512 x 4 over 8192 107, 164 whole).  In a ragged batch of at least 2048, and two
-  // parts only from 8192 tokens on, because other sequences use those SMs too and the join is not free: 15 single tokens
+  // over 4096 tokens 30 us, 81 whole, 30 at 256 tokens, 37 at 1024; 512 x 4 over 8192 107, 164 whole).  In a ragged batch of at least 2048, and where the
+  // SMs are enough for no more than two, those only from 8192 tokens on, because other sequences use those SMs too and the join is not free: 15 single tokens
   // and a piece of 512 over 1024 tokens 50 us whole, 61 in parts of 512; 31 and 512 over 4096 118 whole, 137 in two; 15 and 256 over
   // 4096 114 whole, 83 in parts of 2048; 3 and 512 over 8192 180 whole, 122 in two.
+  if (ragged && splits == 2 && max_kv_len < 8192) splits = 1;
   const int64_t most = max_kv_len / (ragged ? 2048 : 512);
   if (splits > most) splits = most;
-  if (ragged && splits == 2 && max_kv_len < 8192) splits = 1;
   if (splits > 32) splits = 32;
   if (splits < 1) splits = 1;
   p.chunk = (max_kv_len + splits - 1) / splits;
