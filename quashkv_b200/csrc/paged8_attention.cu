@@ -77,10 +77,10 @@ template <int N> __device__ __forceinline__ void lds(uint32_t (&w)[N], const uns
 }
 
 // CTAs on an SM that the registers allow for.
-template <int D, int NG> constexpr int resident() { return D > 64 ? (NG == 1 ? 3 : 2) : (NG == 1 ? 4 : 3); }
+__host__ __device__ constexpr int resident(int d, int ng) { return d > 64 ? (ng == 1 ? 3 : 2) : (ng == 1 ? 4 : 3); }
 
 template <int D, int CODE, int KIND, int NG>
-__global__ void __launch_bounds__(kWarps * 32, resident<D, NG>()) paged8_split_kernel(Attn8Args a) {
+__global__ void __launch_bounds__(kWarps * 32, resident(D, NG)) paged8_split_kernel(Attn8Args a) {
   using P = Split<D, NG>;
   constexpr int QT = KIND == kF32 ? 2 : 1, WT = KIND == kBF16 ? 1 : 2;      // terms of queries and weights
   constexpr int kR = P::kRows, kKeyPitch = Pitch<D>::kKey, kValPitch = Pitch<D>::kVal;
@@ -662,11 +662,14 @@ Plan8 plan_split(int n_seq, int Hkv, int most_rows, int rows_used, int64_t max_k
   // Tokens of a split.  What fits one wave of resident CTAs is cut into one (each at least a step of its four warps); more
   // is cut five times finer than a wave, so that the last CTAs to run, and sequences of different lengths, leave little
   // of the chip idle.  Measured, 32 x 8 heads x 32768 tokens: 16384 tokens 440 us, 8192 384, 4096 367, 2048 376, 1024 404;
-  // 32 x 8 x up to 1278: 128 tokens 54 us (the whole step), 256 47, 512 and more 44; 8 heads x 1000: 64 tokens 11.6 us, 128 11.2, 512 13.7.
+  // 8 heads x 1000: 64 tokens 11.6 us, 128 11.2, 512 13.7; 32 x 8 x 1277 in one split (256 CTAs of 444) 24 us, in two (512) 31.
   const int64_t wave = 3 * kNumSMs, per = (static_cast<int64_t>(n_seq) * Hkv * tiles_used * max_kv_len + wave - 1) / wave;
-  p.chunk = per <= 2048 ? (per < 128 ? 128 : per) : (per / 5 < 1024 ? 1024 : (per / 5 > 4096 ? 4096 : per / 5));
+  const int64_t used = static_cast<int64_t>(n_seq) * Hkv * tiles_used, room = resident(d, p.ng) * kNumSMs;
+  const int64_t one = used > 0 && used <= room ? (max_kv_len + room / used - 1) / (room / used) : max_kv_len;      // tokens, with which it is one wave
+  p.chunk = per <= 2048 ? (one <= 2048 ? one : per) : (per / 5 < 1024 ? 1024 : (per / 5 > 4096 ? 4096 : per / 5));
+  if (p.chunk < 128) p.chunk = 128;
   // Rows for more than eight waves need no splits (fp32, 8 KV heads of 128: 8192 x 4 rows 4702 us in two, 4382 whole).
-  if (static_cast<int64_t>(n_seq) * Hkv * tiles_used > 8 * wave) p.chunk = max_kv_len > 0 ? max_kv_len : 1;
+  if (used > 8 * wave) p.chunk = max_kv_len > 0 ? max_kv_len : 1;
   // Few rows over a short cache: the splits of a row tile are one cluster, whose CTAs join their sums through shared memory:
   // no second launch and no workspace (8 heads x 1000 tokens 12.0 -> 10.3 us, 8 x 4 heads of 64 x 1277 12.1 -> 10.9).  Not where
   // there are CTAs for more than two an SM: a cluster is held up by its longest split and by those that have nothing
