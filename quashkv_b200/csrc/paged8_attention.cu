@@ -650,7 +650,7 @@ __global__ void __launch_bounds__(128) paged8_merge_kernel(Attn8Args a) {
 // piece of 1985 over 4096 tokens 340 us with CTAs for 32 rows, 352 for 64.
 constexpr int kFewRows = 64, kFewRagged = 32;
 
-struct Plan8 { int ng, row_tiles, most_rows, n_splits; bool cluster; int64_t chunk, part_rows; size_t ws; };
+struct Plan8 { int ng, tile_rows, row_tiles, most_rows, n_splits; bool cluster; int64_t chunk, part_rows; size_t ws; };
 
 // `rows_used`: rows that sequences mostly have.
 Plan8 plan_split(int n_seq, int Hkv, int most_rows, int rows_used, int64_t max_kv_len, int d, int dtype) {
@@ -690,9 +690,15 @@ Plan8 plan_split(int n_seq, int Hkv, int most_rows, int rows_used, int64_t max_k
 Plan8 plan_prefill(int n_seq, int Hkv, int G, int q_len, bool ragged, int64_t tokens, int64_t max_kv_len, int d) {
   Plan8 p{};
   p.most_rows = G * q_len;
-  const int rows = prefill8_rows(d);
-  p.row_tiles = (p.most_rows + rows - 1) / rows;
-  const int64_t ctas = (ragged ? (tokens * G + rows - 1) / rows : static_cast<int64_t>(n_seq) * p.row_tiles) * Hkv;
+  auto ctas_of = [&](int rows) { return (ragged ? (tokens * G + rows - 1) / rows : static_cast<int64_t>(n_seq) * ((p.most_rows + rows - 1) / rows)) * Hkv; };
+  p.tile_rows = prefill8_rows(d);
+  // Fewer rows in a CTA where SMs are idle and the cache is short (a long one is better split).  us, full CTAs / fewer rows: one sequence,
+  // 4 KV heads of 64, 8 query heads each: 1024 tokens 51 / 34, 512 30 / 22, 64 over 4096 39 / 30, 512 over 8192 94 / 158; 8 heads of
+  // 128, 4 query heads each: 512 tokens 24.7 / 23.6, 256 over 2048 37 / 39, 512 over 8192 106 / 154; ragged, 15 and 512 over 1024 51 / 57.
+  if (!ragged && max_kv_len <= (d == 64 ? 4096 : 1024))
+    while (p.tile_rows > 128 && ctas_of(p.tile_rows / 2) <= kNumSMs) p.tile_rows /= 2;
+  p.row_tiles = (p.most_rows + p.tile_rows - 1) / p.tile_rows;
+  const int64_t ctas = ctas_of(p.tile_rows);
   int64_t splits = ctas > 0 ? kNumSMs / ctas : 1;
   // What leaves SMs idle is split over its tokens, into parts of at least 512 (one sequence, 8 KV heads of 128, bf16: 32 x 4 rows
   // over 4096 tokens 30 us, 81 whole, 30 at 256 tokens, 37 at 1024; 512 x 4 over 8192 107, 164 whole).  In a ragged batch of at least 2048, and where the
@@ -854,7 +860,7 @@ extern "C" int qkv_attention_paged8(const void* q, int q_dtype, const int64_t* q
   };
   Attn8Args p = with(r.p, r.s.ws), b = with(r.s, 0);
   if (r.prefill) {
-    p.tile_rows = prefill8_rows(pages.d);
+    p.tile_rows = r.p.tile_rows;
     p.by_token = 1;
     p.few_rows = r.split ? kFewRagged : 0;
     if (static_cast<int64_t>(n_seq) * a.Hkv > 0x7fffffffLL || p.row_tiles > 65535) return QKV_EDIM;

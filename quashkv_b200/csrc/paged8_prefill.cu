@@ -262,12 +262,13 @@ __global__ void __launch_bounds__(Pf8<D>::kThreads, 1) paged8_prefill_kernel(Att
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
 
   const int order = gridDim.y - 1 - blockIdx.y, h = blockIdx.x % a.Hkv;      // long rows first
+  const int most = PACKED ? P::kRowsC : a.tile_rows;        // rows of a CTA
   const int seq = PACKED ? owner_of(a, order, P::kRowsC) : blockIdx.x / a.Hkv;
   const Span8 s = span8(a, seq);
   asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");
-  const int rows = a.G * s.q_len, r0 = (PACKED ? order - first_tile(a, seq, P::kRowsC) : order) * P::kRowsC;
+  const int rows = a.G * s.q_len, r0 = (PACKED ? order - first_tile(a, seq, P::kRowsC) : order) * most;
   if ((PACKED && r0 < 0) || r0 >= rows || rows <= a.few_rows) return;
-  const int r_end = min(r0 + P::kRowsC, rows), nt = (r_end - r0 + kRowsT - 1) / kRowsT;
+  const int r_end = min(r0 + most, rows), nt = (r_end - r0 + kRowsT - 1) / kRowsT;
   const int64_t seen = visible8(a, s, (r_end - 1) / a.G);
   const int64_t begin = static_cast<int64_t>(blockIdx.z) * a.chunk, stop = min(seen, begin + a.chunk);
   if (begin > 0 && begin >= seen) return;
