@@ -594,15 +594,26 @@ __global__ void __launch_bounds__(Pf8<D>::kThreads, 1) paged8_prefill_kernel(Att
         umma::fence_after_sync();
       }
       if (!ok) l = __int_as_float(0x7fc00000);             // (a wait that ran out: NaN)
-      // Rows leave through the place of the queries (every product that reads them has ended), so that D / 8 lanes write a row.
+      // Rows leave through the place of the queries, so that D / 8 lanes write a row.  At D = 128 a warp's place there holds
+      // rows of other warps' queries, too: only behind o_full, which every product that reads them and so every warp's
+      // queries are in front of.  Where nothing was summed, or a wait ran out, a thread writes its row by itself.
       const int64_t slot = part_row8(a, s, seq, h, live ? r : 0) * a.n_splits + blockIdx.z;
       const float by = l != 0.f ? ex2(M - m) / l : 0.f;    // a row that has seen nothing is zeros
       unsigned char* rows_s = q_s + t * P::kQBytes + 32 * (warp & 3) * (2 * D);
+      const bool summed = ok && n_sub > 0;                 // (the same for all of a warp)
+      if (!summed && a.n_splits == 1 && live) {
+        uint4* at = reinterpret_cast<uint4*>(static_cast<uint16_t*>(a.out) + row_at(a, s.o_row0, a.o_stride, h, r));
+        const uint32_t x = ok ? 0u : 0x7fff7fffu;          // (NaN in both types)
+#pragma unroll 1
+        for (int c = 0; c < D / 8; ++c) at[c] = make_uint4(x, x, x, x);
+      }
 #pragma unroll
       for (int c = 0; c < D; c += 32) {
         uint32_t o[32];
-        if (ok && n_sub > 0) {
+        if (summed) {
           umma::tmem_ld32(sums + c, o);
+        } else if (a.n_splits == 1) {
+          break;
         } else {
 #pragma unroll
           for (int e = 0; e < 32; ++e) o[e] = ok ? 0u : 0x7fc00000u;
@@ -625,7 +636,7 @@ __global__ void __launch_bounds__(Pf8<D>::kThreads, 1) paged8_prefill_kernel(Att
           *reinterpret_cast<uint4*>(rows_s + lane * (2 * D) + ((((c + e) >> 3) ^ (lane & 7)) << 4)) = make_uint4(y[0], y[1], y[2], y[3]);
         }
       }
-      if (a.n_splits == 1) {
+      if (summed && a.n_splits == 1) {
         constexpr int kLanes = D / 8, kRows = 32 / kLanes;
         const int64_t mine = row_at(a, s.o_row0, a.o_stride, h, live ? r : r0);
         __syncwarp();
