@@ -11,20 +11,20 @@
 //                   inner dimension contiguous, the second product reads V with the outer one contiguous, so nothing is
 //                   transposed
 // The tensor core works for one row tile while the softmax of the others runs.  Rows hold two whole-number reference
-// exponents as in the split kernel, which rise only when a score passes them by 14; only then is the accumulator
+// exponents as in the split kernel, which rise only when a score passes them by 4; only then is the accumulator
 // rescaled (exactly), by the row's own thread.
 //
 // Precision: codes are exact in fp16, 16-bit queries too (scaled by a power of two per row); weights are rounded to
-// fp16 once, 2^-12 on average of each, which is less than the rounding of the output (2^-9 or, fp16, as much), and the sum of weights is
-// fp32 of the unrounded ones.
+// fp16 once, 2^-11 of each at most: an eighth of what the output's own rounding takes with bf16 queries, and as much as that with fp16
+// ones, whose weights the split kernel holds as hi + lo (a second product here).  The sum of weights is fp32 of the unrounded ones.
 //
 // Bound by the chain of a row tile: its scores, its softmax, its weights times V, none of which can overlap another of
 // the same row tile, since scores and weights share their columns.  At head_dim 128 a round of 128 tokens takes about
 // 4400 cycles: 2900 of softmax (two warps on a quarter of the SM, whose exponentials alone take 2048) and 1400 of tensor core
 // and hand-over.  512 columns of tensor memory are two row tiles of 128 scores and 128 sums.  At head_dim 64 they are
 // four of 64 and 64, which lets another row tile's softmax run meanwhile: 130 -> 100 us at 8 x 1024 tokens, 32 heads.
-// Measured (causal, bf16, e4m3): 2 x 4096 tokens, 32 heads of 128 over 8: 344 us, 800 TFLOP/s; 8 x 1024, 32 heads
-// of 64 over 4: 100 us, 344 TFLOP/s counted over visible pairs.
+// Measured (causal, bf16, e4m3): 2 x 4096 tokens, 32 heads of 128 over 8: 362 us, 760 TFLOP/s; 8 x 1024, 32 heads
+// of 64 over 4: 101 us, 340 TFLOP/s counted over visible pairs.
 // Slower at head_dim 128: score tiles of 64 tokens in two buffers each; two threads a row (490 us); rows read twice from
 // tensor memory in place of held in registers (470); arithmetic on single numbers in place of pairs (386).
 //
@@ -40,7 +40,10 @@ namespace qkv {
 namespace {
 
 constexpr int kTok = 128, kRowsT = 128, kStages = 2, kMetaSlots = 4, kGroups = kTok / 16;
-constexpr float kNone = -1e30f, kSlack = 14.f, kLift = 0.f;      // weights reach 2^15 and the largest is at least 1/2
+// Weights reach 2^15 and the largest is at least 2^9, as in the split kernel: half of fp16's least step is 2^-34 of it, so the many small
+// weights of a long cache keep their sum.  (References that rise by 14 and a largest of 1/2 lose weights below 2^-25 of it: 2 x 4096 tokens
+// 349 us in place of 362, 8 x 1024 of 64 100 in place of 101, but weights of 2^-26 beside one came to nothing, however many.)
+constexpr float kNone = -1e30f, kSlack = 4.f, kLift = 10.f;
 __device__ unsigned int g_prefill8_timeouts = 0;
 
 struct TileMeta { float ks[kGroups], ex[kGroups], mant[kGroups]; uint32_t bad; uint32_t pad[7]; };   // per group of 16 tokens
