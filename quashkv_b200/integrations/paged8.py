@@ -186,29 +186,28 @@ class QuashKVPaged8Cache(PagePool):
     def append(self, seq_ids: Sequence, keys: torch.Tensor, values: torch.Tensor) -> None:
         """keys, values (n_seq, num_kv_heads, new_tokens, head_size): the next ``new_tokens`` positions of every listed
         sequence (new sequences start at position 0; the entries of an id that is listed more than once follow one
-        another, each in a call of its own, because they can share a page)."""
+        another, each in a call of its own, because they can share a page).  A call that raises, for want of pages or
+        otherwise, leaves lengths and pages as they were."""
         ops._need_cuda(keys, "QuashKVPaged8Cache.append")
         n, H, T, D = keys.shape
         if n != len(seq_ids) or H != self.num_kv_heads or D != self.head_size or values.shape != keys.shape:
             raise ValueError(f"Expected keys and values of shape ({len(seq_ids)}, {self.num_kv_heads}, T, {self.head_size})")
         if n == 0 or T == 0:
             return
-        starts, turns, seen = [], [], {}
+        turns, seen = [], {}
         for i, s in enumerate(seq_ids):
-            starts.append(self._lens.get(s, 0))
-            self._grow(s, T)
-            self._lens[s] = starts[-1] + T
             turn = seen[s] = seen.get(s, -1) + 1
             if turn == len(turns):
                 turns.append([])
             turns[turn].append(i)
-        table, _, _ = self.block_table(seq_ids)
-        starts = torch.tensor(starts, dtype=torch.int32, device=self.device)
-        if len(turns) == 1:
-            return self.append_with_tables(keys, values, table, starts)
-        for turn in turns:
-            at = torch.tensor(turn, device=self.device)
-            self.append_with_tables(keys[at], values[at], table[at], starts[at])
+        with self._storing(seq_ids, T) as starts:
+            table, _, _ = self.block_table(seq_ids)
+            starts = torch.tensor(starts, dtype=torch.int32, device=self.device)
+            if len(turns) == 1:
+                return self.append_with_tables(keys, values, table, starts)
+            for turn in turns:
+                at = torch.tensor(turn, device=self.device)
+                self.append_with_tables(keys[at], values[at], table[at], starts[at])
 
     def append_with_tables(self, keys: torch.Tensor, values: torch.Tensor, block_table: torch.Tensor,
                            start_lens: torch.Tensor) -> None:

@@ -20,6 +20,7 @@ Only CUDA tensors are accepted; there is no CPU implementation.
 
 from __future__ import annotations
 
+import contextlib
 import math
 from dataclasses import dataclass
 from typing import Optional, Sequence
@@ -179,14 +180,42 @@ class PagePool:
         for seq_id in list(self._blocks):
             self.free(seq_id)
 
-    def _grow(self, seq_id, new_tokens: int) -> None:
+    def _grow(self, seq_id, new_tokens: int) -> list:
+        """Pages for ``new_tokens`` more tokens of a sequence; returns those that it took."""
         blocks = self._blocks.setdefault(seq_id, [])
         need = -(-(self._lens.get(seq_id, 0) + new_tokens) // self.block_size) - len(blocks)
         if need > len(self._free):
             raise RuntimeError(f"KV page pool exhausted: sequence {seq_id!r} needs {need} more pages, "
                                f"{len(self._free)} free")
-        for _ in range(need):
-            blocks.append(self._free.pop())
+        taken = [self._free.pop() for _ in range(need)]
+        blocks.extend(taken)
+        return taken
+
+    @contextlib.contextmanager
+    def _storing(self, seq_ids: Sequence, new_tokens: int):
+        """Pages and lengths for ``new_tokens`` more tokens of every entry, around their store; gives the position that each
+        entry starts at (an id may be listed more than once: each entry starts where the one before it ended).  All or
+        nothing: where the pool is too small for all of them, or the store raises, the pool is as it was."""
+        before, taken, starts = {}, [], []
+        try:
+            for s in seq_ids:
+                before.setdefault(s, (len(self._blocks[s]) if s in self._blocks else None, self._lens.get(s)))
+                starts.append(self._lens.get(s, 0))
+                taken += self._grow(s, new_tokens)
+                self._lens[s] = starts[-1] + new_tokens
+            yield starts
+        except BaseException:
+            for s, (blocks, length) in before.items():
+                if blocks is None:
+                    self._blocks.pop(s, None)
+                else:
+                    del self._blocks[s][blocks:]
+                if length is None:
+                    self._lens.pop(s, None)
+                else:
+                    self._lens[s] = length
+            self._free.extend(reversed(taken))
+            raise
 
     def block_table(self, seq_ids: Sequence) -> tuple:
         """(block_table (n, max_blocks) int32, seq_lens (n) int32, max length) for a batch of sequences."""
@@ -236,7 +265,7 @@ class QuashKVPagedCache(PagePool):
     def append(self, seq_ids: Sequence, keys: torch.Tensor, values: torch.Tensor) -> None:
         """keys, values (n_seq, num_kv_heads, new_tokens, head_size): the next ``new_tokens`` positions of
         every listed sequence (new sequences start at position 0; the entries of an id that is listed more than
-        once follow one another)."""
+        once follow one another).  A call that raises, for want of pages or otherwise, leaves lengths and pages as they were."""
         ops._need_cuda(keys, "QuashKVPagedCache.append")
         n, H, T, D = keys.shape
         if n != len(seq_ids) or H != self.num_kv_heads or D != self.head_size or values.shape != keys.shape:
@@ -244,13 +273,9 @@ class QuashKVPagedCache(PagePool):
                              f"{self.head_size})")
         if n == 0 or T == 0:
             return
-        starts = []
-        for s in seq_ids:            # an id may be listed more than once: each entry starts where the one before it ended
-            starts.append(self._lens.get(s, 0))
-            self._grow(s, T)
-            self._lens[s] = starts[-1] + T
-        table, _, _ = self.block_table(seq_ids)
-        self._store(keys, values, table, torch.tensor(starts, dtype=torch.int32, device=self.device))
+        with self._storing(seq_ids, T) as starts:
+            table, _, _ = self.block_table(seq_ids)
+            self._store(keys, values, table, torch.tensor(starts, dtype=torch.int32, device=self.device))
 
     def append_with_tables(self, keys: torch.Tensor, values: torch.Tensor, block_table: torch.Tensor,
                            start_lens: torch.Tensor) -> None:
