@@ -401,7 +401,10 @@ int64_t qkv_dropped_paged8_tokens(void);
  *   seq_lens   tokens held, clamped to max_kv_len and to the table; a block number outside the pool hides
  *              its tokens; bytes behind the last token may be anything; codes within hold no NaN
  *   scale      any number;  scales of the pages: 0 or more, or NaN, which reaches what sees its page
- *   causal     query token t of n sits at position seq_lens[i] - n + t and sees positions up to its own
+ *   causal     query token t of n sits at position seq_lens[i] - n + t and sees positions up to its own: the queries are the
+ *              last n of the tokens held.  Where not all of them have found a place (qkv_extend_pages), they are not:
+ *              qkv_attention_paged8_from takes their positions, start_lens[i] + t, with start_lens the lengths before (NULL:
+ *              as above); a query whose own token found no place sees the tokens held
  * A row that sees nothing is zeros.
  * Workspace: qkv_attention_paged8_workspace_bytes(...) bytes, 16-byte aligned. */
 size_t qkv_attention_paged8_workspace_bytes(int n_seq, int Hq, int Hkv, int q_len, int ragged, int64_t total_q,
@@ -411,6 +414,11 @@ int qkv_attention_paged8(const void* q, int q_dtype, const int64_t* q_strides, q
                          const int32_t* query_starts, int64_t total_q, int n_seq, int Hq, int q_len, int64_t max_kv_len,
                          float scale, int causal, void* out, const int64_t* out_strides, void* workspace,
                          size_t workspace_bytes, void* stream);
+int qkv_attention_paged8_from(const void* q, int q_dtype, const int64_t* q_strides, qkv_pages8_t pages,
+                              const int32_t* block_table, int64_t table_stride, int max_blocks, const int32_t* seq_lens,
+                              const int32_t* query_starts, int64_t total_q, const int32_t* start_lens, int n_seq, int Hq,
+                              int q_len, int64_t max_kv_len, float scale, int causal, void* out, const int64_t* out_strides,
+                              void* workspace, size_t workspace_bytes, void* stream);
 
 /* ---- block tables and slots on the device ----------------------------------------------------------------
  * A pool's bookkeeping as device memory: a block table of max_blocks entries a sequence (table_stride apart),
@@ -419,7 +427,8 @@ int qkv_attention_paged8(const void* q, int q_dtype, const int64_t* q_strides, q
  * qkv_extend_pages takes new_lens[i] more tokens for every sequence: blocks come off the top of the stack in
  * the order of the sequences and are entered in the table behind the ceil(seq_lens[i] / block_size) that a
  * sequence has; slots[t] (of max_tokens) is block * block_size + offset of new token t, the sequences' tokens one
- * after the other, -1 behind them and for tokens that found no place (stack empty, row of the table full);
+ * after the other, -1 behind them and for tokens that found no place (stack empty, row of the table full; the first of a
+ * sequence's tokens are those that found one);
  * query_starts (n_seq + 1) are the exclusive sums of new_lens, none above max_tokens; seq_lens_out and pool_out
  * may be seq_lens and pool; start_lens_out gets the lengths before (NULL if not wanted, unless in place).
  * qkv_shrink_pages keeps the first min(keep_lens[i], seq_lens[i]) tokens and puts the blocks behind them back; after an

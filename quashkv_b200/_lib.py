@@ -93,6 +93,8 @@ SIGNATURES = {
     "qkv_attention_paged8_workspace_bytes": (_sz, [_i, _i, _i, _i, _i, _i64, _i64, _i, _i]),
     "qkv_attention_paged8": (_i, [_vp, _i, C.POINTER(_i64), Pages8, _vp, _i64, _i, _vp, _vp, _i64, _i, _i, _i, _i64, _f, _i,
                                   _vp, C.POINTER(_i64), _vp, _sz, _vp]),
+    "qkv_attention_paged8_from": (_i, [_vp, _i, C.POINTER(_i64), Pages8, _vp, _i64, _i, _vp, _vp, _i64, _vp, _i, _i, _i, _i64, _f, _i,
+                                       _vp, C.POINTER(_i64), _vp, _sz, _vp]),
     "qkv_extend_pages": (_i, [_vp, _i64, _i, _vp, _vp, _vp, _i64, _vp, _i, _i, _i64, _vp, _vp, _vp, _vp, _vp, _vp]),
     "qkv_shrink_pages": (_i, [_vp, _i64, _i, _vp, _vp, _vp, _i64, _vp, _i, _i, _vp]),
     "qkv_index_workspace_bytes": (_sz, [_i64, _i, _i, _i]),

@@ -29,7 +29,7 @@ using OptTensor = std::optional<Tensor>;
   X(qkv_strerror) X(qkv_compress_mse) X(qkv_compress_ip) X(qkv_compress_mixed) X(qkv_mixed_row_bytes)             \
   X(qkv_decompress) X(qkv_decompress_mixed) X(qkv_attention_workspace_bytes) X(qkv_attention)                     \
   X(qkv_attention_paged) X(qkv_attention_tiled) X(qkv_append_workspace_bytes) X(qkv_append_kv) X(qkv_index_workspace_bytes) X(qkv_index_scan_topk) \
-  X(qkv_append_paged8) X(qkv_attention_paged8_workspace_bytes) X(qkv_attention_paged8) X(qkv_extend_pages) X(qkv_shrink_pages)
+  X(qkv_append_paged8) X(qkv_attention_paged8_workspace_bytes) X(qkv_attention_paged8_from) X(qkv_extend_pages) X(qkv_shrink_pages)
 
 struct Api {
 #define QKV_MEMBER(name) decltype(&::name) name = nullptr;
@@ -489,13 +489,14 @@ void append_paged8(const Tensor& keys_in, const Tensor& values_in, Tensor k_code
                               nullptr, ip(table), table.stride(0), static_cast<int>(table.size(1)), ip(starts), call.stream), "append_paged8");
 }
 
-// queries (n_seq, Hq, q_len, d), or (tokens, Hq, d) with query_starts (n_seq + 1); the result has their shape and type.
+// queries (n_seq, Hq, q_len, d), or (tokens, Hq, d) with query_starts (n_seq + 1); the result has their shape and type.  first: the
+// position of each sequence's first query token.
 Tensor attention_paged8(const Tensor& q_in, const Tensor& k_codes, const Tensor& v_codes, const Tensor& k_scales, const Tensor& v_scales,
                         const Tensor& table_in, const Tensor& lens_in, int64_t max_kv_len, const OptTensor& starts_in, int64_t max_q_len,
-                        double scale, bool causal) {
+                        double scale, bool causal, const OptTensor& first_in) {
   const at::Device dev = q_in.device();
   Call call(dev);
-  same_device(dev, {&k_codes, &v_codes, &k_scales, &v_scales, &table_in, &lens_in, starts_in ? &*starts_in : nullptr});
+  same_device(dev, {&k_codes, &v_codes, &k_scales, &v_scales, &table_in, &lens_in, starts_in ? &*starts_in : nullptr, first_in ? &*first_in : nullptr});
   const qkv_pages8_t pages = pages8(k_codes, v_codes, k_scales, v_scales);
   check_table(table_in, lens_in);
   const bool ragged = starts_in.has_value();
@@ -504,9 +505,13 @@ Tensor attention_paged8(const Tensor& q_in, const Tensor& k_codes, const Tensor&
                     "quashkv_b200: queries ", q_in.sizes(), " do not match ", n, " sequences and ", pages.Hkv, " KV heads of size ", pages.d);
   TORCH_CHECK_VALUE(max_kv_len >= 0 && max_q_len >= 0, "quashkv_b200: negative lengths");
   const Tensor table = table_rows(table_in), lens = lens_in.contiguous(), starts = ragged ? starts_in->contiguous() : Tensor();
+  const Tensor first = first_in ? first_in->contiguous() : Tensor();
   if (ragged)
     TORCH_CHECK_VALUE(starts.scalar_type() == at::kInt && starts.dim() == 1 && starts.size(0) == n + 1,
                       "quashkv_b200: int32 query_starts of ", n + 1, " entries, got ", starts.sizes());
+  if (first_in)
+    TORCH_CHECK_VALUE(first.scalar_type() == at::kInt && first.dim() == 1 && first.size(0) == n,
+                      "quashkv_b200: int32 start_lens of ", n, " entries, got ", first.sizes());
   const Tensor q = rows16(dtype_code(q_in) < 0 ? q_in.to(at::kFloat) : q_in);
   Tensor out = empty(q.sizes(), q.scalar_type(), dev);
   if (q.numel() == 0) return out;
@@ -523,10 +528,10 @@ Tensor attention_paged8(const Tensor& q_in, const Tensor& k_codes, const Tensor&
   TORCH_CHECK_VALUE(hq * std::max<int64_t>(q_len, 1) <= INT32_MAX && n <= INT32_MAX && max_kv_len < INT32_MAX - 64, "quashkv_b200: sizes beyond 32 bits");
   const int64_t need = api.qkv_attention_paged8_workspace_bytes(n, hq, pages.Hkv, q_len, ragged, ragged ? q.size(0) : 0, max_kv_len, pages.d, dtype_code(q));
   const Tensor ws = need > 0 ? empty({need}, at::kByte, dev) : Tensor();
-  check(api.qkv_attention_paged8(q.const_data_ptr(), dtype_code(q), qs, pages, ip(table), table.stride(0), static_cast<int>(table.size(1)),
-                                 ip(lens), ragged ? ip(starts) : nullptr, ragged ? q.size(0) : 0, static_cast<int>(n), static_cast<int>(hq),
-                                 static_cast<int>(q_len), max_kv_len, static_cast<float>(scale), causal, out.data_ptr(), os,
-                                 need > 0 ? ws.data_ptr() : nullptr, need, call.stream), "attention_paged8");
+  check(api.qkv_attention_paged8_from(q.const_data_ptr(), dtype_code(q), qs, pages, ip(table), table.stride(0), static_cast<int>(table.size(1)),
+                                      ip(lens), ragged ? ip(starts) : nullptr, ragged ? q.size(0) : 0, first_in ? ip(first) : nullptr,
+                                      static_cast<int>(n), static_cast<int>(hq), static_cast<int>(q_len), max_kv_len, static_cast<float>(scale),
+                                      causal, out.data_ptr(), os, need > 0 ? ws.data_ptr() : nullptr, need, call.stream), "attention_paged8");
   return out;
 }
 

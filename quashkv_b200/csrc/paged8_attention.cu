@@ -811,6 +811,15 @@ extern "C" int qkv_attention_paged8(const void* q, int q_dtype, const int64_t* q
                                     const int32_t* query_starts, int64_t total_q, int n_seq, int Hq, int q_len, int64_t max_kv_len,
                                     float scale, int causal, void* out, const int64_t* out_strides, void* workspace,
                                     size_t workspace_bytes, void* stream) {
+  return qkv_attention_paged8_from(q, q_dtype, q_strides, pages, block_table, table_stride, max_blocks, seq_lens, query_starts, total_q, nullptr,
+                                   n_seq, Hq, q_len, max_kv_len, scale, causal, out, out_strides, workspace, workspace_bytes, stream);
+}
+
+extern "C" int qkv_attention_paged8_from(const void* q, int q_dtype, const int64_t* q_strides, qkv_pages8_t pages,
+                                         const int32_t* block_table, int64_t table_stride, int max_blocks, const int32_t* seq_lens,
+                                         const int32_t* query_starts, int64_t total_q, const int32_t* start_lens, int n_seq, int Hq,
+                                         int q_len, int64_t max_kv_len, float scale, int causal, void* out, const int64_t* out_strides,
+                                         void* workspace, size_t workspace_bytes, void* stream) {
   if (!q || !q_strides || !block_table || !seq_lens || !out || !out_strides) return QKV_ENULL;
   if (q_dtype != QKV_F32 && q_dtype != QKV_BF16 && q_dtype != QKV_F16) return QKV_EDTYPE;
   if (const int rc = check_pages8(pages)) return rc;
@@ -833,6 +842,7 @@ extern "C" int qkv_attention_paged8(const void* q, int q_dtype, const int64_t* q
   a.seq_lens = seq_lens;
   a.starts = query_starts;
   a.total_q = total_q;
+  a.first = start_lens;
   a.n_seq = n_seq;
   a.Hkv = pages.Hkv;
   a.G = Hq / pages.Hkv;

@@ -14,6 +14,7 @@ struct Attn8Args {
   const int32_t* table; int64_t table_stride; int bs_shift;      // log2 of block_size, -1 where it has none
   const int32_t* seq_lens;
   const int32_t* starts; int64_t total_q;   // ragged queries: rows starts[i] .. starts[i + 1] of total_q are sequence i's
+  const int32_t* first;                     // position of a sequence's first query token; nullptr: its queries are its last positions
   int n_seq, Hkv, G, q_len, causal;         // q_len: of every sequence, or the most of any
   int64_t max_kv_len;                       // within the tables
   float scale;
@@ -32,7 +33,7 @@ int launch_prefill8(const Attn8Args& a, cudaStream_t st);
 unsigned int prefill8_timeouts();
 
 // Tokens and queries of a sequence, within what the host has promised.
-struct Span8 { int64_t len, tok0; int q_len, q_all; int64_t q_row0, o_row0; };      // tok0: query tokens in front of it
+struct Span8 { int64_t len, tok0, pos0; int q_len, q_all; int64_t q_row0, o_row0; };      // tok0: query tokens in front of it; pos0: position of its first
 
 __device__ __forceinline__ Span8 span8(const Attn8Args& a, int seq) {
   Span8 s;
@@ -51,13 +52,14 @@ __device__ __forceinline__ Span8 span8(const Attn8Args& a, int seq) {
     s.q_row0 = seq * a.q_stride[0];
     s.o_row0 = seq * a.o_stride[0];
   }
+  s.pos0 = a.first ? max(a.first[seq], 0) : s.len - s.q_all;
   return s;
 }
 
 // How many tokens the queries at token `tok` of the sequence's block see.
 __device__ __forceinline__ int64_t visible8(const Attn8Args& a, const Span8& s, int tok) {
   if (!a.causal) return s.len;
-  const int64_t v = s.len - s.q_all + tok + 1;
+  const int64_t v = s.pos0 + tok + 1;
   return v < 0 ? 0 : (v > s.len ? s.len : v);
 }
 

@@ -12,7 +12,7 @@ The functions are the same operators over tensors that the caller owns:
     plan = extend_pages(block_table, seq_lens, new_lens, free_pages, pool, block_size, max_tokens)
     append_paged8(keys, values, k_codes, v_codes, k_scales, v_scales, plan.slots)
     out = attention_paged8(queries, k_codes, v_codes, k_scales, v_scales, block_table, plan.seq_lens, max_kv_len,
-                           causal=True, query_starts=plan.query_starts, max_q_len=max_q_len)
+                           causal=True, query_starts=plan.query_starts, max_q_len=max_q_len, start_lens=seq_lens)
 
 The reference stops before real pages (quashkv/integrations/vllm_backend.py:82-195).  Only CUDA tensors are accepted;
 there is no CPU implementation, and nothing here has a derivative.
@@ -54,7 +54,8 @@ def extend_pages(block_table: torch.Tensor, seq_lens: torch.Tensor, new_lens: to
     ``free_pages`` is a stack of which the first ``pool[0]`` are free, taken from the top in the order of the sequences.
     All int32.  ``max_tokens`` (known on the host) is at least the sum of ``new_lens``: the new tokens of all sequences one
     after the other, as a model computes them.  Tokens for which the stack or the row of the table is too short get slot
-    -1, are not counted in ``seq_lens``, and are added to ``pool[1]``.  Lengths and counts are returned and not changed, so
+    -1, are not counted in ``seq_lens``, and are added to ``pool[1]``; they are the last ones of their sequence, and causal
+    attention of the others needs ``start_lens`` then (see ``attention_paged8``).  Lengths and counts are returned and not changed, so
     that a plan can be dropped; ``PageTables.extend`` changes them in place."""
     ops._need_cuda(block_table, "extend_pages")
     return PagePlan(*ops.extend_pages(block_table, seq_lens, new_lens, free_pages, pool, block_size, max_tokens))
@@ -88,14 +89,17 @@ def dropped_tokens() -> int:
 def attention_paged8(queries: torch.Tensor, k_codes: torch.Tensor, v_codes: torch.Tensor, k_scales: torch.Tensor,
                      v_scales: torch.Tensor, block_table: torch.Tensor, seq_lens: torch.Tensor, max_kv_len: int,
                      scale: Optional[float] = None, causal: bool = False, query_starts: Optional[torch.Tensor] = None,
-                     max_q_len: Optional[int] = None) -> torch.Tensor:
+                     max_q_len: Optional[int] = None, start_lens: Optional[torch.Tensor] = None) -> torch.Tensor:
     """softmax(scale * q k^T) v over pages of 8-bit codes; the result has the queries' shape and type.
 
     ``queries``: (n_seq, q_heads, q_len, head_size), or with ``query_starts`` (n_seq + 1) int32 a ragged batch (tokens,
     q_heads, head_size) whose tokens query_starts[i] .. query_starts[i + 1] - 1 are sequence i's, at most ``max_q_len``
     of them (default: as many as there are).  Query head h reads KV head h // (q_heads // kv_heads).  ``seq_lens`` (n_seq)
-    int32 with ``max_kv_len`` an upper bound of them known on the host; with ``causal`` the queries of a sequence are its
-    last positions.  Rows that see nothing, and rows of no sequence, are zeros.
+    int32 with ``max_kv_len`` an upper bound of them known on the host.  With ``causal`` a query sees the positions up to its
+    own: the queries of a sequence are its last positions, or, with ``start_lens`` (n_seq) int32 (the lengths before the
+    step), query t is at start_lens + t.  The two are the same where every new token has found a place; where some have not,
+    only the second is right, and a query whose own token has none sees the tokens that the sequence holds.  Rows that see
+    nothing, and rows of no sequence, are zeros.
 
     Scales are 0 or more, or NaN, which reaches what sees the page; codes must not hold NaN within a sequence's length, and may be anything behind it.  A
     block number outside the pool hides its tokens."""
@@ -107,7 +111,7 @@ def attention_paged8(queries: torch.Tensor, k_codes: torch.Tensor, v_codes: torc
     elif max_q_len is None:
         max_q_len = queries.shape[0]
     return ops.attention_paged8(queries, k_codes, v_codes, k_scales, v_scales, block_table, seq_lens, int(max_kv_len),
-                                query_starts, int(max_q_len), float(scale), bool(causal))
+                                query_starts, int(max_q_len), float(scale), bool(causal), start_lens)
 
 
 class PageTables:
@@ -131,7 +135,9 @@ class PageTables:
         self.pool = torch.tensor([num_blocks, 0], **i32)
 
     def extend(self, new_lens: torch.Tensor, max_tokens: int) -> StepPlan:
-        """Pages for ``new_lens`` (max_seqs) int32 more tokens, 0 for rows that get none (see ``extend_pages``)."""
+        """Pages for ``new_lens`` (max_seqs) int32 more tokens, 0 for rows that get none (see ``extend_pages``).  Give the plan's
+        ``start_lens`` to causal attention, so that it is right for a row that did not get all of its tokens, too (``QuashKVPagedCache`` takes
+        none: there the queries of such a row are not at their positions)."""
         ops._need_cuda(new_lens, "PageTables.extend")
         return StepPlan(*ops.extend_pages_(self.block_table, self.seq_lens, new_lens, self.free_pages, self.pool,
                                            self.block_size, int(max_tokens)))
@@ -222,10 +228,11 @@ class QuashKVPaged8Cache(PagePool):
 
     def attention_with_tables(self, queries: torch.Tensor, block_table: torch.Tensor, seq_lens: torch.Tensor, max_kv_len: int,
                               scale: Optional[float] = None, causal: bool = False,
-                              query_starts: Optional[torch.Tensor] = None, max_q_len: Optional[int] = None) -> torch.Tensor:
+                              query_starts: Optional[torch.Tensor] = None, max_q_len: Optional[int] = None,
+                              start_lens: Optional[torch.Tensor] = None) -> torch.Tensor:
         """Attention of every sequence over its own pages (see ``attention_paged8``)."""
         return attention_paged8(queries, *self.planes, block_table, seq_lens, max_kv_len, scale=scale, causal=causal,
-                                query_starts=query_starts, max_q_len=max_q_len)
+                                query_starts=query_starts, max_q_len=max_q_len, start_lens=start_lens)
 
     def attention(self, seq_ids: Sequence, queries: torch.Tensor, scale: Optional[float] = None,
                   causal: bool = False) -> torch.Tensor:

@@ -121,7 +121,7 @@ for _schema in (
         "append_paged8(Tensor keys, Tensor values, Tensor(a!) k_codes, Tensor(b!) v_codes, Tensor(c!) k_scales, Tensor(d!) v_scales, "
         "Tensor? slots, Tensor? block_table, Tensor? start_lens) -> ()",
         "attention_paged8(Tensor q, Tensor k_codes, Tensor v_codes, Tensor k_scales, Tensor v_scales, Tensor block_table, "
-        "Tensor seq_lens, SymInt max_kv_len, Tensor? query_starts, SymInt max_q_len, float scale, bool causal) -> Tensor",
+        "Tensor seq_lens, SymInt max_kv_len, Tensor? query_starts, SymInt max_q_len, float scale, bool causal, Tensor? start_lens=None) -> Tensor",
         "extend_pages(Tensor(a!) block_table, Tensor seq_lens, Tensor new_lens, Tensor free_pages, Tensor pool, SymInt block_size, "
         "SymInt max_tokens) -> (Tensor, Tensor, Tensor, Tensor)",
         "extend_pages_(Tensor(a!) block_table, Tensor(b!) seq_lens, Tensor new_lens, Tensor free_pages, Tensor(c!) pool, "
@@ -417,7 +417,7 @@ def _(scores, ids, k):
 
 
 @torch.library.register_fake("quashkv_b200::attention_paged8")
-def _(q, k_codes, v_codes, k_scales, v_scales, block_table, seq_lens, max_kv_len, query_starts, max_q_len, scale, causal):
+def _(q, k_codes, v_codes, k_scales, v_scales, block_table, seq_lens, max_kv_len, query_starts, max_q_len, scale, causal, start_lens=None):
     return q.new_empty(q.shape, dtype=q.dtype if q.dtype in _DT else torch.float32)
 
 
