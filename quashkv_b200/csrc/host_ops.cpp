@@ -547,14 +547,6 @@ void check_pool(const Tensor& table, const Tensor& lens, const Tensor& other, co
                     "quashkv_b200: int32 lengths for ", lens.size(0), " sequences, int32 free pages, and pool (2) int32");
 }
 
-// A contiguous tensor on a part of another one's storage: a plan's small results come from one allocation.
-Tensor part_of(const Tensor& base, int64_t byte, at::IntArrayRef size, at::ScalarType type) {
-  Tensor t = at::detail::make_tensor<c10::TensorImpl>(c10::Storage(base.storage()), base.key_set(), c10::scalarTypeToTypeMeta(type));
-  t.unsafeGetTensorImpl()->set_storage_offset(byte / static_cast<int64_t>(c10::elementSize(type)));
-  t.unsafeGetTensorImpl()->set_sizes_contiguous(size);
-  return t;
-}
-
 // lens_out / pool_out: the tensors that get the new lengths and counts (those of the call: in place).
 void run_extend(const Tensor& table, const Tensor& lens, const Tensor& new_in, const Tensor& free_pages, const Tensor& pool, int64_t block_size,
                 const Tensor& slots, const Tensor& starts, const Tensor& lens_out, const Tensor* start_out, const Tensor& pool_out, void* stream) {
@@ -574,10 +566,9 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> extend_pages(Tensor table, const Tens
   check_pool(table, lens, new_lens, free_pages, pool);
   TORCH_CHECK_VALUE(max_tokens >= 0, "quashkv_b200: negative max_tokens");
   const int64_t n = lens.size(0);
-  const int64_t words = 2 * max_tokens;                    // of 32 bits; every part starts on eight bytes
-  const Tensor all = empty({8 * max_tokens + 4 * (2 * n + 8)}, at::kByte, dev);
-  Tensor slots = part_of(all, 0, {max_tokens}, at::kLong), starts = part_of(all, 4 * words, {n + 1}, at::kInt);
-  Tensor after = part_of(all, 4 * (words + (n + 2) / 2 * 2), {n}, at::kInt), count = part_of(all, 4 * (words + (n + 2) / 2 * 2 + (n + 1) / 2 * 2), {2}, at::kInt);
+  // (a storage each, as the schema says: who keeps the lengths does not keep the slots)
+  const Tensor slots = empty({max_tokens}, at::kLong, dev), starts = empty({n + 1}, at::kInt, dev);
+  const Tensor after = empty({n}, at::kInt, dev), count = empty({2}, at::kInt, dev);
   run_extend(table, lens, new_lens, free_pages, pool, block_size, slots, starts, after, nullptr, count, call.stream);
   return {slots, starts, after, count};
 }
@@ -589,10 +580,7 @@ std::tuple<Tensor, Tensor, Tensor> extend_pages_(Tensor table, Tensor lens, cons
   check_pool(table, lens, new_lens, free_pages, pool);
   TORCH_CHECK_VALUE(max_tokens >= 0, "quashkv_b200: negative max_tokens");
   const int64_t n = lens.size(0);
-  const int64_t words = 2 * max_tokens;
-  const Tensor all = empty({8 * max_tokens + 4 * (2 * n + 4)}, at::kByte, dev);
-  Tensor slots = part_of(all, 0, {max_tokens}, at::kLong), starts = part_of(all, 4 * words, {n + 1}, at::kInt);
-  Tensor before = part_of(all, 4 * (words + (n + 2) / 2 * 2), {n}, at::kInt);
+  const Tensor slots = empty({max_tokens}, at::kLong, dev), starts = empty({n + 1}, at::kInt, dev), before = empty({n}, at::kInt, dev);
   run_extend(table, lens, new_lens, free_pages, pool, block_size, slots, starts, lens, &before, pool, call.stream);
   return {slots, starts, before};
 }
