@@ -10,6 +10,7 @@ import torch
 
 import paged8_reference as ref
 from quashkv_b200 import _lib
+from quashkv_b200.integrations import paged8
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda"
@@ -34,7 +35,7 @@ def attend_into(out, q, pages, table, lens, max_kv_len, starts=None, max_q_len=N
     p.code = int(k.dtype == INT8)
     n, d, dtype = table.shape[0], q.shape[-1], {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}[q.dtype]
     ragged = starts is not None
-    total, q_len = (q.shape[0], q.shape[0] if max_q_len is None else max_q_len) if ragged else (0, q.shape[2])
+    total, q_len = (q.shape[0], q.shape[0] if max_q_len is None else min(max_q_len, q.shape[0])) if ragged else (0, q.shape[2])      # as the op does
     strides = lambda t: (I64 * 3)(0, t.stride(0), t.stride(1)) if ragged else (I64 * 3)(t.stride(0), t.stride(2), t.stride(1))      # noqa: E731
     need = L.qkv_attention_paged8_workspace_bytes(n, q.shape[1], p.Hkv, q_len, int(ragged), total, max_kv_len, d, dtype)
     ws = torch.full((max(need, 16),), 0xff, dtype=torch.uint8, device=DEV)
@@ -78,3 +79,49 @@ def test_prompts_that_see_nothing_are_zeros(d, H, G, x_dtype):
     every = torch.full((n, q_len, H * G, d), math.nan, dtype=x_dtype, device=DEV)      # a bound of no tokens at all
     attend_into(every.transpose(1, 2), q, pages, table, _i32(lens), 0, causal=False)
     assert not every.view(torch.int16).any()
+
+
+RAGGED = [([1] * 30 + [9, 500, 1, 0, 65, 64, 63, 0, 1], 0, 700), ([300] + [1] * 70, 3, 1), ([1] * 40 + [128] * 3, 5, 0), ([40] * 33, 0, 2000),
+          ([1] * 9, 2, 40), ([0, 0, 3, 0], 7, 9), ([0, 0], 0, 33), ([200], 1, 1)]
+
+
+@pytest.mark.parametrize("x_dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("d,H,G", [(128, 2, 4), (64, 3, 5), (128, 1, 40), (96, 2, 2), (32, 1, 1)])
+def test_rows_of_no_sequence_are_cleared(d, H, G, x_dtype):
+    """Rows in front of the first sequence, behind the last one, and beyond the most that a sequence is allowed; sequences
+    without a token; partial sums in a workspace that held NaN.  Everything else is what the public call gives."""
+    g = torch.Generator(device=DEV).manual_seed(G)
+    for new, front, behind in RAGGED:
+        for long in (0, 5000):                               # short caches, and one that is split
+            lens = [0 if i % 11 == 7 else n + (37 * i) % 900 + (long if i == 0 else 0) for i, n in enumerate(new)]
+            total = sum(-(-m // 16) for m in lens) + 1
+            pages = ref.random_pages(g, total, H, 16, d, INT8, "nhd")
+            table = ref.random_tables(lens, 16, total, 5).to(DEV)
+            starts = front + np.r_[0, np.cumsum(new)]
+            q = torch.randn(starts[-1] + behind, H * G, d, generator=g, device=DEV).to(x_dtype)
+            for most in (q.shape[0], 60):
+                out = torch.full_like(q, math.nan)
+                attend_into(out, q, pages, table, _i32(lens), max(max(lens), 1), starts=_i32(starts), max_q_len=most)
+                none = torch.ones(q.shape[0], dtype=torch.bool, device=DEV)
+                for i, n in enumerate(new):
+                    see = torch.arange(min(n, most), device=DEV) + lens[i] - n + 1 > 0
+                    none[starts[i]:starts[i] + min(n, most)] = ~see
+                bits = out.view(torch.int16 if x_dtype == torch.bfloat16 else torch.int32)
+                assert not bits[none].any() and out.isfinite().all() and out[~none].any(-1).all()
+                assert torch.equal(out, paged8.attention_paged8(q, *pages, table, _i32(lens), max(max(lens), 1), causal=True,
+                                                                query_starts=_i32(starts), max_q_len=most))
+
+
+@pytest.mark.parametrize("x_dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("d,H,G,q_len", [(128, 2, 4, 1), (64, 2, 8, 1), (96, 1, 3, 5), (32, 4, 1, 2), (128, 1, 4, 90)])
+def test_every_row_of_a_dense_batch_is_written(d, H, G, q_len, x_dtype):
+    g = torch.Generator(device=DEV).manual_seed(q_len)
+    for lens in ([0], [0, 0, 1], [1000, 0, 17, 3], [0] * 40 + [6000]):
+        total = sum(-(-m // 16) for m in lens) + 1
+        pages = ref.random_pages(g, total, H, 16, d, E4M3)
+        table = ref.random_tables(lens, 16, total, 2).to(DEV)
+        q = torch.randn(len(lens), H * G, q_len, d, generator=g, device=DEV).to(x_dtype)
+        out = attend_into(torch.full_like(q, math.nan), q, pages, table, _i32(lens), max(max(lens), 1))
+        see = torch.tensor([[m - q_len + t + 1 > 0 for t in range(q_len)] for m in lens], device=DEV)[:, None].expand(-1, H * G, -1)
+        assert out.isfinite().all() and not out[~see].view(torch.int16).any() and out[see].any(-1).all()
+        assert torch.equal(out, paged8.attention_paged8(q, *pages, table, _i32(lens), max(max(lens), 1), causal=True))
