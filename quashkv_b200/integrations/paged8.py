@@ -90,7 +90,8 @@ def attention_paged8(queries: torch.Tensor, k_codes: torch.Tensor, v_codes: torc
                      v_scales: torch.Tensor, block_table: torch.Tensor, seq_lens: torch.Tensor, max_kv_len: int,
                      scale: Optional[float] = None, causal: bool = False, query_starts: Optional[torch.Tensor] = None,
                      max_q_len: Optional[int] = None, start_lens: Optional[torch.Tensor] = None) -> torch.Tensor:
-    """softmax(scale * q k^T) v over pages of 8-bit codes; the result has the queries' shape and type.
+    """softmax(scale * q k^T) v over pages of 8-bit codes; the result has the queries' shape and their type: fp32, bf16 or
+    fp16.  Queries of any other type, fp64 among them, are taken as fp32 and give fp32.
 
     ``queries``: (n_seq, q_heads, q_len, head_size), or with ``query_starts`` (n_seq + 1) int32 a ragged batch (tokens,
     q_heads, head_size) whose tokens query_starts[i] .. query_starts[i + 1] - 1 are sequence i's, at most ``max_q_len``
@@ -167,7 +168,7 @@ class QuashKVPaged8Cache(PagePool):
     ``codes`` is "e4m3" or "int8"; ``layout`` "hnd" keeps a page's tokens of one head together, "nhd" a token's heads.
     ``k_codes`` / ``v_codes`` are (num_blocks, num_kv_heads, block_size, head_size) in both, ``k_scales`` / ``v_scales``
     (num_blocks, num_kv_heads); coordinate = code * scale.  ``block_size`` is a multiple of 16, ``head_size`` 32, 64, 96
-    or 128.  Attention returns the queries' type."""
+    or 128.  Attention returns the queries' type (see ``attention_paged8``)."""
 
     def __init__(self, num_blocks: int, num_kv_heads: int, head_size: int, block_size: int = 16, codes: str = "e4m3",
                  layout: str = "hnd", device="cuda"):

@@ -125,3 +125,14 @@ def test_every_row_of_a_dense_batch_is_written(d, H, G, q_len, x_dtype):
         see = torch.tensor([[m - q_len + t + 1 > 0 for t in range(q_len)] for m in lens], device=DEV)[:, None].expand(-1, H * G, -1)
         assert out.isfinite().all() and not out[~see].view(torch.int16).any() and out[see].any(-1).all()
         assert torch.equal(out, paged8.attention_paged8(q, *pages, table, _i32(lens), max(max(lens), 1), causal=True))
+
+
+def test_queries_of_other_types_are_taken_as_fp32():
+    g = torch.Generator(device=DEV).manual_seed(0)
+    pages = ref.random_pages(g, 8, 2, 16, 64, INT8)
+    table, lens = ref.random_tables([64, 50], 16, 8, 1).to(DEV), _i32([64, 50])
+    q = torch.randint(-3, 4, (2, 4, 3, 64), generator=g, device=DEV)
+    want = paged8.attention_paged8(q.float(), *pages, table, lens, 64, causal=True)
+    for x in (q, q.double()):
+        got = paged8.attention_paged8(x, *pages, table, lens, 64, causal=True)
+        assert got.dtype == torch.float32 and torch.equal(got, want)

@@ -194,3 +194,16 @@ def test_reference_shrink_undoes_extend():
         back, free2, count2 = ref.shrink(t2, after, lens, free, count, bs)
         assert back == list(lens) and free2 == free and count2[0] == pool[0]
         assert math.isclose(count[1], int(new.sum()) - (sum(after) - int(lens.sum())))
+
+
+def test_types_of_the_result():
+    """fp32, bf16 and fp16 queries give their type, all others fp32, and tracing says the same."""
+    from torch._subclasses.fake_tensor import FakeTensorMode
+    _lib.load_host()
+    with FakeTensorMode(allow_non_fake_inputs=True):
+        make = lambda *s, dt=torch.float32: torch.empty(*s, dtype=dt, device="cuda")      # noqa: E731
+        pages = (make(4, 2, 16, 64, dt=torch.int8), make(4, 2, 16, 64, dt=torch.int8), make(4, 2), make(4, 2))
+        table, lens = make(2, 4, dt=torch.int32), make(2, dt=torch.int32)
+        for dt in (torch.float32, torch.bfloat16, torch.float16, torch.float64, torch.int32):
+            out = paged8.attention_paged8(make(2, 4, 1, 64, dt=dt), *pages, table, lens, 64)
+            assert out.shape == (2, 4, 1, 64) and out.dtype == (dt if dt in (torch.bfloat16, torch.float16) else torch.float32)
