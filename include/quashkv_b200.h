@@ -400,7 +400,8 @@ int64_t qkv_dropped_paged8_tokens(void);
  *              are zeros
  *   seq_lens   tokens held, clamped to max_kv_len and to the table; a block number outside the pool hides
  *              its tokens; bytes behind the last token may be anything; codes within hold no NaN
- *   scale      any number;  scales of the pages: 0 or more, or NaN, which reaches what sees its page
+ *   scale      any number;  scales of the pages: 0 or more, or NaN, which reaches what sees its page; value scales below
+ *              2^-126 count as 0
  *   causal     query token t of n sits at position seq_lens[i] - n + t and sees positions up to its own: the queries are the
  *              last n of the tokens held.  Where not all of them have found a place (qkv_extend_pages), they are not:
  *              qkv_attention_paged8_from takes their positions, start_lens[i] + t, with start_lens the lengths before (NULL:

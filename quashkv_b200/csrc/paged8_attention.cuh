@@ -129,12 +129,20 @@ __device__ __forceinline__ void load_row8(const void* q, int dtype, int64_t at, 
   }
 }
 
+// From sums in units of 2^M to total weight l in units of 2^m: times x, then times y.  Two factors, because 2^(M - m) alone is below the normal
+// numbers (and lost) where value scales are near 2^-126, though the results are not.  0 for a row that has seen nothing.
+struct Unit8 { float x, y; };
+__device__ __forceinline__ Unit8 unit8(float m, float M, float l) {
+  if (l == 0.f) return {0.f, 0.f};
+  const float half = floorf(0.5f * (M - m));
+  return {ex2(half), ex2(M - m - half) / l};
+}
+
 // Coordinates c .. c + 3 of output row r of KV head h: sums o in units of 2^M, total weight l in units of 2^m.  A row that has seen
 // nothing is zeros.  One rounding, to the queries' type.
 __device__ __forceinline__ void store_out8(const Attn8Args& a, const Span8& s, int h, int r, int c, float4 o, float m, float M, float l) {
-  float f = 0.f;
-  if (l != 0.f) f = ex2(M - m) / l;                        // M is far below m where every value was zero
-  o.x *= f; o.y *= f; o.z *= f; o.w *= f;
+  const Unit8 f = unit8(m, M, l);                          // (M is far below m where every value was zero)
+  o.x = o.x * f.x * f.y; o.y = o.y * f.x * f.y; o.z = o.z * f.x * f.y; o.w = o.w * f.x * f.y;
   const int64_t at = s.o_row0 + static_cast<int64_t>(r / a.G) * a.o_stride[1] + static_cast<int64_t>(h * a.G + r % a.G) * a.o_stride[2] + c;
   if (a.dtype == QKV_F32) {
     *reinterpret_cast<float4*>(static_cast<float*>(a.out) + at) = o;

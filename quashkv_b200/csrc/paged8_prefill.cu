@@ -601,7 +601,7 @@ __global__ void __launch_bounds__(Pf8<D>::kThreads, 1) paged8_prefill_kernel(Att
       // rows of other warps' queries, too: only behind o_full, which every product that reads them and so every warp's
       // queries are in front of.  Where nothing was summed, or a wait ran out, a thread writes its row by itself.
       const int64_t slot = part_row8(a, s, seq, h, live ? r : 0) * a.n_splits + blockIdx.z;
-      const float by = l != 0.f ? ex2(M - m) / l : 0.f;    // a row that has seen nothing is zeros
+      const Unit8 by = unit8(m, M, l);                     // a row that has seen nothing is zeros
       unsigned char* rows_s = q_s + t * P::kQBytes + 32 * (warp & 3) * (2 * D);
       const bool summed = ok && n_sub > 0;                 // (the same for all of a warp)
       if (!summed && a.n_splits == 1 && live) {
@@ -632,7 +632,7 @@ __global__ void __launch_bounds__(Pf8<D>::kThreads, 1) paged8_prefill_kernel(Att
           uint32_t y[4];
 #pragma unroll
           for (int k = 0; k < 4; ++k) {
-            const float v0 = __uint_as_float(o[e + 2 * k]) * by, v1 = __uint_as_float(o[e + 2 * k + 1]) * by;
+            const float v0 = __uint_as_float(o[e + 2 * k]) * by.x * by.y, v1 = __uint_as_float(o[e + 2 * k + 1]) * by.x * by.y;
             const __nv_bfloat162 z = __floats2bfloat162_rn(v0, v1);
             y[k] = a.dtype == QKV_BF16 ? *reinterpret_cast<const uint32_t*>(&z) : pack_half2(v0, v1);
           }

@@ -102,8 +102,9 @@ def attention_paged8(queries: torch.Tensor, k_codes: torch.Tensor, v_codes: torc
     only the second is right, and a query whose own token has none sees the tokens that the sequence holds.  Rows that see
     nothing, and rows of no sequence, are zeros.
 
-    Scales are 0 or more, or NaN, which reaches what sees the page; codes must not hold NaN within a sequence's length, and may be anything behind it.  A
-    block number outside the pool hides its tokens."""
+    Scales are 0 or more, or NaN, which reaches what sees the page; a value scale below 2^-126 counts as 0 (appends make none below
+    2^-120).  Codes must not hold NaN within a sequence's length, and may be anything behind it.  A block number outside the pool
+    hides its tokens."""
     ops._need_cuda(queries, "attention_paged8")
     if scale is None:
         scale = 1.0 / math.sqrt(queries.shape[-1])

@@ -136,3 +136,16 @@ def test_queries_of_other_types_are_taken_as_fp32():
     for x in (q, q.double()):
         got = paged8.attention_paged8(x, *pages, table, lens, 64, causal=True)
         assert got.dtype == torch.float32 and torch.equal(got, want)
+
+
+@pytest.mark.parametrize("x_dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("q_len", [1, 90])
+def test_the_least_value_scales(q_len, x_dtype):
+    """2^-126 is a scale like any other; subnormal ones count as 0."""
+    g = torch.Generator(device=DEV).manual_seed(1)
+    k, v, ks, vs = ref.random_pages(g, 8, 2, 16, 128, INT8)
+    table, lens = ref.random_tables([100], 16, 8, 1).to(DEV), _i32([100])
+    q = torch.randn(1, 8, q_len, 128, generator=g, device=DEV).to(x_dtype)
+    call = lambda s: paged8.attention_paged8(q, k, v, ks, torch.full_like(vs, s), table, lens, 100, causal=True)      # noqa: E731
+    assert torch.allclose(call(2.0 ** -126).double() * 2.0 ** 126, call(1.0).double(), rtol=0.02, atol=2.0 ** -7)
+    assert not call(2.0 ** -127).any() and not call(2.0 ** -149).any()
