@@ -67,3 +67,17 @@ def test_an_append_whose_store_is_refused_changes_nothing(which, stores):
     assert pool.seq_len("a") == 3 * T and pool.seq_len("b") == T and pool.free_blocks == 0
     pool.clear()
     assert pool.free_blocks == 6 and pool.seq_len("a") == 0
+
+
+@pytest.mark.parametrize("layout", ["hnd", "nhd"])
+@pytest.mark.parametrize("codes", ["e4m3", "int8"])
+def test_decompress_of_a_sequence_without_tokens(codes, layout):
+    pool = paged8.QuashKVPaged8Cache(6, 2, 32, codes=codes, layout=layout, device="cpu")
+    for x in pool.decompress("nobody"):
+        assert x.shape == (2, 0, 32) and x.dtype == torch.float32
+    pool._grow("a", T)
+    pool._lens["a"] = T
+    pool.k_scales.fill_(2.0)
+    pool.k_codes.view(torch.uint8).fill_(0x38 if codes == "e4m3" else 1)      # 1
+    k, v = pool.decompress("a")
+    assert k.shape == v.shape == (2, T, 32) and (k == 2).all() and not v.any()
