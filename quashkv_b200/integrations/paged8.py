@@ -252,5 +252,5 @@ class QuashKVPaged8Cache(PagePool):
 
         def rows(codes, scales):
             x = codes.view(torch.uint8)[pages].view(CODES[self.codes]).float() * scales[pages][..., None, None]
-            return x.transpose(0, 1).reshape(self.num_kv_heads, len(pages) * bs, self.head_size)[:, :n]
+            return x.transpose(0, 1).reshape(self.num_kv_heads, -1, self.head_size)[:, :n]
         return rows(self.k_codes, self.k_scales), rows(self.v_codes, self.v_scales)
