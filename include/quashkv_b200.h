@@ -407,7 +407,9 @@ int64_t qkv_dropped_paged8_tokens(void);
  *              qkv_attention_paged8_from takes their positions, start_lens[i] + t, with start_lens the lengths before (NULL:
  *              as above); a query whose own token found no place sees the tokens held
  * A row that sees nothing is zeros.
- * Workspace: qkv_attention_paged8_workspace_bytes(...) bytes, 16-byte aligned. */
+ * Workspace: qkv_attention_paged8_workspace_bytes(...) bytes, 16-byte aligned.  It follows the bounds, not the lengths: a
+ * ragged call of more than 32 rows (q_len times Hq / Hkv) has room for 32 rows of every sequence and KV head in each split (32 / 8
+ * heads of 128, bound 131072: 296 MB for 64 sequences, 1107 MB for 256). */
 size_t qkv_attention_paged8_workspace_bytes(int n_seq, int Hq, int Hkv, int q_len, int ragged, int64_t total_q,
                                             int64_t max_kv_len, int d, int q_dtype);
 int qkv_attention_paged8(const void* q, int q_dtype, const int64_t* q_strides, qkv_pages8_t pages,

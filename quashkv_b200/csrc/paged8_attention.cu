@@ -19,9 +19,9 @@
 // which is rare after the first granules.
 //
 // Bound by the bytes of the pages: (2 D + 8 / block_size) a token and KV head.  Measured, 32 x 8 KV heads x 32768 tokens of 128, four
-// bf16 queries a head: 370-395 us by the box, 5.4-5.8 TB/s; the schedulers' issue slots are 48 % busy, their three warps mostly wait for results of their own.
+// bf16 queries a head: 365-396 us by the box, 5.4-5.9 TB/s; the schedulers' issue slots are 48 % busy, their three warps mostly wait for results of their own.
 // fp32 queries take four MMAs in place of one, and 16 rows fill the registers (two CTAs an SM): 32 sequences of up to 16384
-// tokens, 16 rows a head: 236 us, 2.6 TB/s, bound by the latency of a warp's own chain.
+// tokens, 16 rows a head: 241 us, 2.6 TB/s, bound by the latency of a warp's own chain.
 #include <math.h>
 
 #include <cooperative_groups.h>
@@ -41,7 +41,7 @@ constexpr float kNone = -1e30f;          // reference exponent before anything h
 enum { kBF16 = 0, kF16 = 1, kF32 = 2 };
 constexpr int kMostCluster = 8;          // CTAs of a cluster (the portable size)
 constexpr float kSlack = 4.f;
-constexpr float kLift = 10.f;            // the largest weight is near 2^kLift: fp16 then has 2^-35 of it as its least step
+constexpr float kLift = 10.f;            // the largest weight is at least 2^(kLift - 1): fp16's least step is 2^-33 of it at most, half of it 2^-34
 
 // Bytes from one token's row to the next in the ring: without bank conflicts for both operands' reads.
 template <int D> struct Pitch { static constexpr int kKey = D == 128 || D == 96 ? D + 16 : D, kVal = D + 16; };
@@ -653,7 +653,7 @@ constexpr int kFewRows = 64, kFewRagged = 32;
 struct Plan8 { int ng, tile_rows, row_tiles, most_rows, n_splits; bool cluster; int64_t chunk, part_rows; size_t ws; };
 
 // `rows_used`: rows that sequences mostly have.
-Plan8 plan_split(int n_seq, int Hkv, int most_rows, int rows_used, int64_t max_kv_len, int d, int dtype) {
+Plan8 plan_split(int n_seq, int Hkv, int most_rows, int rows_used, int64_t max_kv_len, int d) {
   Plan8 p{};
   p.most_rows = most_rows;
   p.ng = rows_used > 8 ? 2 : 1;                            // groups of eight rows in a CTA (16 fp32 rows a head: 236 us in one, 288 in two)
@@ -671,7 +671,9 @@ Plan8 plan_split(int n_seq, int Hkv, int most_rows, int rows_used, int64_t max_k
   // Rows for more than eight waves need no splits (fp32, 8 KV heads of 128: 8192 x 4 rows 4702 us in two, 4382 whole).
   if (used > 8 * wave) p.chunk = max_kv_len > 0 ? max_kv_len : 1;
   // Few rows over a short cache: the splits of a row tile are one cluster, whose CTAs join their sums through shared memory:
-  // no second launch and no workspace (8 heads x 1000 tokens 12.0 -> 10.3 us, 8 x 4 heads of 64 x 1277 12.1 -> 10.9).  Not where
+  // no second launch and no workspace (8 heads x 1000 tokens 12.0 -> 10.3 us, 8 x 4 heads of 64 x 1277 12.1 -> 10.9).  Above 2048
+  // tokens the one launch speaks for it, not the time (in a graph, 8 heads of 128, joined in a cluster / by a second launch: 2000
+  // tokens 10.3 / 10.3 us, 3000 12.3 / 11.5, 4096 12.3 / 12.3; two sequences of 4096 14.4 / 12.3; 4 heads of 64, 4096 12.0 / 10.3).  Not where
   // there are CTAs for more than two an SM: a cluster is held up by its longest split and by those that have nothing
   // (32 x 8 x up to 1278 in two splits 39 -> 48 us for the whole step).
   const int64_t items = static_cast<int64_t>(n_seq) * Hkv * p.row_tiles;
@@ -704,7 +706,9 @@ Plan8 plan_prefill(int n_seq, int Hkv, int G, int q_len, bool ragged, int64_t to
   // over 4096 tokens 30 us, 81 whole, 30 at 256 tokens, 37 at 1024; 512 x 4 over 8192 107, 164 whole).  In a ragged batch of at least 2048, and where the
   // SMs are enough for no more than two, those only from 8192 tokens on, because other sequences use those SMs too and the join is not free: 15 single tokens
   // and a piece of 512 over 1024 tokens 50 us whole, 61 in parts of 512; 31 and 512 over 4096 118 whole, 137 in two; 15 and 256 over
-  // 4096 114 whole, 83 in parts of 2048; 3 and 512 over 8192 180 whole, 122 in two.
+  // 4096 114 whole, 83 in parts of 2048; 3 and 512 over 8192 180 whole, 122 in two.  Where a batch has one request, or a few, those
+  // SMs are idle and this is too cautious (one piece, ragged / the same rows dense: 8 heads of 128, 200 x 4 rows over 3500 98 / 43 us,
+  // 512 x 4 over 8000 166 / 105; 4 heads of 64, 64 x 8 over 3500 122 / 29): such a batch is better given as a dense call.
   if (ragged && splits == 2 && max_kv_len < 8192) splits = 1;
   const int64_t most = max_kv_len / (ragged ? 2048 : 512);
   if (splits > most) splits = most;
@@ -728,7 +732,7 @@ Route8 route8(int n_seq, int Hkv, int G, int q_len, bool ragged, int64_t tokens,
   const int few = ragged ? kFewRagged : kFewRows;
   r.prefill = rows > few && dtype != QKV_F32 && (d == 64 || d == 128);
   r.split = !r.prefill || ragged;                          // (it clears the rows of no sequence, too)
-  if (r.split) r.s = plan_split(n_seq, Hkv, r.prefill ? few : rows, r.prefill ? G : rows, r.prefill && G > few ? 0 : max_kv_len, d, dtype);
+  if (r.split) r.s = plan_split(n_seq, Hkv, r.prefill ? few : rows, r.prefill ? G : rows, r.prefill && G > few ? 0 : max_kv_len, d);
   if (r.prefill) r.p = plan_prefill(n_seq, Hkv, G, q_len, ragged, tokens, max_kv_len, d);
   r.ws = r.s.ws + r.p.ws;                                  // they overlap: each has a place of its own
   return r;
