@@ -16,7 +16,8 @@
 // exponents a row, so that rescaling is exact: m for the scores t, M for t + log2 of the page's value scale.  The weights
 // of the second product, 2^(t - M) vs, are then at most 2^15 and the largest at least 2^9 whatever the scales are: a page
 // of large values that a row hardly weighs takes no bits from the others.  References rise when a score is 4 above them,
-// which is rare after the first granules.
+// which is rare after the first granules.  M is held as dM = M - m, which stays exact where scores are so large (from 2^24 on)
+// that m + 1 is no number any more; there the largest score has all the weight, as it should.
 //
 // Bound by the bytes of the pages: (2 D + 8 / block_size) a token and KV head.  Measured, 32 x 8 KV heads x 32768 tokens of 128, four
 // bf16 queries a head: 365-396 us by the box, 5.4-5.9 TB/s; the schedulers' issue slots are 48 % busy, their three warps mostly wait for results of their own.
@@ -36,7 +37,7 @@ namespace {
 
 constexpr int kWarps = 4;
 constexpr int kStages = 2;               // steps of 32 tokens in a warp's ring: one in work, one on its way
-constexpr float kNone = -1e30f;          // reference exponent before anything has been seen
+constexpr float kNone = -3e38f;          // reference exponent before anything has been seen, and below every score's
 // What queries and weights are held as: fp16 once each (bf16), queries once and weights as hi + lo (fp16), both as hi + lo (fp32).
 enum { kBF16 = 0, kF16 = 1, kF32 = 2 };
 constexpr int kMostCluster = 8;          // CTAs of a cluster (the portable size)
@@ -154,7 +155,7 @@ __global__ void __launch_bounds__(kWarps * 32, resident(D, NG)) paged8_split_ker
   const int all_see = static_cast<int>(max(min(visible8(a, s, r0 / a.G) - begin, a.chunk), static_cast<int64_t>(0))) - 1;
 
   float acc[NG][2 * kVW][4];                               // [m tile]: coordinates 2j, 2j + 1 of the lane's, rows 2t, 2t + 1
-  float m[NG][2], M[NG][2], l[NG][2];
+  float m[NG][2], dM[NG][2], l[NG][2];
 #pragma unroll
   for (int n = 0; n < NG; ++n) {
 #pragma unroll
@@ -162,7 +163,7 @@ __global__ void __launch_bounds__(kWarps * 32, resident(D, NG)) paged8_split_ker
 #pragma unroll
       for (int e = 0; e < 4; ++e) acc[n][j][e] = 0.f;
 #pragma unroll
-    for (int e = 0; e < 2; ++e) { m[n][e] = kNone; M[n][e] = 0.5f * kNone; l[n][e] = 0.f; }
+    for (int e = 0; e < 2; ++e) { m[n][e] = kNone; dM[n][e] = -0.5f * kNone; l[n][e] = 0.f; }
   }
 
   // ---- granules: this warp has the pairs warp, warp + 4, ... of the chunk ----
@@ -303,32 +304,33 @@ __global__ void __launch_bounds__(kWarps * 32, resident(D, NG)) paged8_split_ker
       nan_page |= vexp == 255;
     }
     bool rise = false;
-    float top[NG][2], topM[NG][2];                         // of this lane's tokens
+    float top[2][NG][2];                                   // of this lane's tokens
 #pragma unroll
     for (int n = 0; n < NG; ++n)
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
-        const float t0 = fmaxf(sc[0][n][e], sc[0][n][e + 2]), t1 = fmaxf(sc[1][n][e], sc[1][n][e + 2]);
-        top[n][e] = fmaxf(t0, t1);
-        topM[n][e] = fmaxf(t0 + ex[0], t1 + ex[1]);
-        rise |= top[n][e] > m[n][e] + kSlack || topM[n][e] > M[n][e] + (kLift + kSlack);
+#pragma unroll
+        for (int u = 0; u < 2; ++u) top[u][n][e] = fmaxf(sc[u][n][e], sc[u][n][e + 2]);
+        const float t0 = top[0][n][e] - m[n][e], t1 = top[1][n][e] - m[n][e];
+        rise |= fmaxf(t0, t1) > kSlack || fmaxf(t0 + ex[0], t1 + ex[1]) > dM[n][e] + (kLift + kSlack);
       }
     if (__any_sync(QKV_FULL_MASK, rise)) {
 #pragma unroll
       for (int n = 0; n < NG; ++n)
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          float x = top[n][e], y = topM[n][e];
+          float x = top[0][n][e], y = top[1][n][e];
 #pragma unroll
           for (int o = 4; o < 32; o <<= 1) {
             x = fmaxf(x, __shfl_xor_sync(QKV_FULL_MASK, x, o));
             y = fmaxf(y, __shfl_xor_sync(QKV_FULL_MASK, y, o));
           }
-          const float m1 = fmaxf(m[n][e], ceilf(x)), M1 = fmaxf(M[n][e], ceilf(y) - kLift);
+          const float m1 = fmaxf(m[n][e], ceilf(fmaxf(x, y)));
+          const float was = dM[n][e] + (m[n][e] - m1), dM1 = fmaxf(was, ceilf(fmaxf(x - m1 + ex[0], y - m1 + ex[1])) - kLift);
           l[n][e] *= ex2(m[n][e] - m1);
-          const float f = ex2(M[n][e] - M1);
+          const float f = ex2(was - dM1);
           m[n][e] = m1;
-          M[n][e] = M1;
+          dM[n][e] = dM1;
 #pragma unroll
           for (int j = 0; j < 2 * kVW; ++j) {
             acc[n][j][e] *= f;
@@ -344,8 +346,9 @@ __global__ void __launch_bounds__(kWarps * 32, resident(D, NG)) paged8_split_ker
         float w[4];
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          l[n][e & 1] += ex2(sc[u][n][e] - m[n][e & 1]);
-          w[e] = ex2(sc[u][n][e] - (M[n][e & 1] - ex[u])) * mant[u];
+          const float x = sc[u][n][e] - m[n][e & 1];
+          l[n][e & 1] += ex2(x);
+          w[e] = ex2(x + (ex[u] - dM[n][e & 1])) * mant[u];
         }
         if (!whole && nan_page) {                          // a page of NaN: nothing from tokens that are not seen
 #pragma unroll
@@ -429,7 +432,7 @@ __global__ void __launch_bounds__(kWarps * 32, resident(D, NG)) paged8_split_ker
 
   // ---- the four warps' sums ----
   __syncthreads();                                         // the ring has been read
-  float* sums = reinterpret_cast<float*>(smem);            // [warp][row][kAccPitch], then [warp][row][4]: m, M, l
+  float* sums = reinterpret_cast<float*>(smem);            // [warp][row][kAccPitch], then [warp][row][4]: m, dM, l
   float* ref = sums + kWarps * kR * P::kAccPitch;
 #pragma unroll
   for (int n = 0; n < NG; ++n)
@@ -440,7 +443,7 @@ __global__ void __launch_bounds__(kWarps * 32, resident(D, NG)) paged8_split_ker
       x += __shfl_xor_sync(QKV_FULL_MASK, x, 8);
       x += __shfl_xor_sync(QKV_FULL_MASK, x, 16);
       const int r = 8 * n + 2 * t + e;
-      if (g == 0) *reinterpret_cast<float4*>(ref + (warp * kR + r) * 4) = make_float4(m[n][e], M[n][e], x, 0.f);
+      if (g == 0) *reinterpret_cast<float4*>(ref + (warp * kR + r) * 4) = make_float4(m[n][e], dM[n][e], x, 0.f);
 #pragma unroll
       for (int j = 0; j < 2 * kVW; ++j)
         *reinterpret_cast<float2*>(sums + (warp * kR + r) * P::kAccPitch + g * (D / 8) + 2 * j) = make_float2(acc[n][j][e], acc[n][j][e + 2]);
@@ -449,33 +452,39 @@ __global__ void __launch_bounds__(kWarps * 32, resident(D, NG)) paged8_split_ker
   const int n_rows = r_end - r0;
   for (int x = threadIdx.x; x < n_rows * (D / 4); x += kWarps * 32) {
     const int r = x / (D / 4), c = 4 * (x % (D / 4));
-    float mt = kNone, Mt = 0.5f * kNone;
+    float4 q[kWarps];
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) q[w] = *reinterpret_cast<const float4*>(ref + (w * kR + r) * 4);
+    float mt = kNone;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) mt = max_or_nan(mt, q[w].x);
+    float dMt = -0.5f * kNone + (kNone - mt);              // (as of a warp that has seen nothing)
 #pragma unroll
     for (int w = 0; w < kWarps; ++w) {
-      mt = max_or_nan(mt, ref[(w * kR + r) * 4]);
-      Mt = max_or_nan(Mt, ref[(w * kR + r) * 4 + 1]);
+      q[w].x -= mt;
+      q[w].y += q[w].x;
+      dMt = max_or_nan(dMt, q[w].y);
     }
     float lt = 0.f;
     float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
     for (int w = 0; w < kWarps; ++w) {
-      const float4 q = *reinterpret_cast<const float4*>(ref + (w * kR + r) * 4);
       const float4 y = *reinterpret_cast<const float4*>(sums + (w * kR + r) * P::kAccPitch + c);
-      lt = fmaf(q.z, ex2(q.x - mt), lt);
-      const float f = ex2(q.y - Mt);
+      lt = fmaf(q[w].z, ex2(q[w].x), lt);
+      const float f = ex2(q[w].y - dMt);
       o.x = fmaf(y.x, f, o.x); o.y = fmaf(y.y, f, o.y); o.z = fmaf(y.z, f, o.z); o.w = fmaf(y.w, f, o.w);
     }
     const int rr = r0 + r;
     if (a.n_splits == 1) {
-      store_out8(a, s, h, rr, c, o, mt, Mt, lt);
+      store_out8(a, s, h, rr, c, o, dMt, lt);
     } else if (a.in_cluster) {
       float* own = reinterpret_cast<float*>(smem + P::kOwn);
       *reinterpret_cast<float4*>(own + r * D + c) = o;
-      if (c == 0) *reinterpret_cast<float4*>(own + kR * D + r * 4) = make_float4(mt, Mt, lt, 0.f);
+      if (c == 0) *reinterpret_cast<float4*>(own + kR * D + r * 4) = make_float4(mt, dMt, lt, 0.f);
     } else {
       const int64_t slot = part_row8(a, s, seq, h, rr) * a.n_splits + blockIdx.y;
       *reinterpret_cast<float4*>(a.part + slot * D + c) = o;
-      if (c == 0) *reinterpret_cast<float4*>(a.ref + slot * 4) = make_float4(mt, Mt, lt, 0.f);
+      if (c == 0) *reinterpret_cast<float4*>(a.ref + slot * 4) = make_float4(mt, dMt, lt, 0.f);
     }
   }
   if (a.in_cluster) {                                      // the splits of these rows are one cluster: joined through shared memory
@@ -490,24 +499,27 @@ __global__ void __launch_bounds__(kWarps * 32, resident(D, NG)) paged8_split_ker
 #pragma unroll
       for (int p = 0; p < kMostCluster; ++p) {
         const float* theirs = cluster.map_shared_rank(own, p < parts ? p : 0);
-        q[p] = p < parts ? *reinterpret_cast<const float4*>(theirs + kR * D + r * 4) : make_float4(kNone, 0.5f * kNone, 0.f, 0.f);
+        q[p] = p < parts ? *reinterpret_cast<const float4*>(theirs + kR * D + r * 4) : make_float4(kNone, -0.5f * kNone, 0.f, 0.f);
         y[p] = *reinterpret_cast<const float4*>(theirs + r * D + c);
       }
-      float mt = kNone, Mt = 0.5f * kNone, lt = 0.f;
+      float mt = kNone, lt = 0.f;
+#pragma unroll
+      for (int p = 0; p < kMostCluster; ++p) mt = max_or_nan(mt, q[p].x);
+      float dMt = -0.5f * kNone + (kNone - mt);
 #pragma unroll
       for (int p = 0; p < kMostCluster; ++p) {
-        mt = max_or_nan(mt, q[p].x);
-        Mt = max_or_nan(Mt, q[p].y);
+        q[p].y += q[p].x - mt;
+        dMt = max_or_nan(dMt, q[p].y);
       }
       float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
       for (int p = 0; p < kMostCluster; ++p) {
         if (p >= parts) continue;
         lt = fmaf(q[p].z, ex2(q[p].x - mt), lt);
-        const float f = ex2(q[p].y - Mt);
+        const float f = ex2(q[p].y - dMt);
         o.x = fmaf(y[p].x, f, o.x); o.y = fmaf(y[p].y, f, o.y); o.z = fmaf(y[p].z, f, o.z); o.w = fmaf(y[p].w, f, o.w);
       }
-      store_out8(a, s, h, r0 + r, c, o, mt, Mt, lt);
+      store_out8(a, s, h, r0 + r, c, o, dMt, lt);
     }
     cluster.sync();                                        // nobody leaves while others read
   }
@@ -563,7 +575,7 @@ __global__ void __launch_bounds__(128) paged8_merge_kernel(Attn8Args a) {
   // (rows of a token are of one tile or of neighbours, whose last tokens differ: the parts are counted for each)
   const int in_head = rr % a.G, first = rr - in_head;      // head h * G + in_head of the token, then the next ones (of the next KV heads, too)
   float4 q[R][kU];
-  float mt[R], Mt[R], lt[R];
+  float mt[R], dMt[R], lt[R];
   int parts[R], most = 0;
 #pragma unroll
   for (int r = 0; r < R; ++r) {
@@ -576,7 +588,7 @@ __global__ void __launch_bounds__(128) paged8_merge_kernel(Attn8Args a) {
   for (int r = 0; r < R; ++r)
 #pragma unroll
     for (int u = 0; u < kU; ++u)
-      q[r][u] = lane + 32 * u < parts[r] ? *reinterpret_cast<const float4*>(a.ref + ((row0 + r) * a.n_splits + lane + 32 * u) * 4) : make_float4(kNone, 0.5f * kNone, 0.f, 0.f);
+      q[r][u] = lane + 32 * u < parts[r] ? *reinterpret_cast<const float4*>(a.ref + ((row0 + r) * a.n_splits + lane + 32 * u) * 4) : make_float4(kNone, -0.5f * kNone, 0.f, 0.f);
   float4 y[R][kP];
   auto fetch = [&](int p0) {
 #pragma unroll
@@ -592,28 +604,32 @@ __global__ void __launch_bounds__(128) paged8_merge_kernel(Attn8Args a) {
 #pragma unroll
   for (int r = 0; r < R; ++r) {
     mt[r] = q[r][0].x;
-    Mt[r] = q[r][0].y;
-    if (kU > 1) {
-      mt[r] = max_or_nan(mt[r], q[r][kU - 1].x);
-      Mt[r] = max_or_nan(Mt[r], q[r][kU - 1].y);
-    }
+    if (kU > 1) mt[r] = max_or_nan(mt[r], q[r][kU - 1].x);
   }
 #pragma unroll 1
   for (int x = width >> 1; x > 0; x >>= 1)
 #pragma unroll
-    for (int r = 0; r < R; ++r) {
-      mt[r] = max_or_nan(mt[r], __shfl_xor_sync(QKV_FULL_MASK, mt[r], x));
-      Mt[r] = max_or_nan(Mt[r], __shfl_xor_sync(QKV_FULL_MASK, Mt[r], x));
-    }
+    for (int r = 0; r < R; ++r) mt[r] = max_or_nan(mt[r], __shfl_xor_sync(QKV_FULL_MASK, mt[r], x));
 #pragma unroll
   for (int r = 0; r < R; ++r) {
     mt[r] = __shfl_sync(QKV_FULL_MASK, mt[r], 0);
-    Mt[r] = __shfl_sync(QKV_FULL_MASK, Mt[r], 0);
+#pragma unroll
+    for (int u = 0; u < kU; ++u) q[r][u].y += q[r][u].x - mt[r];
+    dMt[r] = q[r][0].y;
+    if (kU > 1) dMt[r] = max_or_nan(dMt[r], q[r][kU - 1].y);
+  }
+#pragma unroll 1
+  for (int x = width >> 1; x > 0; x >>= 1)
+#pragma unroll
+    for (int r = 0; r < R; ++r) dMt[r] = max_or_nan(dMt[r], __shfl_xor_sync(QKV_FULL_MASK, dMt[r], x));
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    dMt[r] = __shfl_sync(QKV_FULL_MASK, dMt[r], 0);
     lt[r] = 0.f;
 #pragma unroll
     for (int u = 0; u < kU; ++u) {
       lt[r] = fmaf(q[r][u].z, ex2(q[r][u].x - mt[r]), lt[r]);
-      q[r][u].w = ex2(q[r][u].y - Mt[r]);
+      q[r][u].w = ex2(q[r][u].y - dMt[r]);
     }
     o[r] = make_float4(0.f, 0.f, 0.f, 0.f);
   }
@@ -638,7 +654,7 @@ __global__ void __launch_bounds__(128) paged8_merge_kernel(Attn8Args a) {
 #pragma unroll
   for (int r = 0; r < R; ++r) {
     const int in = in_head + r;
-    if (c < D && r < rows_here) store_out8(a, s, h + in / a.G, first + in % a.G, c, o[r], mt[r], Mt[r], lt[r]);
+    if (c < D && r < rows_here) store_out8(a, s, h + in / a.G, first + in % a.G, c, o[r], dMt[r], lt[r]);
   }
 }
 

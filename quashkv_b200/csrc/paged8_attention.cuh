@@ -20,7 +20,7 @@ struct Attn8Args {
   float scale;
   void* out;
   int row_tiles, tile_rows, most_rows, n_splits; int64_t chunk;
-  float* part; float* ref;                  // [row][n_splits] sums, and their (m, M, l, -); rows as part_row8 numbers them
+  float* part; float* ref;                  // [row][n_splits] sums, and their (m, M - m, l, -); rows as part_row8 numbers them
   int few_rows;                             // sequences of no more rows (query tokens x heads of a KV head) are not this kernel's,
   int by_token;                             // most_rows: nor are those of more.  by_token: see part_row8
   int in_cluster;                           // split kernel: the splits of a row tile are one cluster
@@ -129,19 +129,19 @@ __device__ __forceinline__ void load_row8(const void* q, int dtype, int64_t at, 
   }
 }
 
-// From sums in units of 2^M to total weight l in units of 2^m: times x, then times y.  Two factors, because 2^(M - m) alone is below the normal
-// numbers (and lost) where value scales are near 2^-126, though the results are not.  0 for a row that has seen nothing.
+// From sums in units of 2^M to total weight l in units of 2^m (dM = M - m): times x, then times y.  Two factors, because 2^dM alone is below
+// the normal numbers (and lost) where value scales are near 2^-126, though the results are not.  0 for a row that has seen nothing.
 struct Unit8 { float x, y; };
-__device__ __forceinline__ Unit8 unit8(float m, float M, float l) {
+__device__ __forceinline__ Unit8 unit8(float dM, float l) {
   if (l == 0.f) return {0.f, 0.f};
-  const float half = floorf(0.5f * (M - m));
-  return {ex2(half), ex2(M - m - half) / l};
+  const float half = floorf(0.5f * dM);
+  return {ex2(half), ex2(dM - half) / l};
 }
 
-// Coordinates c .. c + 3 of output row r of KV head h: sums o in units of 2^M, total weight l in units of 2^m.  A row that has seen
+// Coordinates c .. c + 3 of output row r of KV head h: sums o in units of 2^(m + dM), total weight l in units of 2^m.  A row that has seen
 // nothing is zeros.  One rounding, to the queries' type.
-__device__ __forceinline__ void store_out8(const Attn8Args& a, const Span8& s, int h, int r, int c, float4 o, float m, float M, float l) {
-  const Unit8 f = unit8(m, M, l);                          // (M is far below m where every value was zero)
+__device__ __forceinline__ void store_out8(const Attn8Args& a, const Span8& s, int h, int r, int c, float4 o, float dM, float l) {
+  const Unit8 f = unit8(dM, l);                            // (dM is far below 0 where every value was zero)
   o.x = o.x * f.x * f.y; o.y = o.y * f.x * f.y; o.z = o.z * f.x * f.y; o.w = o.w * f.x * f.y;
   const int64_t at = s.o_row0 + static_cast<int64_t>(r / a.G) * a.o_stride[1] + static_cast<int64_t>(h * a.G + r % a.G) * a.o_stride[2] + c;
   if (a.dtype == QKV_F32) {

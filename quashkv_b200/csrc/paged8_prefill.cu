@@ -43,10 +43,13 @@ constexpr int kTok = 128, kRowsT = 128, kStages = 2, kMetaSlots = 4, kGroups = k
 // Weights reach 2^15 and the largest is at least 2^9, as in the split kernel: half of fp16's least step is 2^-34 of it, so the many small
 // weights of a long cache keep their sum.  (References that rise by 14 and a largest of 1/2 lose weights below 2^-25 of it: 2 x 4096 tokens
 // 349 us in place of 362, 8 x 1024 of 64 100 in place of 101, but weights of 2^-26 beside one came to nothing, however many.)
-constexpr float kNone = -1e30f, kSlack = 4.f, kLift = 10.f;
+constexpr float kNone = -3e38f, kSlack = 4.f, kLift = 10.f;
+// A score is at most 128 x 448 x 2^14 (below 2^30) times its factor: with factors up to this one they stay below 2^22 and references in fp32
+// are exact.  Tiles of larger ones are done with more care (`huge` below).
+constexpr float kPlainFactor = 1.f / 256.f;
 __device__ unsigned int g_prefill8_timeouts = 0;
 
-struct TileMeta { float ks[kGroups], ex[kGroups], mant[kGroups]; uint32_t bad; uint32_t pad[7]; };   // per group of 16 tokens
+struct TileMeta { float ks[kGroups], ex[kGroups], mant[kGroups]; uint32_t bad; float ks_most; uint32_t pad[6]; };   // per group of 16 tokens
 static_assert(sizeof(TileMeta) % 16 == 0, "read as 16-byte words");
 
 template <int D> struct Pf8 {
@@ -429,7 +432,8 @@ __global__ void __launch_bounds__(Pf8<D>::kThreads, 1) paged8_prefill_kernel(Att
             mt->mant[lane] = e ? (e == 255 ? vs : __uint_as_float((bits & 0x807fffffu) | 0x3f800000u)) : 0.f;
           }
           const uint32_t bad = __ballot_sync(QKV_FULL_MASK, lane < kGroups && id < 0);
-          if (lane == 0) mt->bad = bad;
+          const uint32_t most = __reduce_max_sync(QKV_FULL_MASK, lane < kGroups && ks == ks ? __float_as_uint(ks) : 0u);      // (0 or more)
+          if (lane == 0) { mt->bad = bad; mt->ks_most = __uint_as_float(most); }
           __syncwarp();
           if (lane == 0) arrive(m_full + j % kMetaSlots);
         }
@@ -462,11 +466,15 @@ __global__ void __launch_bounds__(Pf8<D>::kThreads, 1) paged8_prefill_kernel(Att
                                    : stage_queries<D, false>(a, s, h, first, r_end, q_s + t * P::kQBytes, row0);
         umma::fence_smem_to_async();
         arrive(p_ready + t);
+        // An infinity among the queries (2^115 is beyond what any number gives): the row is NaN in any case, and not `huge`.
+        if (unit > fabsf(a.scale) * (1.4426950408889634f * 0x1.8p114f)) unit = 0.f;
       }
       // last token that this row sees, relative to `begin`
       const int lim = live ? static_cast<int>(max(min(visible8(a, s, r / a.G) - begin, a.chunk), static_cast<int64_t>(0))) - 1 : -1;
       float m = kNone, M = 0.5f * kNone, l = 0.f;
-      bool ok = true;
+      // From the row's first tile on whose scores may be far from 0: products are rounded before a reference
+      // is taken from them, so that none passes it, and M is held as M - m, which stays exact where m + 1 is no number any more.
+      bool ok = true, huge = false;
       constexpr int kG = kSub / 16;
       for (int i = 0; i < n_sub; ++i) {
         const int j = i / kParts, g0 = i % kParts * kG;    // groups g0 .. of operand tile j
@@ -481,15 +489,19 @@ __global__ void __launch_bounds__(Pf8<D>::kThreads, 1) paged8_prefill_kernel(Att
         }
         auto factors = [&] {
 #pragma unroll
-          for (int g = 0; g < kG; ++g) up[g] = mt.mant[g0 + g] * ex2(fminf(m + ex[g] - M, 120.f));
+          for (int g = 0; g < kG; ++g) up[g] = mt.mant[g0 + g] * ex2(fminf((huge ? 0.f : m) + ex[g] - M, 120.f));
         };
+        if (!huge && mt.ks_most * unit > kPlainFactor) {
+          huge = true;
+          M -= m;
+        }
         factors();
         const uint32_t bad = (mt.bad >> g0) & ((1u << kG) - 1u);
         if (!(ok = wait_all(s_full + t, i & 1))) break;
         umma::fence_after_sync();
         uint32_t x[kSub / 64][64];
         const int left = lim - i * kSub;                   // tokens 0 .. left of the tile are visible
-        const bool masked = __any_sync(QKV_FULL_MASK, left < kSub - 1) || bad != 0;
+        const bool masked = __any_sync(QKV_FULL_MASK, left < kSub - 1 || huge) || bad != 0;
 #pragma unroll
         for (int hf = 0; hf < kSub / 64; ++hf) umma::tmem_ld64_issue(my + 64 * hf, x[hf]);
 #pragma unroll
@@ -510,6 +522,7 @@ __global__ void __launch_bounds__(Pf8<D>::kThreads, 1) paged8_prefill_kernel(Att
             tm = fmaxf(tm, top);
             tM = fmaxf(tM, top + ex[g]);
             f[g] = 1.f;
+            if (huge) up[g] = top;                         // (factors come anew below)
           }
         } else {
 #pragma unroll
@@ -523,9 +536,16 @@ __global__ void __launch_bounds__(Pf8<D>::kThreads, 1) paged8_prefill_kernel(Att
             tM = fmaxf(tM, v + ex[g]);
           }
         }
-        const bool rise = tm > m + kSlack || tM > M + (kLift + kSlack);
-        if (__any_sync(QKV_FULL_MASK, rise)) {             // scores of this tile are there, so the sums of the one before are
-          const float m1 = fmaxf(m, ceilf(tm)), M1 = fmaxf(M, ceilf(tM) - kLift);
+        const bool rise = tm > m + kSlack || tM > M + (kLift + kSlack) || huge;
+        if (__any_sync(QKV_FULL_MASK, rise)) {     // scores of this tile are there, so the sums of the one before are
+          const float m1 = fmaxf(m, ceilf(tm));
+          if (huge) {
+            M += m - m1;
+            tM = -INFINITY;
+#pragma unroll
+            for (int g = 0; g < kG; ++g) tM = fmaxf(tM, up[g] - m1 + ex[g]);
+          }
+          const float M1 = fmaxf(M, ceilf(tM) - kLift);
           l *= ex2(m - m1);
           const float alpha = ex2(M - M1);
           m = m1;
@@ -601,7 +621,8 @@ __global__ void __launch_bounds__(Pf8<D>::kThreads, 1) paged8_prefill_kernel(Att
       // rows of other warps' queries, too: only behind o_full, which every product that reads them and so every warp's
       // queries are in front of.  Where nothing was summed, or a wait ran out, a thread writes its row by itself.
       const int64_t slot = part_row8(a, s, seq, h, live ? r : 0) * a.n_splits + blockIdx.z;
-      const Unit8 by = unit8(m, M, l);                     // a row that has seen nothing is zeros
+      const float dM = huge ? M : M - m;
+      const Unit8 by = unit8(dM, l);                       // a row that has seen nothing is zeros
       unsigned char* rows_s = q_s + t * P::kQBytes + 32 * (warp & 3) * (2 * D);
       const bool summed = ok && n_sub > 0;                 // (the same for all of a warp)
       if (!summed && a.n_splits == 1 && live) {
@@ -651,7 +672,7 @@ __global__ void __launch_bounds__(Pf8<D>::kThreads, 1) paged8_prefill_kernel(Att
           if (r - lane + k < r_end) *(reinterpret_cast<uint4*>(static_cast<uint16_t*>(a.out) + at) + c) = y;
         }
       }
-      if (live && a.n_splits > 1) *reinterpret_cast<float4*>(a.ref + slot * 4) = make_float4(m, M, l, 0.f);
+      if (live && a.n_splits > 1) *reinterpret_cast<float4*>(a.ref + slot * 4) = make_float4(m, dM, l, 0.f);
     }
   }
   umma::fence_before_sync();
