@@ -20,9 +20,9 @@
 // that m + 1 is no number any more; there the largest score has all the weight, as it should.
 //
 // Bound by the bytes of the pages: (2 D + 8 / block_size) a token and KV head.  Measured, 32 x 8 KV heads x 32768 tokens of 128, four
-// bf16 queries a head: 365-396 us by the box, 5.4-5.9 TB/s; the schedulers' issue slots are 48 % busy, their three warps mostly wait for results of their own.
+// bf16 queries a head: 365-408 us by the box, 5.3-5.9 TB/s; the schedulers' issue slots are 48 % busy, their three warps mostly wait for results of their own.
 // fp32 queries take four MMAs in place of one, and 16 rows fill the registers (two CTAs an SM): 32 sequences of up to 16384
-// tokens, 16 rows a head: 241 us, 2.6 TB/s, bound by the latency of a warp's own chain.
+// tokens, 16 rows a head: 242 us, 2.6 TB/s, bound by the latency of a warp's own chain.
 #include <math.h>
 
 #include <cooperative_groups.h>

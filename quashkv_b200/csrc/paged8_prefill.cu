@@ -23,8 +23,8 @@
 // 4400 cycles: 2900 of softmax (two warps on a quarter of the SM, whose exponentials alone take 2048) and 1400 of tensor core
 // and hand-over.  512 columns of tensor memory are two row tiles of 128 scores and 128 sums.  At head_dim 64 they are
 // four of 64 and 64, which lets another row tile's softmax run meanwhile: 130 -> 100 us at 8 x 1024 tokens, 32 heads.
-// Measured (causal, bf16, e4m3): 2 x 4096 tokens, 32 heads of 128 over 8: 362 us, 760 TFLOP/s; 8 x 1024, 32 heads
-// of 64 over 4: 101 us, 340 TFLOP/s counted over visible pairs.
+// Measured (causal, bf16, e4m3): 2 x 4096 tokens, 32 heads of 128 over 8: 362-374 us by the box, 735-760 TFLOP/s; 8 x 1024, 32
+// heads of 64 over 4: 103 us, 334 TFLOP/s counted over visible pairs.
 // Slower at head_dim 128: score tiles of 64 tokens in two buffers each; two threads a row (490 us); rows read twice from
 // tensor memory in place of held in registers (470); arithmetic on single numbers in place of pairs (386).
 //
@@ -42,7 +42,7 @@ namespace {
 constexpr int kTok = 128, kRowsT = 128, kStages = 2, kMetaSlots = 4, kGroups = kTok / 16;
 // Weights reach 2^15 and the largest is at least 2^9, as in the split kernel: half of fp16's least step is 2^-34 of it, so the many small
 // weights of a long cache keep their sum.  (References that rise by 14 and a largest of 1/2 lose weights below 2^-25 of it: 2 x 4096 tokens
-// 349 us in place of 362, 8 x 1024 of 64 100 in place of 101, but weights of 2^-26 beside one came to nothing, however many.)
+// 349 us where this took 362, 8 x 1024 of 64 100 and 101, but weights of 2^-26 beside one came to nothing, however many.)
 constexpr float kNone = -3e38f, kSlack = 4.f, kLift = 10.f;
 // A score is at most 128 x 448 x 2^14 (below 2^30) times its factor: with factors up to this one they stay below 2^22 and references in fp32
 // are exact.  Tiles of larger ones are done with more care (`huge` below).
