@@ -131,7 +131,8 @@ template <typename T, int CODE, int D> struct Head {
     top = __reduce_max_sync(QKV_FULL_MASK, top);
     float scale = p8::scale_for<CODE>(Raw<T>::magnitude(top));
     if (at > 0) scale = (old != old || scale != scale) ? __int_as_float(0x7fc00000) : fmaxf(old, scale);
-    const float inv = scale > 0.f ? 1.f / scale : 0.f;                         // 0 for NaN: codes are zeros
+    // 0 for NaN: codes are zeros.  (A page whose own scale is below 2^-128 can only go on with zeros: these times a finite number.)
+    const float inv = scale > 0.f ? fminf(1.f / scale, 0x1.fffffep127f) : 0.f;
     if (scale > 0.f && old != scale && at > 0) {                               // raised: what the page holds moves along
       const float ratio = old / scale;
       for (int k = row; k < at && row < kRows; k += kRows) {
